@@ -57,6 +57,9 @@ def _hipcc():
 # gchain.hip keeps its MFMA accumulators in VGPRs: they are read by VALU epilogues every tile, and the
 # AGPR form costs a v_accvgpr_read per element
 PER_FILE_FLAGS = {"gchain.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# no packed fp32 arithmetic (v_pk_add / mul / fma_f32): hipcc forms it by itself from scalar code, and some of its forms have
+# given wrong results on this hardware, rarely and without an error.  (The host pass warns that it does not know the feature.)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # sources compiled as several objects (-D<macro>=0..n-1), each instantiating a part of the kernels: gemm3.hip's
 # launcher is split in four (its template instantiations are most of the build time)
 MULTI_PART = {"gemm3.hip": ("GEMM3_PART", 4)}
@@ -69,7 +72,7 @@ def build_hip(jobs: int = 4):
     hipcc = _hipcc()
     srcs = sorted((CSRC / "hip").glob("*.hip"))
     flags = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={OFFLOAD_ARCH}", "-mcode-object-version=5",
-             "-Wno-unused-result", f"-I{CSRC / 'hip'}", *_pybind_includes()]
+             *NO_PACKED_FP32, "-Wno-unused-result", f"-I{CSRC / 'hip'}", *_pybind_includes()]
     objs = []
 
     hdr_mtime = max((h.stat().st_mtime for h in (CSRC / "hip").glob("*.h")), default=0.0)
