@@ -75,4 +75,10 @@ PYBIND11_MODULE(serann_hip, m) {
           py::arg("L"), py::arg("V"), py::arg("stream"), py::arg("bf16") = 0);
     m.def("onehot", &launch_onehot);
     m.def("bin", &launch_bin);
+    m.def("tok_score_segments", &tok_score_segments);
+    m.def("tok_score", &launch_tok_score);
+    m.def("tok_score_grad", &launch_tok_score_grad);
+    m.def("tok_distill_segments", &tok_distill_segments);
+    m.def("tok_distill", &launch_tok_distill);
+    m.def("tok_distill_grad", &launch_tok_distill_grad);
 }

@@ -1,0 +1,302 @@
+// Shared by the token operators (token_score.hip, token_distill.hip): rows of logits in registers, reductions, launch shapes.
+//
+// A row is V logits x (fp32, bf16 or fp16) at temperature T; c = log2(e) / T.  With m = max x and mc = m c rounded to fp32,
+//   d_v = fma(x_v, c, -mc),  e_v = exp2(d_v),  dmax = fma(m, c, -mc)     (dmax: what the rounding of mc left, |mc| 2^-24)
+// every d_v is shifted by the same dmax, so it is taken back once a row instead of paying a subtraction an element.  The
+// elements equal to m are counted (n) and left out of the sums: of a row that is nearly sure of one token the rest
+//   S = sum_{x_v < m} e_v 2^-dmax
+// keeps its digits (1 + S would not), and ln sum = ln(n + S) is log1p(S) for n = 1.  All sums are fp32 over at most 128
+// terms a thread, then a fixed tree over lanes and waves (no atomics: the same bits on every run); the distillation loss, a
+// small difference of large terms, takes its logarithms and its K terms in fp64.
+//
+// Rows whose elements are all -inf have no distribution: S = n = 0, flagged by l2S = +inf, which makes every q_v = 0.
+// A NaN or +inf logit makes the row's sums NaN.
+#pragma once
+#include "common.h"
+#include "serann_hip.h"
+#include <stdexcept>
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 f16_t;
+
+constexpr int TOK_MAX_K = 128;        // top alternatives / teacher entries a row
+constexpr int TOK_MAX_SEG = 64;       // segments a row is split into at most
+constexpr int64_t TOK_MAX_V = 1 << 20;
+constexpr int TOK_NARROW_V = 512;     // rows of up to 64 x 8 elements: a group of 8-64 lanes a row, no LDS reduction
+
+// Rows of a [n0][n1][V] tensor with strides s0, s1 (elements) and unit stride inside a row; row r = (r / n1, r % n1)
+struct TokRows {
+    int64_t x, rows, n1, s0, s1;
+    int V;
+    float c, inv_t;       // log2(e) / T, 1 / T
+    double dinv_t;
+};
+
+template <typename T> struct TokElem;
+template <> struct TokElem<float> {
+    static constexpr int VEC = 4;
+    static constexpr uint32_t NEG_INF = 0xff800000u;
+    static __device__ __forceinline__ float get(const u32x4_t& v, int e) { return __uint_as_float(v[e]); }
+    static __device__ __forceinline__ float one(float v) { return v; }
+    static __device__ __forceinline__ u32x4_t pack(const float* f) {
+        return u32x4_t{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+    }
+    static __device__ __forceinline__ float put(float f) { return f; }
+};
+template <> struct TokElem<bf16_t> {
+    static constexpr int VEC = 8;
+    static constexpr uint32_t NEG_INF = 0xff80ff80u;
+    static __device__ __forceinline__ float get(const u32x4_t& v, int e) {
+        return __uint_as_float((e & 1) ? (v[e >> 1] & 0xffff0000u) : (v[e >> 1] << 16));
+    }
+    static __device__ __forceinline__ float one(bf16_t v) { return bf2f(v); }
+    static __device__ __forceinline__ u32x4_t pack(const float* f) {
+        return u32x4_t{f2bf2(f[0], f[1]), f2bf2(f[2], f[3]), f2bf2(f[4], f[5]), f2bf2(f[6], f[7])};
+    }
+    static __device__ __forceinline__ bf16_t put(float f) { return f2bf(f); }
+};
+template <> struct TokElem<f16_t> {
+    static constexpr int VEC = 8;
+    static constexpr uint32_t NEG_INF = 0xfc00fc00u;
+    static __device__ __forceinline__ float get(const u32x4_t& v, int e) {
+        return (float)__builtin_bit_cast(f16_t, (uint16_t)(v[e >> 1] >> ((e & 1) * 16)));
+    }
+    static __device__ __forceinline__ float one(f16_t v) { return (float)v; }
+    static __device__ __forceinline__ u32x4_t pack(const float* f) {
+        u32x4_t o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            o[i] = (uint32_t)__builtin_bit_cast(uint16_t, (f16_t)f[2 * i]) |
+                   ((uint32_t)__builtin_bit_cast(uint16_t, (f16_t)f[2 * i + 1]) << 16);
+        return o;
+    }
+    static __device__ __forceinline__ f16_t put(float f) { return (f16_t)f; }
+};
+
+// 16 bytes at any element's address: a row starts where its stride puts it (odd V), and gfx950 takes unaligned vectors
+__device__ __forceinline__ u32x4_t tok_ld16(const void* p) {
+    u32x4_t v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+__device__ __forceinline__ void tok_st16(void* p, u32x4_t v) { __builtin_memcpy(p, &v, 16); }
+
+// max without the canonicalising multiplies that fmaxf brings for signalling NaNs; a NaN operand is passed over (it comes
+// back through the sums)
+__device__ __forceinline__ float tok_max(float a, float b) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ float tok_max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float tok_exp2(float d) { return __builtin_amdgcn_exp2f(d); }
+
+template <int CTRL> __device__ __forceinline__ float tok_dpp(float v) {
+    const int i = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
+}
+template <int CTRL> __device__ __forceinline__ uint32_t tok_dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <int CTRL> __device__ __forceinline__ uint64_t tok_dpp(uint64_t v) {
+    return (uint64_t)tok_dpp<CTRL>((uint32_t)v) | ((uint64_t)tok_dpp<CTRL>((uint32_t)(v >> 32)) << 32);
+}
+template <int CTRL> __device__ __forceinline__ double tok_dpp(double v) {
+    return __builtin_bit_cast(double, tok_dpp<CTRL>(__builtin_bit_cast(uint64_t, v)));
+}
+struct TokMax { static __device__ __forceinline__ float f(float a, float b) { return tok_max(a, b); } };
+struct TokMin { static __device__ __forceinline__ float f(float a, float b) { return fminf(a, b); } };
+struct TokSum {
+    static __device__ __forceinline__ float f(float a, float b) { return a + b; }
+    static __device__ __forceinline__ double f(double a, double b) { return a + b; }
+};
+struct TokTop {
+    static __device__ __forceinline__ uint32_t f(uint32_t a, uint32_t b) { return a > b ? a : b; }
+    static __device__ __forceinline__ uint64_t f(uint64_t a, uint64_t b) { return a > b ? a : b; }
+    static __device__ __forceinline__ double f(double a, double b) { return a > b ? a : b; }
+};
+// Reduction over aligned groups of G lanes, every lane gets the result: lanes 1 and 2 apart (quad_perm), then the mirrored
+// half row and row (their quads / halves are uniform by then), then across rows of 16
+template <int G, typename OP, typename V> __device__ __forceinline__ V tok_group(V v) {
+    if constexpr (G > 1) v = OP::f(v, tok_dpp<0xB1>(v));
+    if constexpr (G > 2) v = OP::f(v, tok_dpp<0x4E>(v));
+    if constexpr (G > 4) v = OP::f(v, tok_dpp<0x141>(v));
+    if constexpr (G > 8) v = OP::f(v, tok_dpp<0x140>(v));
+    if constexpr (G > 16) v = OP::f(v, (V)__shfl_xor(v, 16, 64));
+    if constexpr (G > 32) v = OP::f(v, (V)__shfl_xor(v, 32, 64));
+    return v;
+}
+
+// (value, index) as one unsigned key, larger = ranked first: the float's bits in their order, then the lowest index.
+// +0.0 joins -0 and +0, which are equal values.
+__device__ __forceinline__ uint32_t tok_order(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float tok_unorder(uint32_t o) {
+    return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ uint64_t tok_key(float x, int i) {
+    return ((uint64_t)tok_order(x) << 32) | (uint32_t)~(uint32_t)i;
+}
+__device__ __forceinline__ int tok_key_index(uint64_t k) { return (int)~(uint32_t)k; }
+__device__ __forceinline__ float tok_key_value(uint64_t k) { return tok_unorder((uint32_t)(k >> 32)); }
+
+template <typename T> __device__ __forceinline__ const T* tok_row(const TokRows& r, int64_t row) {
+    const int64_t i0 = r.n1 == r.rows ? 0 : row / r.n1;
+    return reinterpret_cast<const T*>(r.x) + i0 * r.s0 + (row - i0 * r.n1) * r.s1;
+}
+__device__ __forceinline__ int64_t tok_int(int64_t base, int is64, int64_t i) {
+    return is64 ? reinterpret_cast<const int64_t*>(base)[i] : (int64_t) reinterpret_cast<const int32_t*>(base)[i];
+}
+
+// A row's exponents, d = fma(x, c, -mc).  Where |m| c is near overflow (a row of the type's lowest values), two different
+// logits lie so far apart that only those equal to m count: everything else gets -inf.
+struct TokRef {
+    float c, mc, dmax, meq;      // meq: the value of the elements to count (a NaN, equal to nothing, in a row of -inf)
+};
+__device__ __forceinline__ TokRef tok_ref(float m, float c) {
+    const bool none = m == -INFINITY, big = !none && fabsf(m) * c >= 1e37f;
+    TokRef r;
+    r.c = big ? 1e-30f : c;
+    r.mc = none ? 0.f : big ? INFINITY : m * c;
+    r.dmax = none || big ? 0.f : __builtin_fmaf(m, c, -r.mc);
+    r.meq = none ? NAN : m;
+    return r;
+}
+
+// ln(n + S) of a row's sums (n elements at the maximum, S over the others)
+__device__ __forceinline__ float tok_ln(float n, float S) { return n == 1.f ? log1pf(S) : logf(n + S); }
+
+// A segment of a row in registers: NV 16-byte vectors a thread and one of the < VEC last elements of the row.  Vector
+// i * NT + tid of the segment is r[i]; vm[i] its maximum.
+template <typename T, int NT, int NV> struct TokSeg {
+    static constexpr int VEC = TokElem<T>::VEC;
+    u32x4_t r[NV];
+    float vm[NV];
+    float xt;
+    int nv, tail0;      // full vectors of the segment; first element (from the segment's start) behind them
+    __device__ __forceinline__ void load(const T* __restrict__ x, int nvec, int ntail) {
+        const int tid = threadIdx.x;
+        nv = nvec;
+        tail0 = nvec * VEC;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t u = (uint32_t)(i * NT + tid);
+            r[i] = u32x4_t{TokElem<T>::NEG_INF, TokElem<T>::NEG_INF, TokElem<T>::NEG_INF, TokElem<T>::NEG_INF};
+            if (u < (uint32_t)nvec) r[i] = tok_ld16(reinterpret_cast<const char*>(x) + (size_t)(u * 16u));
+        }
+        xt = -INFINITY;
+        if (tid < ntail) xt = TokElem<T>::one(x[tail0 + tid]);
+    }
+    __device__ __forceinline__ float max_of() {
+        float m = xt;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float a = tok_max3(TokElem<T>::get(r[i], 0), TokElem<T>::get(r[i], 1), TokElem<T>::get(r[i], 2));
+            if constexpr (VEC == 4) {
+                a = tok_max(a, TokElem<T>::get(r[i], 3));
+            } else {
+                a = tok_max3(a, TokElem<T>::get(r[i], 3), TokElem<T>::get(r[i], 4));
+                a = tok_max3(a, TokElem<T>::get(r[i], 5), TokElem<T>::get(r[i], 6));
+                a = tok_max(a, TokElem<T>::get(r[i], 7));
+            }
+            vm[i] = a;
+            m = tok_max(m, a);
+        }
+        forget();
+        return m;
+    }
+    // The next pass unpacks the elements again: kept from pass to pass they would take a register each, not half of one
+    __device__ __forceinline__ void forget() {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) asm("" : "+v"(r[i]));
+    }
+};
+
+// Narrow rows: the 8 elements from e0 on that a lane holds, -inf behind the row's end
+template <typename T> __device__ __forceinline__ void tok_narrow_load(const T* x, int V, int e0, bool live, float* f) {
+    constexpr int VEC = TokElem<T>::VEC;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = -INFINITY;
+    if (!live) return;
+    if (e0 + 8 <= V) {
+#pragma unroll
+        for (int h = 0; h < 8 / VEC; ++h) {
+            const u32x4_t v = tok_ld16(x + e0 + h * VEC);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) f[h * VEC + e] = TokElem<T>::get(v, e);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e0 + e < V) f[e] = TokElem<T>::one(x[e0 + e]);
+    }
+}
+template <typename T> __device__ __forceinline__ void tok_narrow_store(T* o, int V, int e0, const float* f) {
+    constexpr int VEC = TokElem<T>::VEC;
+    if (e0 + 8 <= V) {
+#pragma unroll
+        for (int h = 0; h < 8 / VEC; ++h) tok_st16(o + e0 + h * VEC, TokElem<T>::pack(f + h * VEC));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e0 + e < V) o[e0 + e] = TokElem<T>::put(f[e]);
+    }
+}
+
+// How a row is cut: NT threads x NV vectors a segment.  Whole rows of up to 4096 vectors (64 KB: 16 of 64 registers' vectors
+// a thread) stay one block; longer ones, and rows too few to fill 256 CUs, are cut and joined by a second, small launch.
+struct TokPlan {
+    int nt, nv, nseg, segvec;
+};
+inline TokPlan tok_plan(int64_t V, int esize, int64_t rows, int max_vec, bool may_split) {
+    const int64_t vec = 16 / esize, nvec = V / vec;
+    int64_t nseg = (nvec + max_vec - 1) / max_vec;
+    if (nseg < 1) nseg = 1;
+    if (may_split && nvec > 1024) {
+        int64_t want = (512 + rows - 1) / rows;             // two blocks a CU
+        if (want > nvec / 512) want = nvec / 512;           // at least 8 KB a block
+        if (nseg < want) nseg = want;
+    }
+    if (nseg > TOK_MAX_SEG) nseg = TOK_MAX_SEG;
+    const int64_t segvec = (nvec + nseg - 1) / nseg;
+    nseg = segvec ? (nvec + segvec - 1) / segvec : 1;        // no empty segment
+    TokPlan p{0, 0, (int)nseg, (int)segvec};
+    static const int shapes[][2] = {{64, 2}, {64, 4}, {64, 8}, {256, 4}, {256, 8}, {256, 16}, {512, 16}};
+    for (auto& s : shapes)
+        if ((int64_t)s[0] * s[1] >= segvec) {
+            p.nt = s[0];
+            p.nv = s[1];
+            break;
+        }
+    return p;
+}
+// blocks of nt threads for `units` of work: HIP counts threads of a launch in 32 bits, longer work is looped over
+inline unsigned tok_blocks(int64_t units, int nt) {
+    const int64_t cap = ((int64_t)1 << 31) / nt;
+    return (unsigned)(units < cap ? units : cap);
+}
+inline TokRows tok_rows_of(uint64_t x, int64_t rows, int64_t n1, int64_t s0, int64_t s1, int64_t V, double temperature) {
+    if (rows < 0 || V < 1 || V > TOK_MAX_V) throw std::runtime_error("token operators: vocabulary must be in [1, 2^20]");
+    if (n1 < 1 || (rows && rows % n1)) throw std::runtime_error("token operators: rows must be a multiple of n1");
+    if (!(temperature > 0)) throw std::runtime_error("token operators: temperature must be positive");
+    TokRows r;
+    r.x = (int64_t)x;
+    r.rows = rows;
+    r.n1 = n1;
+    r.s0 = s0;
+    r.s1 = s1;
+    r.V = (int)V;
+    r.c = (float)(1.4426950408889634 / temperature);
+    r.inv_t = (float)(1.0 / temperature);
+    r.dinv_t = 1.0 / temperature;
+    return r;
+}
+inline int tok_esize(int dtype) { return dtype == 0 ? 4 : 2; }
+// lanes a narrow row takes: 8 elements a lane
+inline int tok_narrow_lanes(int64_t V) { return V <= 64 ? 8 : V <= 128 ? 16 : V <= 256 ? 32 : 64; }

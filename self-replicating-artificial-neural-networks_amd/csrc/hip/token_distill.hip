@@ -1,0 +1,708 @@
+// Distillation from a teacher's top tokens: the loss of a row of student logits x and its gradient.
+//
+// The teacher gives K pairs (id i_k, log-probability t_k) a row; pairs whose id is outside [0, V) are absent, pairs of the
+// same id add up.  With z = x / T, q = softmax(z):
+//   drop  : p_k = exp(t_k) / sum_k exp(t_k)                                   loss = w T^2 sum_k p_k (ln p_k - ln q_ik)
+//   bucket: p_k = exp(t_k), p_0 = max(0, 1 - sum p_k), q_0 = sum_{v not listed} q_v,
+//           loss = w T^2 ( sum_k p_k (ln p_k - ln q_ik) + p_0 (ln p_0 - ln q_0) )       (no bucket where q_0 = 0)
+//   gradient, with P = sum p_k, A = P + p_0, B = A - p_0 / q_0 (drop: A = B = P):
+//           dx_v = w T ( A q_v - p_v ) for listed v,   w T B q_v for the others
+// A row of weight 0 is not read: loss and gradient 0.
+//
+// The loss of a good student is a small difference of large terms (its digits go with the rounding of ln sum alone), so a
+// row's sums are fp32 but its logarithms and K terms fp64: K + 3 transcendentals a row, next to V fp32 ones.
+//
+// One pass (tok_distill_kernel, GRAD): a block holds the row in registers, so the gradient needs no second read of HBM:
+// 2 V elements moved a row, which is the floor.  Listed tokens are marked in an LDS bitmap (one byte a 16-bit vector), so
+// q_0 is summed over the others directly and not as 1 - sum.  Rows too long for a block's registers, and the autograd
+// form, whose gradient comes later, take the statistics first (joined over segments where a row is cut) and the gradient in
+// a second launch.
+#include "token.h"
+
+constexpr int DIST_MAX_K = 256;
+
+struct DistArgs {
+    TokRows r;
+    int64_t ids;
+    const float *t, *w;
+    int id64, K, bucket;
+    int nseg, segvec;
+    float T;
+    float* loss;
+    void* dx;             // [rows][V], one-pass form
+    float4* stat;         // (m, log2 sum, A, B) for the gradient launch
+    float* pk;            // [rows][K]: the entry's p (its first occurrence carries the sum), -1: skip
+    float4* part;         // nseg > 1: (m, n, S, -) of each segment; bucket: over unlisted elements, m over all
+};
+
+// The K entries of a row in LDS: id (-1: absent), the student's logit there, p
+struct DistEntries {
+    int id[DIST_MAX_K];
+    float x[DIST_MAX_K], t[DIST_MAX_K], p[DIST_MAX_K];
+};
+struct DistRow {
+    float m, l2S, A, B;
+};
+
+__device__ __forceinline__ double group_sum64(double v) { return tok_group<64, TokSum>(v); }
+// LDS writes of this wave's lanes before its later reads (one wave: in order in hardware, so a compiler fence)
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The first wave's work on a row: p, the loss, and the gradient's factors.  n, S: the sums relative to m (tok_ln) over all
+// elements, or in bucket mode over the unlisted ones.  dup: some id may occur twice.
+__device__ __forceinline__ DistRow dist_epilogue(const DistArgs& a, DistEntries& E, int64_t row, float w, float m, float n,
+                                                 float S, bool dup, int lane) {
+    const int K = a.K;
+    // teacher: drop mode normalises over the entries that are there
+    double shift = 0.0;
+    if (!a.bucket) {
+        float tm = -INFINITY;
+        for (int j = lane; j < K; j += 64)
+            if (E.id[j] >= 0) tm = tok_max(tm, E.t[j]);
+        tm = tok_group<64, TokMax>(tm);
+        double tot = 0.0;
+        if (tm > -INFINITY) {
+            for (int j = lane; j < K; j += 64)
+                if (E.id[j] >= 0) tot += exp((double)E.t[j] - (double)tm);
+            tot = group_sum64(tot);
+            shift = (double)tm + log(tot);
+        }
+    }
+    double P = 0.0;
+    for (int j = lane; j < K; j += 64) {
+        const double p = E.id[j] < 0 ? 0.0 : exp((double)E.t[j] - shift);
+        E.p[j] = (float)p;
+        P += p;
+    }
+    P = group_sum64(P);
+    wave_fence();
+    // ids that occur again: the first occurrence carries the gradient's sum, the others none
+    float psum[DIST_MAX_K / 64];
+#pragma unroll
+    for (int s = 0; s < DIST_MAX_K / 64; ++s) {
+        const int j = s * 64 + lane;
+        psum[s] = -1.f;
+        if (j < K && E.id[j] >= 0) {
+            psum[s] = E.p[j];
+            if (dup) {
+                float sum = 0.f;
+                bool first = true;
+                for (int i = 0; i < K; ++i)
+                    if (E.id[i] == E.id[j]) {
+                        if (i < j) first = false;
+                        sum += E.p[i];
+                    }
+                psum[s] = first ? sum : -1.f;
+            }
+        }
+    }
+    // sums over the vocabulary
+    double nl = 0.0, Sl = 0.0;
+    if (a.bucket) {
+#pragma unroll
+        for (int s = 0; s < DIST_MAX_K / 64; ++s) {
+            const int j = s * 64 + lane;
+            if (j < K && !(psum[s] < 0.f)) {
+                if (E.x[j] == m) nl += m > -INFINITY ? 1.0 : 0.0;
+                else if (m > -INFINITY) Sl += exp(((double)E.x[j] - (double)m) * a.r.dinv_t);
+            }
+        }
+        nl = group_sum64(nl);
+        Sl = group_sum64(Sl);
+    }
+    const double rest = (double)n + (double)S, listed = nl + Sl;
+    double sum = rest + listed;
+    if (m == INFINITY) sum = (double)NAN;
+    const bool none = sum == 0.0;
+    const double lnS = none ? 0.0 : log(sum);
+    // the loss
+    double kl = 0.0;
+    for (int j = lane; j < K; j += 64) {
+        if (E.id[j] < 0) continue;
+        const double lp = (double)E.t[j] - shift, p = exp(lp);
+        if (p != 0.0) {
+            const double lq = none ? -(double)INFINITY : ((double)E.x[j] - (double)m) * a.r.dinv_t - lnS;
+            kl += p * (lp - lq);
+        }
+    }
+    kl = group_sum64(kl);
+    double A = P, B = P;
+    if (a.bucket) {
+        const double p0 = rest == 0.0 ? 0.0 : 1.0 - P;
+        if (p0 > 0.0) {
+            const double lq0 = listed < rest ? log1p(-listed / sum) : log(rest / sum);
+            kl += p0 * (log(p0) - lq0);
+            A = P + p0;
+            B = A - p0 * (sum / rest);
+        }
+    }
+    DistRow d;
+    d.m = none ? 0.f : m;
+    d.l2S = none ? INFINITY : (float)(lnS * 1.4426950408889634);
+    d.A = (float)A;
+    d.B = (float)B;
+    wave_fence();
+#pragma unroll
+    for (int s = 0; s < DIST_MAX_K / 64; ++s) {
+        const int j = s * 64 + lane;
+        if (j < K) E.p[j] = none ? -1.f : psum[s];
+    }
+    if (lane == 0) {
+        a.loss[row] = (float)((double)w * (double)a.T * (double)a.T * kl);
+        if (a.stat) a.stat[row] = make_float4(d.m, d.l2S, d.A, d.B);
+    }
+    if (a.pk)
+        for (int j = lane; j < K; j += 64) a.pk[row * K + j] = E.p[j];
+    return d;
+}
+
+__device__ __forceinline__ float dist_q(const DistRow& d, float c, float x) {
+    return tok_exp2(__builtin_fmaf(x - d.m, c, -d.l2S));
+}
+
+template <typename T> __device__ __forceinline__ void dist_load_entry(const DistArgs& a, DistEntries& E, int64_t row, const T* x,
+                                                                      int j) {
+    int64_t id = tok_int(a.ids, a.id64, row * a.K + j);
+    const bool in = (uint64_t)id < (uint64_t)a.r.V;
+    E.id[j] = in ? (int)id : -1;
+    E.t[j] = a.t[row * a.K + j];
+    E.x[j] = in ? TokElem<T>::one(x[id]) : 0.f;
+}
+
+template <typename T, int NT, int NV, bool GRAD>
+__global__ __launch_bounds__(NT) void tok_distill_kernel(DistArgs a) {
+    constexpr int VEC = TokElem<T>::VEC, NW = NT / 64;
+    constexpr int WORDS = NT * NV * VEC / 32 + 1;
+    __shared__ DistEntries E;
+    __shared__ uint32_t bits[WORDS];
+    __shared__ float red[NW][3];
+    __shared__ int dup;
+    __shared__ DistRow rowd;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int nvec_row = a.r.V / VEC, ntail_row = a.r.V - nvec_row * VEC;
+    const int64_t units = a.r.rows * a.nseg;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int64_t row = a.nseg == 1 ? u : u / a.nseg;
+        const int seg = (int)(u - row * a.nseg);
+        const float w = a.w ? a.w[row] : 1.f;
+        T* o = reinterpret_cast<T*>(a.dx) + row * a.r.V;
+        if (w == 0.f) {
+            if (a.nseg == 1 && tid == 0) {
+                a.loss[row] = 0.f;
+                if (a.stat) a.stat[row] = make_float4(0.f, INFINITY, 0.f, 0.f);
+            }
+            if constexpr (GRAD) {
+                for (int v = tid; v < nvec_row; v += NT) tok_st16(o + (int64_t)v * VEC, u32x4_t{0, 0, 0, 0});
+                if (tid < ntail_row) o[nvec_row * VEC + tid] = TokElem<T>::put(0.f);
+            }
+            continue;
+        }
+        const T* x = tok_row<T>(a.r, row);
+        const int v0 = seg * a.segvec;
+        const int nv = min(a.segvec, nvec_row - v0);
+        const int ntail = seg == a.nseg - 1 ? ntail_row : 0;
+        TokSeg<T, NT, NV> s;
+        s.load(x + (int64_t)v0 * VEC, nv, ntail);
+        const int e0 = v0 * VEC, len = nv * VEC + ntail;
+        for (int i = tid; i < (len + 31) / 32; i += NT) bits[i] = 0;
+        if (tid == 0) dup = 0;
+        for (int j = tid; j < a.K; j += NT) dist_load_entry<T>(a, E, row, x, j);
+        __syncthreads();
+        // mark this segment's listed tokens; a bit found set already means an id that occurs twice
+        for (int j = tid; j < a.K; j += NT) {
+            const int id = E.id[j] - e0;
+            if (E.id[j] >= 0 && id >= 0 && id < len) {
+                const uint32_t bit = 1u << (id & 31);
+                if (atomicOr(&bits[id >> 5], bit) & bit) dup = 1;
+            }
+        }
+        const float wm = tok_group<64, TokMax>(s.max_of());
+        if (lane == 0) red[wave][0] = wm;
+        __syncthreads();
+        float m = red[0][0];
+#pragma unroll
+        for (int k = 1; k < NW; ++k) m = tok_max(m, red[k][0]);
+        const TokRef ref = tok_ref(m, a.r.c);
+        const float meq = ref.meq, mc = ref.mc, c = ref.c;
+        float S = 0.f, n = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (i * NT < nv) {
+                float cs = 0.f;
+                uint32_t skip = 0;                           // listed elements of this vector (bucket mode)
+                if (a.bucket && i * NT + tid < nv) {
+                    const int at = i * NT + tid;
+                    const uint8_t by = reinterpret_cast<const uint8_t*>(bits)[VEC == 8 ? at : at >> 1];
+                    skip = VEC == 8 ? by : (by >> ((at & 1) * 4)) & 15u;
+                }
+                if (s.vm[i] == meq || skip) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float xv = TokElem<T>::get(s.r[i], e);
+                        const bool is = xv == meq, out = (skip >> e) & 1;
+                        cs += is || out ? 0.f : tok_exp2(__builtin_fmaf(xv, c, -mc));
+                        n += is && !out ? 1.f : 0.f;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) cs += tok_exp2(__builtin_fmaf(TokElem<T>::get(s.r[i], e), c, -mc));
+                }
+                S += cs;
+            }
+        }
+        if (tid < ntail) {
+            const int at = nv * VEC + tid;
+            const bool is = s.xt == meq, out = a.bucket && ((bits[at >> 5] >> (at & 31)) & 1);
+            S += is || out ? 0.f : tok_exp2(__builtin_fmaf(s.xt, c, -mc));
+            n += is && !out ? 1.f : 0.f;
+        }
+        S = tok_group<64, TokSum>(S);
+        n = tok_group<64, TokSum>(n);
+        if (lane == 0) {
+            red[wave][1] = S;
+            red[wave][2] = n;
+        }
+        __syncthreads();
+        if (wave == 0) {
+            S = red[0][1];
+            n = red[0][2];
+#pragma unroll
+            for (int k = 1; k < NW; ++k) {
+                S += red[k][1];
+                n += red[k][2];
+            }
+            S *= tok_exp2(-ref.dmax);
+            if (a.nseg > 1) {
+                if (lane == 0) a.part[u] = make_float4(m, n, S, 0.f);
+            } else {
+                const DistRow d = dist_epilogue(a, E, row, w, m, n, S, dup != 0, lane);
+                if (lane == 0) rowd = d;
+            }
+        }
+        __syncthreads();
+        if constexpr (GRAD) {
+            s.forget();
+            const DistRow d = rowd;
+            const float f = w * a.T, fB = f * d.B;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (i * NT + tid < nv) {
+                    float g[VEC];
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) g[e] = fB * dist_q(d, a.r.c, TokElem<T>::get(s.r[i], e));
+                    tok_st16(o + (int64_t)(i * NT + tid) * VEC, TokElem<T>::pack(g));
+                }
+            }
+            if (tid < ntail) o[nv * VEC + tid] = TokElem<T>::put(fB * dist_q(d, a.r.c, s.xt));
+            __syncthreads();                                 // the listed tokens' stores follow the row's
+            for (int j = tid; j < a.K; j += NT) {
+                const float p = E.p[j];
+                if (E.id[j] >= 0 && p >= 0.f) o[E.id[j]] = TokElem<T>::put(f * (d.A * dist_q(d, a.r.c, E.x[j]) - p));
+            }
+            __syncthreads();                                 // E is used again by the next row
+        }
+    }
+}
+
+// Joins the segments of a row: one wave a row
+template <typename T> __global__ __launch_bounds__(64) void tok_distill_join_kernel(DistArgs a) {
+    __shared__ DistEntries E;
+    const int lane = threadIdx.x;
+    for (int64_t row = blockIdx.x; row < a.r.rows; row += gridDim.x) {
+        const float w = a.w ? a.w[row] : 1.f;
+        if (w == 0.f) {
+            if (lane == 0) {
+                a.loss[row] = 0.f;
+                if (a.stat) a.stat[row] = make_float4(0.f, INFINITY, 0.f, 0.f);
+            }
+            continue;
+        }
+        const T* x = tok_row<T>(a.r, row);
+        for (int j = lane; j < a.K; j += 64) dist_load_entry<T>(a, E, row, x, j);
+        const float4* part = a.part + row * a.nseg;
+        float m = -INFINITY;
+        for (int s = 0; s < a.nseg; ++s) m = tok_max(m, part[s].x);
+        float S = 0.f, n = 0.f;
+        for (int s = 0; s < a.nseg; ++s) {
+            const float4 p = part[s];
+            if (p.x == m) {
+                n += p.y;
+                S += p.z;
+            } else if (p.x > -INFINITY) {
+                S += (p.y + p.z) * tok_exp2((p.x - m) * a.r.c);
+            } else {
+                S += p.z;
+            }
+        }
+        __syncthreads();
+        dist_epilogue(a, E, row, w, m, n, S, true, lane);
+        __syncthreads();
+    }
+}
+
+// ---- narrow rows: G lanes a row, 8 elements a lane ------------------------------------------------------------------------
+// p of the listed tokens goes through LDS (one word an element, NOT_LISTED where none): the lane that owns the element picks
+// it up for the sums and the gradient.
+constexpr uint32_t NOT_LISTED = 0xffffffffu;
+
+template <typename T, int G, bool GRAD>
+__global__ __launch_bounds__(256) void tok_distill_narrow_kernel(DistArgs a) {
+    constexpr int RB = 256 / G;
+    __shared__ uint32_t buf[256 * 8];
+    const int gl = threadIdx.x & (G - 1), gr = threadIdx.x / G;
+    uint32_t* mine = buf + gr * G * 8;
+    const int V = a.r.V, K = a.K;
+    for (int64_t r0 = (int64_t)blockIdx.x * RB; r0 < a.r.rows; r0 += (int64_t)gridDim.x * RB) {
+        const int64_t row = r0 + gr;
+        const bool there = row < a.r.rows;
+        const float w = there ? (a.w ? a.w[row] : 1.f) : 0.f;
+        const bool live = there && w != 0.f;
+        const T* x = live ? tok_row<T>(a.r, row) : nullptr;
+        float f[8];
+        tok_narrow_load<T>(x, V, gl * 8, live, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mine[gl * 8 + e] = NOT_LISTED;
+        __syncthreads();
+        bool twice = false;
+        float tm = -INFINITY;
+        if (live)
+            for (int j = gl; j < K; j += G) {
+                const int64_t id = tok_int(a.ids, a.id64, row * K + j);
+                if ((uint64_t)id < (uint64_t)V) {
+                    twice |= atomicExch(&mine[id], 0u) != NOT_LISTED;
+                    tm = tok_max(tm, a.t[row * K + j]);
+                }
+            }
+        __syncthreads();
+        float m = tok_max(tok_max3(tok_max3(f[0], f[1], f[2]), f[3], f[4]), tok_max3(f[5], f[6], f[7]));
+        m = tok_group<G, TokMax>(m);
+        const TokRef ref = tok_ref(m, a.r.c);
+        const float meq = ref.meq, mc = ref.mc, c = ref.c;
+        float S = 0.f, n = 0.f, Sl = 0.f, nl = 0.f;          // unlisted, listed (drop mode needs their sum alone)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool is = f[e] == meq, li = mine[gl * 8 + e] != NOT_LISTED;
+            const float ev = is ? 0.f : tok_exp2(__builtin_fmaf(f[e], c, -mc));
+            S += li ? 0.f : ev;
+            Sl += li ? ev : 0.f;
+            n += is && !li ? 1.f : 0.f;
+            nl += is && li ? 1.f : 0.f;
+        }
+        S = tok_group<G, TokSum>(S);
+        Sl = tok_group<G, TokSum>(Sl);
+        n = tok_group<G, TokSum>(n);
+        nl = tok_group<G, TokSum>(nl);
+        const double sc = (double)tok_exp2(-ref.dmax);
+        const double rest = (double)n + (double)S * sc, listed = (double)nl + (double)Sl * sc;
+        double sum = rest + listed;
+        if (m == INFINITY) sum = (double)NAN;
+        const bool none = sum == 0.0;
+        const double lnS = none ? 0.0 : log(sum);
+        double shift = 0.0;
+        if (!a.bucket) {
+            tm = tok_group<G, TokMax>(tm);
+            double tot = 0.0;
+            if (live && tm > -INFINITY)
+                for (int j = gl; j < K; j += G) {
+                    const int64_t id = tok_int(a.ids, a.id64, row * K + j);
+                    if ((uint64_t)id < (uint64_t)V) tot += exp((double)a.t[row * K + j] - (double)tm);
+                }
+            tot = tok_group<G, TokSum>(tot);
+            if (tm > -INFINITY) shift = (double)tm + log(tot);
+        }
+        const bool dup = __ballot(twice) != 0;               // any row of this wave
+        __syncthreads();                                     // the marks have been read
+        double P = 0.0, kl = 0.0;
+        if (live)
+            for (int j = gl; j < K; j += G) {
+                const int64_t id = tok_int(a.ids, a.id64, row * K + j);
+                if ((uint64_t)id >= (uint64_t)V) continue;
+                const double lp = (double)a.t[row * K + j] - shift, p = exp(lp);
+                P += p;
+                if (p != 0.0) {
+                    const double xv = (double)TokElem<T>::one(x[id]);
+                    kl += p * (lp - (none ? -(double)INFINITY : (xv - (double)m) * a.r.dinv_t - lnS));
+                }
+                float ps = (float)p;
+                bool first = true;
+                if (dup) {
+                    ps = 0.f;
+                    for (int i = 0; i < K; ++i)
+                        if (tok_int(a.ids, a.id64, row * K + i) == id) {
+                            if (i < j) first = false;
+                            ps += (float)exp((double)a.t[row * K + i] - shift);
+                        }
+                }
+                if (first) mine[id] = __float_as_uint(ps);
+                if (a.pk) a.pk[row * K + j] = first && !none ? ps : -1.f;
+            }
+        P = tok_group<G, TokSum>(P);
+        kl = tok_group<G, TokSum>(kl);
+        double A = P, B = P;
+        if (a.bucket) {
+            const double p0 = rest == 0.0 ? 0.0 : 1.0 - P;
+            if (p0 > 0.0) {
+                const double lq0 = listed < rest ? log1p(-listed / sum) : log(rest / sum);
+                kl += p0 * (log(p0) - lq0);
+                A = P + p0;
+                B = A - p0 * (sum / rest);
+            }
+        }
+        DistRow d;
+        d.m = none ? 0.f : m;
+        d.l2S = none ? INFINITY : (float)(lnS * 1.4426950408889634);
+        d.A = (float)A;
+        d.B = (float)B;
+        if (there && gl == 0) {
+            a.loss[row] = live ? (float)((double)w * (double)a.T * (double)a.T * kl) : 0.f;
+            if (a.stat) a.stat[row] = live ? make_float4(d.m, d.l2S, d.A, d.B) : make_float4(0.f, INFINITY, 0.f, 0.f);
+        }
+        __syncthreads();
+        if constexpr (GRAD) {
+            if (there && gl * 8 < V) {
+                const float fw = w * a.T;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t pb = mine[gl * 8 + e];
+                    const float q = dist_q(d, a.r.c, f[e]);
+                    const float g = pb == NOT_LISTED ? d.B * q : none ? 0.f : __builtin_fmaf(d.A, q, -__uint_as_float(pb));
+                    f[e] = live ? fw * g : 0.f;
+                }
+                tok_narrow_store<T>(reinterpret_cast<T*>(a.dx) + row * V, V, gl * 8, f);
+            }
+        }
+        __syncthreads();                                     // the buffer is used again by the next rows
+    }
+}
+
+// ---- gradient from the saved statistics ------------------------------------------------------------------------------------
+struct DistGradArgs {
+    TokRows r;
+    int64_t ids;
+    int id64, K, chunks;
+    float T;
+    const float *w, *g, *pk;     // g: the gradient of each row's loss
+    const float4* stat;
+    void* dx;
+};
+
+template <typename T> __global__ __launch_bounds__(256) void tok_distill_grad_kernel(DistGradArgs a) {
+    constexpr int VEC = TokElem<T>::VEC, U = 4;
+    const int tid = threadIdx.x;
+    const int nvec = a.r.V / VEC, ntail = a.r.V - nvec * VEC;
+    const int64_t units = a.r.rows * a.chunks;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int64_t row = u / a.chunks;
+        const int ch = (int)(u - row * a.chunks);
+        const float w = a.w ? a.w[row] : 1.f;
+        T* o = reinterpret_cast<T*>(a.dx) + row * a.r.V;
+        const T* x = tok_row<T>(a.r, row);
+        const int b0 = ch * 256 * U;
+        const bool live = w != 0.f;
+        const float4 st = live ? a.stat[row] : make_float4(0.f, INFINITY, 0.f, 0.f);
+        const DistRow d{st.x, st.y, st.z, st.w};
+        const float f = live ? w * a.T * (a.g ? a.g[row] : 1.f) : 0.f, fB = f * d.B;
+        u32x4_t r[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int v = b0 + i * 256 + tid;
+            r[i] = u32x4_t{0, 0, 0, 0};
+            if (live && v < nvec) r[i] = tok_ld16(x + (int64_t)v * VEC);
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int v = b0 + i * 256 + tid;
+            if (v < nvec) {
+                float g[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) g[e] = live ? fB * dist_q(d, a.r.c, TokElem<T>::get(r[i], e)) : 0.f;
+                tok_st16(o + (int64_t)v * VEC, TokElem<T>::pack(g));
+            }
+        }
+        const bool last = ch == a.chunks - 1;
+        if (last && tid < ntail) {
+            const int e = nvec * VEC + tid;
+            o[e] = TokElem<T>::put(live ? fB * dist_q(d, a.r.c, TokElem<T>::one(x[e])) : 0.f);
+        }
+        __syncthreads();                                     // the listed tokens' stores follow the block's own
+        if (live) {
+            const int64_t lo = (int64_t)b0 * VEC, hi = last ? a.r.V : lo + 256 * U * VEC;
+            for (int j = tid; j < a.K; j += 256) {
+                const int64_t id = tok_int(a.ids, a.id64, row * a.K + j);
+                const float p = a.pk[row * a.K + j];
+                if (id >= lo && id < hi && p >= 0.f)
+                    o[id] = TokElem<T>::put(f * (d.A * dist_q(d, a.r.c, TokElem<T>::one(x[id])) - p));
+            }
+        }
+    }
+}
+
+template <typename T, int G> __global__ __launch_bounds__(256) void tok_distill_grad_narrow_kernel(DistGradArgs a) {
+    constexpr int RB = 256 / G;
+    __shared__ uint32_t buf[256 * 8];
+    const int gl = threadIdx.x & (G - 1), gr = threadIdx.x / G;
+    uint32_t* mine = buf + gr * G * 8;
+    const int V = a.r.V, K = a.K;
+    for (int64_t r0 = (int64_t)blockIdx.x * RB; r0 < a.r.rows; r0 += (int64_t)gridDim.x * RB) {
+        const int64_t row = r0 + gr;
+        const bool there = row < a.r.rows;
+        const float w = there ? (a.w ? a.w[row] : 1.f) : 0.f;
+        const bool live = there && w != 0.f;
+        float f[8];
+        tok_narrow_load<T>(live ? tok_row<T>(a.r, row) : nullptr, V, gl * 8, live, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mine[gl * 8 + e] = NOT_LISTED;
+        __syncthreads();
+        if (live)
+            for (int j = gl; j < K; j += G) {
+                const int64_t id = tok_int(a.ids, a.id64, row * K + j);
+                const float p = a.pk[row * K + j];
+                if ((uint64_t)id < (uint64_t)V && p >= 0.f) mine[id] = __float_as_uint(p);
+            }
+        __syncthreads();
+        if (there && gl * 8 < V) {
+            const float4 st = live ? a.stat[row] : make_float4(0.f, INFINITY, 0.f, 0.f);
+            const DistRow d{st.x, st.y, st.z, st.w};
+            const float fw = live ? w * a.T * (a.g ? a.g[row] : 1.f) : 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t pb = mine[gl * 8 + e];
+                const float q = dist_q(d, a.r.c, f[e]);
+                const float g = pb == NOT_LISTED ? d.B * q : __builtin_fmaf(d.A, q, -__uint_as_float(pb));
+                f[e] = live ? fw * g : 0.f;
+            }
+            tok_narrow_store<T>(reinterpret_cast<T*>(a.dx) + row * V, V, gl * 8, f);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- launchers -------------------------------------------------------------------------------------------------------------
+// One pass (loss and gradient from one read) for rows of up to 8192 vectors (512 threads x 16)
+constexpr int DIST_ONE_PASS_VEC = 8192;
+
+static TokPlan dist_plan(int64_t V, int dtype, int64_t rows) { return tok_plan(V, tok_esize(dtype), rows, 4096, true); }
+static bool dist_one_pass(int64_t V, int dtype) { return V / (16 / tok_esize(dtype)) <= DIST_ONE_PASS_VEC; }
+
+// Workspace of a call: segments a row is cut into (16 bytes each when more than one); 0: the one-pass form (with a gradient),
+// which needs no workspace, stat or pk
+int64_t tok_distill_segments(int64_t V, int dtype, int64_t rows, int grad) {
+    if (V <= TOK_NARROW_V || rows <= 0) return grad ? 0 : 1;
+    if (grad && dist_one_pass(V, dtype)) return 0;
+    return dist_plan(V, dtype, rows).nseg;
+}
+
+template <typename T, bool GRAD> static void distill_wide(const DistArgs& a, const TokPlan& p, hipStream_t s) {
+    const dim3 grid(tok_blocks(a.r.rows * p.nseg, p.nt)), blk(p.nt);
+    if (p.nt == 64 && p.nv == 2) hipLaunchKernelGGL((tok_distill_kernel<T, 64, 2, GRAD>), grid, blk, 0, s, a);
+    else if (p.nt == 64 && p.nv == 4) hipLaunchKernelGGL((tok_distill_kernel<T, 64, 4, GRAD>), grid, blk, 0, s, a);
+    else if (p.nt == 64) hipLaunchKernelGGL((tok_distill_kernel<T, 64, 8, GRAD>), grid, blk, 0, s, a);
+    else if (p.nv == 4) hipLaunchKernelGGL((tok_distill_kernel<T, 256, 4, GRAD>), grid, blk, 0, s, a);
+    else if (p.nv == 8) hipLaunchKernelGGL((tok_distill_kernel<T, 256, 8, GRAD>), grid, blk, 0, s, a);
+    else if (p.nt == 256) hipLaunchKernelGGL((tok_distill_kernel<T, 256, 16, GRAD>), grid, blk, 0, s, a);
+    else if constexpr (GRAD) hipLaunchKernelGGL((tok_distill_kernel<T, 512, 16, GRAD>), grid, blk, 0, s, a);
+}
+template <typename T, bool GRAD> static void distill_narrow(const DistArgs& a, hipStream_t s) {
+    const int G = tok_narrow_lanes(a.r.V);
+    const int64_t rb = 256 / G;
+    const dim3 grid(tok_blocks((a.r.rows + rb - 1) / rb, 256)), blk(256);
+    if (G == 8) hipLaunchKernelGGL((tok_distill_narrow_kernel<T, 8, GRAD>), grid, blk, 0, s, a);
+    else if (G == 16) hipLaunchKernelGGL((tok_distill_narrow_kernel<T, 16, GRAD>), grid, blk, 0, s, a);
+    else if (G == 32) hipLaunchKernelGGL((tok_distill_narrow_kernel<T, 32, GRAD>), grid, blk, 0, s, a);
+    else hipLaunchKernelGGL((tok_distill_narrow_kernel<T, 64, GRAD>), grid, blk, 0, s, a);
+}
+template <typename T> static void distill_any(const DistArgs& a, const TokPlan* p, bool grad, hipStream_t s) {
+    if (!p) grad ? distill_narrow<T, true>(a, s) : distill_narrow<T, false>(a, s);
+    else grad ? distill_wide<T, true>(a, *p, s) : distill_wide<T, false>(a, *p, s);
+}
+template <typename T> static void distill_grad_any(DistGradArgs a, hipStream_t s) {
+    const int V = a.r.V;
+    if (V <= TOK_NARROW_V) {
+        const int G = tok_narrow_lanes(V);
+        const int64_t rb = 256 / G;
+        const dim3 grid(tok_blocks((a.r.rows + rb - 1) / rb, 256)), blk(256);
+        if (G == 8) hipLaunchKernelGGL((tok_distill_grad_narrow_kernel<T, 8>), grid, blk, 0, s, a);
+        else if (G == 16) hipLaunchKernelGGL((tok_distill_grad_narrow_kernel<T, 16>), grid, blk, 0, s, a);
+        else if (G == 32) hipLaunchKernelGGL((tok_distill_grad_narrow_kernel<T, 32>), grid, blk, 0, s, a);
+        else hipLaunchKernelGGL((tok_distill_grad_narrow_kernel<T, 64>), grid, blk, 0, s, a);
+        return;
+    }
+    a.chunks = (V / TokElem<T>::VEC + 1023) / 1024;
+    hipLaunchKernelGGL((tok_distill_grad_kernel<T>), dim3(tok_blocks(a.r.rows * a.chunks, 256)), dim3(256), 0, s, a);
+}
+
+// dtype: 0 fp32, 1 bf16, 2 fp16.  dx = 0: loss, stat and pk (for launch_tok_distill_grad).  dx: the gradient too, for a loss
+// gradient of 1 a row; stat / pk / ws as tok_distill_segments says.
+void launch_tok_distill(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s0, int64_t s1, int64_t V, double temperature,
+                        uint64_t ids, int id64, uint64_t t, uint64_t w, int K, int bucket, uint64_t loss, uint64_t dx,
+                        uint64_t stat, uint64_t pk, uint64_t ws, uint64_t stream) {
+    if (rows <= 0) return;
+    if (dtype < 0 || dtype > 2) throw std::runtime_error("token operators: unknown logits type");
+    if (K < 1 || K > DIST_MAX_K) throw std::runtime_error("tok_distill: 1 to 256 teacher entries a row");
+    DistArgs a{};
+    a.r = tok_rows_of(x, rows, n1, s0, s1, V, temperature);
+    a.ids = (int64_t)ids;
+    a.id64 = id64;
+    a.t = as_ptr<const float>(t);
+    a.w = as_ptr<const float>(w);
+    a.K = K;
+    a.bucket = bucket;
+    a.T = (float)temperature;
+    a.loss = as_ptr<float>(loss);
+    a.dx = as_ptr<void>(dx);
+    a.stat = as_ptr<float4>(stat);
+    a.pk = as_ptr<float>(pk);
+    a.nseg = 1;
+    const hipStream_t s = as_stream(stream);
+    const bool narrow = V <= TOK_NARROW_V, one = narrow || dist_one_pass(V, dtype), grad = dx && one;
+    TokPlan p{};
+    if (!narrow) {
+        p = grad ? tok_plan(V, tok_esize(dtype), rows, DIST_ONE_PASS_VEC, false) : dist_plan(V, dtype, rows);
+        a.nseg = p.nseg;
+        a.segvec = p.segvec;
+        if (p.nseg > 1 && !ws) throw std::runtime_error("tok_distill: this shape needs a workspace");
+        a.part = as_ptr<float4>(ws);
+    }
+    if (dx && !grad && (!stat || !pk)) throw std::runtime_error("tok_distill: this shape needs the stat and pk buffers");
+    if (dtype == 0) distill_any<float>(a, narrow ? nullptr : &p, grad, s);
+    else if (dtype == 1) distill_any<bf16_t>(a, narrow ? nullptr : &p, grad, s);
+    else distill_any<f16_t>(a, narrow ? nullptr : &p, grad, s);
+    SERANN_CHECK(hipGetLastError());
+    if (a.nseg > 1) {
+        const dim3 grid(tok_blocks(rows, 64)), blk(64);
+        if (dtype == 0) hipLaunchKernelGGL((tok_distill_join_kernel<float>), grid, blk, 0, s, a);
+        else if (dtype == 1) hipLaunchKernelGGL((tok_distill_join_kernel<bf16_t>), grid, blk, 0, s, a);
+        else hipLaunchKernelGGL((tok_distill_join_kernel<f16_t>), grid, blk, 0, s, a);
+        SERANN_CHECK(hipGetLastError());
+    }
+    if (dx && !grad)
+        launch_tok_distill_grad(x, dtype, rows, n1, s0, s1, V, temperature, ids, id64, w, K, 0, stat, pk, dx, stream);
+}
+
+// g = 0: a loss gradient of 1 a row
+void launch_tok_distill_grad(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s0, int64_t s1, int64_t V,
+                             double temperature, uint64_t ids, int id64, uint64_t w, int K, uint64_t g, uint64_t stat,
+                             uint64_t pk, uint64_t dx, uint64_t stream) {
+    if (rows <= 0) return;
+    if (dtype < 0 || dtype > 2) throw std::runtime_error("token operators: unknown logits type");
+    if (K < 1 || K > DIST_MAX_K) throw std::runtime_error("tok_distill: 1 to 256 teacher entries a row");
+    DistGradArgs a{};
+    a.r = tok_rows_of(x, rows, n1, s0, s1, V, temperature);
+    a.ids = (int64_t)ids;
+    a.id64 = id64;
+    a.K = K;
+    a.T = (float)temperature;
+    a.w = as_ptr<const float>(w);
+    a.g = as_ptr<const float>(g);
+    a.pk = as_ptr<const float>(pk);
+    a.stat = as_ptr<const float4>(stat);
+    a.dx = as_ptr<void>(dx);
+    const hipStream_t s = as_stream(stream);
+    if (dtype == 0) distill_grad_any<float>(a, s);
+    else if (dtype == 1) distill_grad_any<bf16_t>(a, s);
+    else distill_grad_any<f16_t>(a, s);
+    SERANN_CHECK(hipGetLastError());
+}

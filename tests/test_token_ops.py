@@ -1,0 +1,161 @@
+"""Token operators (ops/token_ops.py) on the CPU: the torch forms against the definitions in 64 bits, and the refusals."""
+import math
+
+import pytest
+import torch
+
+from . import token_oracle as O
+from serann.ops import token_ops as TO
+
+IGN = -100
+
+
+def _rows(R, V, seed, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(R, V, generator=g) * 3).to(dtype), torch.randint(0, V, (R,), generator=g), g
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V,k", [(1, 1), (40, 5), (300, 0)])
+def test_score_matches_the_definition(V, k, dtype):
+    x, y, g = _rows(8, V, V, dtype)
+    y[2] = IGN
+    gl, gh = torch.randn(8, generator=g), torch.randn(8, generator=g)
+    x[3, 1:] = -math.inf
+    ref = O.score(x, y, 0.7, k, IGN, gl, gh)
+    xd = x.clone().requires_grad_(True)
+    r = TO.token_logprobs(xd, y, temperature=0.7, top_k=k)
+    tol = 64 * O.U * 20
+    assert torch.allclose(r.logprob.double(), ref["logprob"], rtol=tol, atol=tol)
+    assert torch.allclose(r.entropy.double(), ref["entropy"], rtol=tol, atol=tol)
+    dx, = torch.autograd.grad([r.logprob, r.entropy], [xd], [gl, gh])
+    lim = O.half_ulp(ref["grad"], dtype) + tol * 4
+    assert ((dx.double() - ref["grad"]).abs() <= lim).all()
+    if k:
+        assert torch.equal(r.top_ids, ref["top_ids"])
+    else:
+        assert r.top_ids is None and r.top_logprobs is None
+
+
+def test_score_odd_rows():
+    x, y, _ = _rows(6, 40, 1)
+    x[0] = -math.inf
+    x[1, 3] = math.nan
+    x[2, 3] = math.inf
+    x[3] = math.nan
+    y[3] = IGN
+    y[4] = 40
+    x.requires_grad_(True)
+    r = TO.token_logprobs(x, y, top_k=3)
+    ref = O.score(x.detach(), y, 1.0, 3, IGN)
+    assert r.logprob[0] == -math.inf and r.entropy[0] == 0
+    assert r.logprob[[1, 2, 4]].isnan().all() and r.logprob[3] == 0 and r.entropy[3] == 0
+    assert torch.equal(r.top_ids, ref["top_ids"])
+    assert r.top_ids[[1, 2, 3]].eq(-1).all()
+
+
+@pytest.mark.parametrize("tail", ["drop", "bucket"])
+@pytest.mark.parametrize("V,K", [(1, 1), (40, 8), (40, 40), (300, 12)])
+def test_distill_matches_the_definition(V, K, tail):
+    x, _, g = _rows(7, V, K)
+    ids = torch.randint(0, V, (7, K), generator=g)
+    t = torch.log_softmax(torch.randn(7, K + 3, generator=g), -1)[:, :K].contiguous()
+    if K > 4:
+        ids[0, 1] = ids[0, 0]
+        ids[1, 2:] = -1
+        ids[2, 3] = V
+        ids[3] = -1
+        t[4, 1] = -math.inf
+    w = torch.rand(7, generator=g) + 0.5
+    w[6] = 0
+    x[6] = math.nan
+    loss, dx = O.distill(x, ids, t, 2.0, tail, w)
+    l, d = TO.topk_distill_grad(x, ids, t, temperature=2.0, tail=tail, weight=w)
+    assert torch.allclose(l.double(), loss, rtol=4 * O.U, atol=1e-9)
+    assert torch.allclose(d.double(), dx, rtol=4 * O.U, atol=4 * O.U)
+    xd = x.clone().requires_grad_(True)
+    l2 = TO.topk_distill_loss(xd, ids, t, temperature=2.0, tail=tail, weight=w)
+    d2, = torch.autograd.grad(l2.sum(), xd)
+    assert torch.equal(l2.detach(), l) and torch.equal(d2, d)
+
+
+def test_teacher_to_student():
+    t, y, g = _rows(9, 40, 4)
+    s = t + torch.randn(9, 40, generator=g)
+    y[1] = IGN
+    r = TO.token_logprobs(t, y, top_k=6, temperature=1.5)
+    loss = TO.topk_distill_loss(s, r.top_ids, r.top_logprobs, temperature=1.5)
+    want, _ = O.distill(s, r.top_ids, r.top_logprobs, 1.5, "drop", None)
+    assert loss[1] == 0 and torch.allclose(loss.double(), want, rtol=4 * O.U, atol=1e-9)
+
+
+def test_score_refusals():
+    x, y, _ = _rows(4, 10, 0)
+    ok = TO.token_logprobs
+    for bad in (x.double(), x.long(), [[1.0]]):
+        with pytest.raises(TypeError):
+            ok(bad, y)
+    for bad in (torch.zeros(4, 0), torch.tensor(1.0), torch.zeros(1, (1 << 20) + 1)):
+        with pytest.raises(ValueError):
+            ok(bad)
+    for T in (0.0, -1.0, math.nan, math.inf, 1e-9):
+        with pytest.raises(ValueError):
+            ok(x, y, temperature=T)
+    for k in (-1, 11, 200):
+        with pytest.raises(ValueError):
+            ok(x, y, top_k=k)
+    with pytest.raises(ValueError):
+        ok(torch.zeros(2, 500), top_k=129)
+    with pytest.raises(TypeError):
+        ok(x, y.float())
+    with pytest.raises(TypeError):
+        ok(x, [1, 2, 3, 4])
+    for bad in (y[:3], y[:, None], y.new_zeros(())):
+        with pytest.raises(ValueError):
+            ok(x, bad)
+    with pytest.raises(ValueError):
+        ok(x, torch.zeros(4, dtype=torch.int64, device="meta"))
+
+
+def test_distill_refusals():
+    x, _, _ = _rows(4, 10, 0)
+    ids, t = torch.zeros(4, 3, dtype=torch.int64), torch.zeros(4, 3)
+    for f in (TO.topk_distill_loss, TO.topk_distill_grad):
+        for args in ((x.double(), ids, t), (x, ids.float(), t), (x, ids, t.double()), (x, ids, t.long())):
+            with pytest.raises(TypeError):
+                f(*args)
+        for args in ((x, ids[:, :2], t), (x, ids[:3], t[:3]), (x, ids[..., None], t[..., None]),
+                     (x, torch.zeros(4, 0, dtype=torch.int64), torch.zeros(4, 0)),
+                     (x, torch.zeros(4, 257, dtype=torch.int64), torch.zeros(4, 257)),
+                     (x, ids, t.clone().requires_grad_(True))):
+            with pytest.raises(ValueError):
+                f(*args)
+        with pytest.raises(ValueError):
+            f(x, ids, t, tail="sum")
+        with pytest.raises(ValueError):
+            f(x, ids, t, temperature=0)
+        with pytest.raises(ValueError):
+            f(x, ids, t, weight=torch.ones(3))
+        with pytest.raises(TypeError):
+            f(x, ids, t, weight=torch.ones(4, dtype=torch.int64))
+        with pytest.raises(ValueError):
+            f(x, ids, t, weight=torch.ones(4, requires_grad=True))
+    for out in (torch.zeros(4, 9), torch.zeros(4, 10, dtype=torch.bfloat16), torch.zeros(4, 20)[:, ::2], x):
+        with pytest.raises(ValueError):
+            TO.topk_distill_grad(x, ids, t, out=out)
+
+
+def test_row_layouts():
+    """Strided rows are described, not copied, where two strides do."""
+    x = torch.zeros(3, 6, 10)
+    for v, want in ((x, (18, 18, 0, 10)), (x[:, :-1], (15, 5, 60, 10)), (x[..., 1:9], (18, 18, 0, 10)),
+                    (x.transpose(0, 1), (18, 3, 10, 60)), (x[:, :1], (3, 3, 0, 60)), (x[:1].expand(4, 6, 10), (24, 6, 0, 10))):
+        y, rows, n1, s0, s1 = TO._rows(v)
+        assert y.data_ptr() == v.data_ptr() and (rows, n1, s0, s1) == want, (v.shape, v.stride())
+        off = [(r // n1) * s0 + (r % n1) * s1 for r in range(rows)]
+        base = torch.arange(x.numel()).as_strided(v.shape, v.stride())
+        assert off == (base[..., 0].reshape(-1)).tolist()
+    y = TO._rows(torch.zeros(3, 5, 20)[..., ::2])[0]
+    assert y.is_contiguous()
+    y = TO._rows(torch.zeros(2, 3, 4, 7).permute(2, 0, 1, 3)[:, :, :2])[0]
+    assert y.is_contiguous()
