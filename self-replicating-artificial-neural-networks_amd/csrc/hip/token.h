@@ -27,6 +27,7 @@ constexpr int TOK_NARROW_V = 512;     // rows of up to 64 x 8 elements: a group 
 // Rows of a [n0][n1][V] tensor with strides s0, s1 (elements) and unit stride inside a row; row r = (r / n1, r % n1)
 struct TokRows {
     int64_t x, rows, n1, s0, s1;
+    int64_t u0;           // first unit of this launch (tok_launch)
     int V;
     float c, inv_t;       // log2(e) / T, 1 / T
     double dinv_t;
@@ -73,13 +74,16 @@ template <> struct TokElem<f16_t> {
     static __device__ __forceinline__ f16_t put(float f) { return (f16_t)f; }
 };
 
-// 16 bytes at any element's address: a row starts where its stride puts it (odd V), and gfx950 takes unaligned vectors
-__device__ __forceinline__ u32x4_t tok_ld16(const void* p) {
-    u32x4_t v;
-    __builtin_memcpy(&v, p, 16);
-    return v;
+// 16 bytes at any element's address: a row starts where its stride puts it (odd V), and gfx950 takes unaligned vectors.
+// Addresses that come as integers are told to be global memory (a flat access would wait for LDS too).
+#define TOK_GLOBAL __attribute__((address_space(1)))
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T> using tok_in = const TOK_GLOBAL T*;
+template <typename T> using tok_out = TOK_GLOBAL T*;
+template <typename T> __device__ __forceinline__ u32x4_t tok_ld16(tok_in<T> p) {
+    return *(tok_in<u32x4_any>)p;
 }
-__device__ __forceinline__ void tok_st16(void* p, u32x4_t v) { __builtin_memcpy(p, &v, 16); }
+template <typename T> __device__ __forceinline__ void tok_st16(tok_out<T> p, u32x4_t v) { *(tok_out<u32x4_any>)p = v; }
 
 // max without the canonicalising multiplies that fmaxf brings for signalling NaNs; a NaN operand is passed over (it comes
 // back through the sums)
@@ -146,12 +150,12 @@ __device__ __forceinline__ uint64_t tok_key(float x, int i) {
 __device__ __forceinline__ int tok_key_index(uint64_t k) { return (int)~(uint32_t)k; }
 __device__ __forceinline__ float tok_key_value(uint64_t k) { return tok_unorder((uint32_t)(k >> 32)); }
 
-template <typename T> __device__ __forceinline__ const T* tok_row(const TokRows& r, int64_t row) {
-    const int64_t i0 = r.n1 == r.rows ? 0 : row / r.n1;
-    return reinterpret_cast<const T*>(r.x) + i0 * r.s0 + (row - i0 * r.n1) * r.s1;
+template <typename T> __device__ __forceinline__ tok_in<T> tok_row(const TokRows& r, int64_t row) {
+    const int64_t i0 = r.n1 == r.rows ? 0 : (int64_t)((uint32_t)row / (uint32_t)r.n1);      // fewer than 2^31 rows
+    return (tok_in<T>)r.x + i0 * r.s0 + (row - i0 * r.n1) * r.s1;
 }
 __device__ __forceinline__ int64_t tok_int(int64_t base, int is64, int64_t i) {
-    return is64 ? reinterpret_cast<const int64_t*>(base)[i] : (int64_t) reinterpret_cast<const int32_t*>(base)[i];
+    return is64 ? ((tok_in<int64_t>)base)[i] : (int64_t)((tok_in<int32_t>)base)[i];
 }
 
 // A row's exponents, d = fma(x, c, -mc).  Where |m| c is near overflow (a row of the type's lowest values), two different
@@ -172,6 +176,28 @@ __device__ __forceinline__ TokRef tok_ref(float m, float c) {
 // ln(n + S) of a row's sums (n elements at the maximum, S over the others)
 __device__ __forceinline__ float tok_ln(float n, float S) { return n == 1.f ? log1pf(S) : logf(n + S); }
 
+// Vectors that need a look at each element (one with the maximum, with candidates of the top k, with listed tokens) go, data
+// and place, to this LDS list, out of the unrolled pass.  Slots are handed out by an atomic, in any order; what is summed is
+// summed by the thread that pushed the vector, along its own chain of slots, so the sums do not depend on that order.
+template <int CAP> struct TokSpecial {
+    u32x4_t data[CAP];
+    int at[CAP], next[CAP];      // vector of the segment (bit 31: to be summed), the thread's slot before this one
+    int n;
+    __device__ __forceinline__ void push(const u32x4_t& v, int where, bool sum, int& chain) {
+        const int i = atomicAdd(&n, 1);
+        if (i < CAP) {
+            data[i] = v;
+            at[i] = where | (sum ? (int)0x80000000 : 0);
+            next[i] = chain;
+            chain = i;
+        }
+    }
+    __device__ __forceinline__ int vec(int slot) const { return at[slot] & 0x7fffffff; }
+    template <typename T> __device__ __forceinline__ float get(int slot, int e) const {
+        return TokElem<T>::one(reinterpret_cast<const T*>(&data[slot])[e]);
+    }
+};
+
 // A segment of a row in registers: NV 16-byte vectors a thread and one of the < VEC last elements of the row.  Vector
 // i * NT + tid of the segment is r[i]; vm[i] its maximum.
 template <typename T, int NT, int NV> struct TokSeg {
@@ -179,19 +205,23 @@ template <typename T, int NT, int NV> struct TokSeg {
     u32x4_t r[NV];
     float vm[NV];
     float xt;
-    int nv, tail0;      // full vectors of the segment; first element (from the segment's start) behind them
-    __device__ __forceinline__ void load(const T* __restrict__ x, int nvec, int ntail) {
+    int nv;             // full vectors of the segment
+    __device__ __forceinline__ void load(tok_in<T> x, int nvec, int ntail) {
         const int tid = threadIdx.x;
+        asm("" : "+s"(nvec));                               // masks made here and now, not kept from row to row
         nv = nvec;
-        tail0 = nvec * VEC;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const uint32_t u = (uint32_t)(i * NT + tid);
-            r[i] = u32x4_t{TokElem<T>::NEG_INF, TokElem<T>::NEG_INF, TokElem<T>::NEG_INF, TokElem<T>::NEG_INF};
-            if (u < (uint32_t)nvec) r[i] = tok_ld16(reinterpret_cast<const char*>(x) + (size_t)(u * 16u));
+            tok_in<T> p = x + i * NT * VEC;                 // uniform; the thread's part of the address is one 32-bit offset
+            if ((i + 1) * NT <= nvec) {
+                r[i] = tok_ld16<T>((tok_in<T>)((tok_in<char>)p + (uint32_t)tid * 16u));
+            } else {
+                r[i] = u32x4_t{TokElem<T>::NEG_INF, TokElem<T>::NEG_INF, TokElem<T>::NEG_INF, TokElem<T>::NEG_INF};
+                if (i * NT + tid < nvec) r[i] = tok_ld16<T>((tok_in<T>)((tok_in<char>)p + (uint32_t)tid * 16u));
+            }
         }
         xt = -INFINITY;
-        if (tid < ntail) xt = TokElem<T>::one(x[tail0 + tid]);
+        if (tid < ntail) xt = TokElem<T>::one(x[nvec * VEC + tid]);
     }
     __device__ __forceinline__ float max_of() {
         float m = xt;
@@ -219,7 +249,7 @@ template <typename T, int NT, int NV> struct TokSeg {
 };
 
 // Narrow rows: the 8 elements from e0 on that a lane holds, -inf behind the row's end
-template <typename T> __device__ __forceinline__ void tok_narrow_load(const T* x, int V, int e0, bool live, float* f) {
+template <typename T> __device__ __forceinline__ void tok_narrow_load(tok_in<T> x, int V, int e0, bool live, float* f) {
     constexpr int VEC = TokElem<T>::VEC;
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = -INFINITY;
@@ -227,7 +257,7 @@ template <typename T> __device__ __forceinline__ void tok_narrow_load(const T* x
     if (e0 + 8 <= V) {
 #pragma unroll
         for (int h = 0; h < 8 / VEC; ++h) {
-            const u32x4_t v = tok_ld16(x + e0 + h * VEC);
+            const u32x4_t v = tok_ld16<T>(x + e0 + h * VEC);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) f[h * VEC + e] = TokElem<T>::get(v, e);
         }
@@ -237,11 +267,11 @@ template <typename T> __device__ __forceinline__ void tok_narrow_load(const T* x
             if (e0 + e < V) f[e] = TokElem<T>::one(x[e0 + e]);
     }
 }
-template <typename T> __device__ __forceinline__ void tok_narrow_store(T* o, int V, int e0, const float* f) {
+template <typename T> __device__ __forceinline__ void tok_narrow_store(tok_out<T> o, int V, int e0, const float* f) {
     constexpr int VEC = TokElem<T>::VEC;
     if (e0 + 8 <= V) {
 #pragma unroll
-        for (int h = 0; h < 8 / VEC; ++h) tok_st16(o + e0 + h * VEC, TokElem<T>::pack(f + h * VEC));
+        for (int h = 0; h < 8 / VEC; ++h) tok_st16<T>(o + e0 + h * VEC, TokElem<T>::pack(f + h * VEC));
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -276,10 +306,17 @@ inline TokPlan tok_plan(int64_t V, int esize, int64_t rows, int max_vec, bool ma
         }
     return p;
 }
-// blocks of nt threads for `units` of work: HIP counts threads of a launch in 32 bits, longer work is looped over
-inline unsigned tok_blocks(int64_t units, int nt) {
+// Launches over `units` of work, a block each: HIP counts a launch's threads in 32 bits, so longer work is several launches.
+// (A loop over units inside the kernels would do too, but the compiler then keeps the constants of
+// the fp64 functions in registers from unit to unit, up to 60 of them.)
+template <typename A, typename... X>
+inline void tok_launch(void (*kernel)(A, X...), int64_t units, int nt, size_t lds, hipStream_t s, A a, X... more) {
     const int64_t cap = ((int64_t)1 << 31) / nt;
-    return (unsigned)(units < cap ? units : cap);
+    for (a.r.u0 = 0; a.r.u0 < units; a.r.u0 += cap) {
+        const int64_t n = units - a.r.u0 < cap ? units - a.r.u0 : cap;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(nt), lds, s, a, more...);
+        SERANN_CHECK(hipGetLastError());
+    }
 }
 inline TokRows tok_rows_of(uint64_t x, int64_t rows, int64_t n1, int64_t s0, int64_t s1, int64_t V, double temperature) {
     if (rows < 0 || V < 1 || V > TOK_MAX_V) throw std::runtime_error("token operators: vocabulary must be in [1, 2^20]");
@@ -291,6 +328,7 @@ inline TokRows tok_rows_of(uint64_t x, int64_t rows, int64_t n1, int64_t s0, int
     r.n1 = n1;
     r.s0 = s0;
     r.s1 = s1;
+    r.u0 = 0;
     r.V = (int)V;
     r.c = (float)(1.4426950408889634 / temperature);
     r.inv_t = (float)(1.0 / temperature);

@@ -29,7 +29,7 @@ struct DistArgs {
     int nseg, segvec;
     float T;
     float* loss;
-    void* dx;             // [rows][V], one-pass form
+    int64_t dx;           // [rows][V], one-pass form
     float4* stat;         // (m, log2 sum, A, B) for the gradient launch
     float* pk;            // [rows][K]: the entry's p (its first occurrence carries the sum), -1: skip
     float4* part;         // nseg > 1: (m, n, S, -) of each segment; bucket: over unlisted elements, m over all
@@ -163,7 +163,7 @@ __device__ __forceinline__ float dist_q(const DistRow& d, float c, float x) {
     return tok_exp2(__builtin_fmaf(x - d.m, c, -d.l2S));
 }
 
-template <typename T> __device__ __forceinline__ void dist_load_entry(const DistArgs& a, DistEntries& E, int64_t row, const T* x,
+template <typename T> __device__ __forceinline__ void dist_load_entry(const DistArgs& a, DistEntries& E, int64_t row, tok_in<T> x,
                                                                       int j) {
     int64_t id = tok_int(a.ids, a.id64, row * a.K + j);
     const bool in = (uint64_t)id < (uint64_t)a.r.V;
@@ -171,138 +171,155 @@ template <typename T> __device__ __forceinline__ void dist_load_entry(const Dist
     E.t[j] = a.t[row * a.K + j];
     E.x[j] = in ? TokElem<T>::one(x[id]) : 0.f;
 }
+// One element's share of the sums; skip: listed, in bucket mode
+struct DistSums {
+    float S, n;
+    __device__ __forceinline__ void add(float x, const TokRef& ref, bool skip) {
+        const bool is = x == ref.meq;
+        S += is || skip ? 0.f : tok_exp2(__builtin_fmaf(x, ref.c, -ref.mc));
+        n += is && !skip ? 1.f : 0.f;
+    }
+};
 
 template <typename T, int NT, int NV, bool GRAD>
-__global__ __launch_bounds__(NT) void tok_distill_kernel(DistArgs a) {
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void tok_distill_kernel(DistArgs a) {
     constexpr int VEC = TokElem<T>::VEC, NW = NT / 64;
     constexpr int WORDS = NT * NV * VEC / 32 + 1;
     __shared__ DistEntries E;
-    __shared__ uint32_t bits[WORDS];
+    __shared__ uint32_t bits[WORDS];                         // listed tokens of the segment
+    constexpr int SPECIAL = NT == 64 ? 192 : 512;
+    __shared__ TokSpecial<SPECIAL> list;
     __shared__ float red[NW][3];
     __shared__ int dup;
     __shared__ DistRow rowd;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nvec_row = a.r.V / VEC, ntail_row = a.r.V - nvec_row * VEC;
-    const int64_t units = a.r.rows * a.nseg;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const int64_t row = a.nseg == 1 ? u : u / a.nseg;
-        const int seg = (int)(u - row * a.nseg);
-        const float w = a.w ? a.w[row] : 1.f;
-        T* o = reinterpret_cast<T*>(a.dx) + row * a.r.V;
-        if (w == 0.f) {
-            if (a.nseg == 1 && tid == 0) {
-                a.loss[row] = 0.f;
-                if (a.stat) a.stat[row] = make_float4(0.f, INFINITY, 0.f, 0.f);
-            }
-            if constexpr (GRAD) {
-                for (int v = tid; v < nvec_row; v += NT) tok_st16(o + (int64_t)v * VEC, u32x4_t{0, 0, 0, 0});
-                if (tid < ntail_row) o[nvec_row * VEC + tid] = TokElem<T>::put(0.f);
-            }
-            continue;
+    const int64_t u = a.r.u0 + blockIdx.x;
+    const int64_t row = a.nseg == 1 ? u : u / a.nseg;
+    const int seg = (int)(u - row * a.nseg);
+    const float w = a.w ? a.w[row] : 1.f;
+    tok_out<T> o = (tok_out<T>)a.dx + row * a.r.V;
+    if (w == 0.f) {
+        if (a.nseg == 1 && tid == 0) {
+            a.loss[row] = 0.f;
+            if (a.stat) a.stat[row] = make_float4(0.f, INFINITY, 0.f, 0.f);
         }
-        const T* x = tok_row<T>(a.r, row);
-        const int v0 = seg * a.segvec;
-        const int nv = min(a.segvec, nvec_row - v0);
-        const int ntail = seg == a.nseg - 1 ? ntail_row : 0;
-        TokSeg<T, NT, NV> s;
-        s.load(x + (int64_t)v0 * VEC, nv, ntail);
-        const int e0 = v0 * VEC, len = nv * VEC + ntail;
-        for (int i = tid; i < (len + 31) / 32; i += NT) bits[i] = 0;
-        if (tid == 0) dup = 0;
-        for (int j = tid; j < a.K; j += NT) dist_load_entry<T>(a, E, row, x, j);
-        __syncthreads();
-        // mark this segment's listed tokens; a bit found set already means an id that occurs twice
-        for (int j = tid; j < a.K; j += NT) {
-            const int id = E.id[j] - e0;
-            if (E.id[j] >= 0 && id >= 0 && id < len) {
-                const uint32_t bit = 1u << (id & 31);
-                if (atomicOr(&bits[id >> 5], bit) & bit) dup = 1;
-            }
+        if constexpr (GRAD) {
+            for (int v = tid; v < nvec_row; v += NT) tok_st16<T>(o + (int64_t)v * VEC, u32x4_t{0, 0, 0, 0});
+            if (tid < ntail_row) o[nvec_row * VEC + tid] = TokElem<T>::put(0.f);
         }
-        const float wm = tok_group<64, TokMax>(s.max_of());
-        if (lane == 0) red[wave][0] = wm;
-        __syncthreads();
-        float m = red[0][0];
+        return;
+    }
+    tok_in<T> x = tok_row<T>(a.r, row);
+    const int v0 = seg * a.segvec;
+    const int nv = min(a.segvec, nvec_row - v0);
+    const int ntail = seg == a.nseg - 1 ? ntail_row : 0;
+    const int e0 = v0 * VEC, len = nv * VEC + ntail;
+    TokSeg<T, NT, NV> s;
+    s.load(x + e0, nv, ntail);
+    for (int i = tid; i < WORDS; i += NT) bits[i] = 0;
+    if (tid == 0) dup = list.n = 0;
+    for (int j = tid; j < a.K; j += NT) dist_load_entry<T>(a, E, row, x, j);
+    __syncthreads();
+    // mark this segment's listed tokens; a bit found set already means an id that occurs twice
+    for (int j = tid; j < a.K; j += NT) {
+        const int id = E.id[j] - e0;
+        if (E.id[j] >= 0 && id >= 0 && id < len) {
+            const uint32_t bit = 1u << (id & 31);
+            if (atomicOr(&bits[id >> 5], bit) & bit) dup = 1;
+        }
+    }
+    const float wm = tok_group<64, TokMax>(s.max_of());
+    if (lane == 0) red[wave][0] = wm;
+    __syncthreads();
+    float m = red[0][0];
 #pragma unroll
-        for (int k = 1; k < NW; ++k) m = tok_max(m, red[k][0]);
-        const TokRef ref = tok_ref(m, a.r.c);
-        const float meq = ref.meq, mc = ref.mc, c = ref.c;
-        float S = 0.f, n = 0.f;
+    for (int k = 1; k < NW; ++k) m = tok_max(m, red[k][0]);
+    const TokRef ref = tok_ref(m, a.r.c);
+    DistSums sum{0.f, 0.f};
+    int chain = -1;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (i * NT < nv) {
+            float cs = 0.f;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) cs += tok_exp2(__builtin_fmaf(TokElem<T>::get(s.r[i], e), ref.c, -ref.mc));
+            bool special = s.vm[i] == ref.meq;
+            if (a.bucket) {
+                const int at = i * NT + tid;
+                const uint8_t by = reinterpret_cast<const uint8_t*>(bits)[VEC == 8 ? at : at >> 1];
+                special |= (VEC == 8 ? by : by & (15u << ((at & 1) * 4))) != 0;
+            }
+            if (special) list.push(s.r[i], i * NT + tid, true, chain);
+            sum.S += special ? 0.f : cs;
+        }
+    }
+    __syncthreads();
+    const int nl = list.n;
+    if (nl <= SPECIAL) {
+        for (; chain >= 0; chain = list.next[chain]) {
+            const int at = list.vec(chain) * VEC;
+            const uint32_t out = a.bucket ? bits[at >> 5] >> (at & 31) : 0;      // a vector's bits lie in one word
+            for (int e = 0; e < VEC; ++e) sum.add(list.template get<T>(chain, e), ref, (out >> e) & 1);
+        }
+    } else {                                             // thousands of elements at the maximum: one by one, read again
+        sum = DistSums{0.f, 0.f};
+        for (int v = tid; v < nv; v += NT) {
+            const u32x4_t r = tok_ld16<T>(x + e0 + (int64_t)v * VEC);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int at = v * VEC + e;
+                sum.add(TokElem<T>::get(r, e), ref, a.bucket && ((bits[at >> 5] >> (at & 31)) & 1));
+            }
+        }
+    }
+    if (tid < ntail) {
+        const int at = nv * VEC + tid;
+        sum.add(s.xt, ref, a.bucket && ((bits[at >> 5] >> (at & 31)) & 1));
+    }
+    const float S1 = tok_group<64, TokSum>(sum.S), n1 = tok_group<64, TokSum>(sum.n);
+    if (lane == 0) {
+        red[wave][1] = S1;
+        red[wave][2] = n1;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        float S = red[0][1], n = red[0][2];
+#pragma unroll
+        for (int k = 1; k < NW; ++k) {
+            S += red[k][1];
+            n += red[k][2];
+        }
+        S *= tok_exp2(-ref.dmax);
+        if (a.nseg > 1) {
+            if (lane == 0) a.part[u] = make_float4(m, n, S, 0.f);
+        } else {
+            const DistRow d = dist_epilogue(a, E, row, w, m, n, S, dup != 0, lane);
+            if (lane == 0) rowd = d;
+        }
+        // fp64 logarithms take as many registers as the row: this wave gives its part up and reads it again (L2)
+        if constexpr (GRAD) s.load(x + e0, nv, ntail);
+    }
+    __syncthreads();
+    if constexpr (GRAD) {
+        s.forget();
+        const DistRow d = rowd;
+        const float f = w * a.T, fB = f * d.B;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (i * NT < nv) {
-                float cs = 0.f;
-                uint32_t skip = 0;                           // listed elements of this vector (bucket mode)
-                if (a.bucket && i * NT + tid < nv) {
-                    const int at = i * NT + tid;
-                    const uint8_t by = reinterpret_cast<const uint8_t*>(bits)[VEC == 8 ? at : at >> 1];
-                    skip = VEC == 8 ? by : (by >> ((at & 1) * 4)) & 15u;
-                }
-                if (s.vm[i] == meq || skip) {
+            if (i * NT + tid < nv) {
+                float g[VEC];
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float xv = TokElem<T>::get(s.r[i], e);
-                        const bool is = xv == meq, out = (skip >> e) & 1;
-                        cs += is || out ? 0.f : tok_exp2(__builtin_fmaf(xv, c, -mc));
-                        n += is && !out ? 1.f : 0.f;
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) cs += tok_exp2(__builtin_fmaf(TokElem<T>::get(s.r[i], e), c, -mc));
-                }
-                S += cs;
+                for (int e = 0; e < VEC; ++e) g[e] = fB * dist_q(d, a.r.c, TokElem<T>::get(s.r[i], e));
+                tok_st16<T>(o + (int64_t)(i * NT + tid) * VEC, TokElem<T>::pack(g));
             }
         }
-        if (tid < ntail) {
-            const int at = nv * VEC + tid;
-            const bool is = s.xt == meq, out = a.bucket && ((bits[at >> 5] >> (at & 31)) & 1);
-            S += is || out ? 0.f : tok_exp2(__builtin_fmaf(s.xt, c, -mc));
-            n += is && !out ? 1.f : 0.f;
-        }
-        S = tok_group<64, TokSum>(S);
-        n = tok_group<64, TokSum>(n);
-        if (lane == 0) {
-            red[wave][1] = S;
-            red[wave][2] = n;
-        }
-        __syncthreads();
-        if (wave == 0) {
-            S = red[0][1];
-            n = red[0][2];
-#pragma unroll
-            for (int k = 1; k < NW; ++k) {
-                S += red[k][1];
-                n += red[k][2];
-            }
-            S *= tok_exp2(-ref.dmax);
-            if (a.nseg > 1) {
-                if (lane == 0) a.part[u] = make_float4(m, n, S, 0.f);
-            } else {
-                const DistRow d = dist_epilogue(a, E, row, w, m, n, S, dup != 0, lane);
-                if (lane == 0) rowd = d;
-            }
-        }
-        __syncthreads();
-        if constexpr (GRAD) {
-            s.forget();
-            const DistRow d = rowd;
-            const float f = w * a.T, fB = f * d.B;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                if (i * NT + tid < nv) {
-                    float g[VEC];
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) g[e] = fB * dist_q(d, a.r.c, TokElem<T>::get(s.r[i], e));
-                    tok_st16(o + (int64_t)(i * NT + tid) * VEC, TokElem<T>::pack(g));
-                }
-            }
-            if (tid < ntail) o[nv * VEC + tid] = TokElem<T>::put(fB * dist_q(d, a.r.c, s.xt));
-            __syncthreads();                                 // the listed tokens' stores follow the row's
-            for (int j = tid; j < a.K; j += NT) {
-                const float p = E.p[j];
-                if (E.id[j] >= 0 && p >= 0.f) o[E.id[j]] = TokElem<T>::put(f * (d.A * dist_q(d, a.r.c, E.x[j]) - p));
-            }
-            __syncthreads();                                 // E is used again by the next row
+        if (tid < ntail) o[nv * VEC + tid] = TokElem<T>::put(fB * dist_q(d, a.r.c, s.xt));
+        __syncthreads();                                 // the listed tokens' stores follow the row's
+        for (int j = tid; j < a.K; j += NT) {
+            const float p = E.p[j];
+            if (E.id[j] >= 0 && p >= 0.f) o[E.id[j]] = TokElem<T>::put(f * (d.A * dist_q(d, a.r.c, E.x[j]) - p));
         }
     }
 }
@@ -311,36 +328,35 @@ __global__ __launch_bounds__(NT) void tok_distill_kernel(DistArgs a) {
 template <typename T> __global__ __launch_bounds__(64) void tok_distill_join_kernel(DistArgs a) {
     __shared__ DistEntries E;
     const int lane = threadIdx.x;
-    for (int64_t row = blockIdx.x; row < a.r.rows; row += gridDim.x) {
-        const float w = a.w ? a.w[row] : 1.f;
-        if (w == 0.f) {
-            if (lane == 0) {
-                a.loss[row] = 0.f;
-                if (a.stat) a.stat[row] = make_float4(0.f, INFINITY, 0.f, 0.f);
-            }
-            continue;
+    const int64_t row = a.r.u0 + blockIdx.x;
+    const float w = a.w ? a.w[row] : 1.f;
+    if (w == 0.f) {
+        if (lane == 0) {
+            a.loss[row] = 0.f;
+            if (a.stat) a.stat[row] = make_float4(0.f, INFINITY, 0.f, 0.f);
         }
-        const T* x = tok_row<T>(a.r, row);
-        for (int j = lane; j < a.K; j += 64) dist_load_entry<T>(a, E, row, x, j);
-        const float4* part = a.part + row * a.nseg;
-        float m = -INFINITY;
-        for (int s = 0; s < a.nseg; ++s) m = tok_max(m, part[s].x);
-        float S = 0.f, n = 0.f;
-        for (int s = 0; s < a.nseg; ++s) {
-            const float4 p = part[s];
-            if (p.x == m) {
-                n += p.y;
-                S += p.z;
-            } else if (p.x > -INFINITY) {
-                S += (p.y + p.z) * tok_exp2((p.x - m) * a.r.c);
-            } else {
-                S += p.z;
-            }
-        }
-        __syncthreads();
-        dist_epilogue(a, E, row, w, m, n, S, true, lane);
-        __syncthreads();
+        return;
     }
+    tok_in<T> x = tok_row<T>(a.r, row);
+    for (int j = lane; j < a.K; j += 64) dist_load_entry<T>(a, E, row, x, j);
+    const float4* part = a.part + row * a.nseg;
+    float m = -INFINITY;
+    for (int s = 0; s < a.nseg; ++s) m = tok_max(m, part[s].x);
+    float S = 0.f, n = 0.f;
+    for (int s = 0; s < a.nseg; ++s) {
+        const float4 p = part[s];
+        if (p.x == m) {
+            n += p.y;
+            S += p.z;
+        } else if (p.x > -INFINITY) {
+            S += (p.y + p.z) * tok_exp2((p.x - m) * a.r.c);
+        } else {
+            S += p.z;
+        }
+    }
+    __syncthreads();
+    dist_epilogue(a, E, row, w, m, n, S, true, lane);
+    __syncthreads();
 }
 
 // ---- narrow rows: G lanes a row, 8 elements a lane ------------------------------------------------------------------------
@@ -355,126 +371,118 @@ __global__ __launch_bounds__(256) void tok_distill_narrow_kernel(DistArgs a) {
     const int gl = threadIdx.x & (G - 1), gr = threadIdx.x / G;
     uint32_t* mine = buf + gr * G * 8;
     const int V = a.r.V, K = a.K;
-    for (int64_t r0 = (int64_t)blockIdx.x * RB; r0 < a.r.rows; r0 += (int64_t)gridDim.x * RB) {
-        const int64_t row = r0 + gr;
-        const bool there = row < a.r.rows;
-        const float w = there ? (a.w ? a.w[row] : 1.f) : 0.f;
-        const bool live = there && w != 0.f;
-        const T* x = live ? tok_row<T>(a.r, row) : nullptr;
-        float f[8];
-        tok_narrow_load<T>(x, V, gl * 8, live, f);
+    const int64_t r0 = (a.r.u0 + blockIdx.x) * RB;
+    const int64_t row = r0 + gr;
+    const bool there = row < a.r.rows;
+    const float w = there ? (a.w ? a.w[row] : 1.f) : 0.f;
+    const bool live = there && w != 0.f;
+    tok_in<T> x = live ? tok_row<T>(a.r, row) : (tok_in<T>)0;
+    float f[8];
+    tok_narrow_load<T>(x, V, gl * 8, live, f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mine[gl * 8 + e] = NOT_LISTED;
-        __syncthreads();
-        bool twice = false;
-        float tm = -INFINITY;
-        if (live)
+    for (int e = 0; e < 8; ++e) mine[gl * 8 + e] = NOT_LISTED;
+    __syncthreads();
+    bool twice = false;
+    float tm = -INFINITY;
+    if (live)
+        for (int j = gl; j < K; j += G) {
+            const int64_t id = tok_int(a.ids, a.id64, row * K + j);
+            if ((uint64_t)id < (uint64_t)V) {
+                twice |= atomicExch(&mine[id], 0u) != NOT_LISTED;
+                tm = tok_max(tm, a.t[row * K + j]);
+            }
+        }
+    __syncthreads();
+    float m = tok_max(tok_max3(tok_max3(f[0], f[1], f[2]), f[3], f[4]), tok_max3(f[5], f[6], f[7]));
+    m = tok_group<G, TokMax>(m);
+    const TokRef ref = tok_ref(m, a.r.c);
+    DistSums un{0.f, 0.f}, li{0.f, 0.f};                 // unlisted, listed (drop mode needs their sum alone)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const bool l = mine[gl * 8 + e] != NOT_LISTED;
+        un.add(f[e], ref, l);
+        li.add(f[e], ref, !l);
+    }
+    const float S = tok_group<G, TokSum>(un.S), Sl = tok_group<G, TokSum>(li.S);
+    const float n = tok_group<G, TokSum>(un.n), nl = tok_group<G, TokSum>(li.n);
+    const double sc = (double)tok_exp2(-ref.dmax);
+    const double rest = (double)n + (double)S * sc, listed = (double)nl + (double)Sl * sc;
+    double sum = rest + listed;
+    if (m == INFINITY) sum = (double)NAN;
+    const bool none = sum == 0.0;
+    const double lnS = none ? 0.0 : log(sum);
+    double shift = 0.0;
+    if (!a.bucket) {
+        tm = tok_group<G, TokMax>(tm);
+        double tot = 0.0;
+        if (live && tm > -INFINITY)
             for (int j = gl; j < K; j += G) {
                 const int64_t id = tok_int(a.ids, a.id64, row * K + j);
-                if ((uint64_t)id < (uint64_t)V) {
-                    twice |= atomicExch(&mine[id], 0u) != NOT_LISTED;
-                    tm = tok_max(tm, a.t[row * K + j]);
-                }
+                if ((uint64_t)id < (uint64_t)V) tot += exp((double)a.t[row * K + j] - (double)tm);
             }
-        __syncthreads();
-        float m = tok_max(tok_max3(tok_max3(f[0], f[1], f[2]), f[3], f[4]), tok_max3(f[5], f[6], f[7]));
-        m = tok_group<G, TokMax>(m);
-        const TokRef ref = tok_ref(m, a.r.c);
-        const float meq = ref.meq, mc = ref.mc, c = ref.c;
-        float S = 0.f, n = 0.f, Sl = 0.f, nl = 0.f;          // unlisted, listed (drop mode needs their sum alone)
+        tot = tok_group<G, TokSum>(tot);
+        if (tm > -INFINITY) shift = (double)tm + log(tot);
+    }
+    const bool dup = __ballot(twice) != 0;               // any row of this wave
+    __syncthreads();                                     // the marks have been read
+    double P = 0.0, kl = 0.0;
+    if (live)
+        for (int j = gl; j < K; j += G) {
+            const int64_t id = tok_int(a.ids, a.id64, row * K + j);
+            if ((uint64_t)id >= (uint64_t)V) continue;
+            const double lp = (double)a.t[row * K + j] - shift, p = exp(lp);
+            P += p;
+            if (p != 0.0) {
+                const double xv = (double)TokElem<T>::one(x[id]);
+                kl += p * (lp - (none ? -(double)INFINITY : (xv - (double)m) * a.r.dinv_t - lnS));
+            }
+            float ps = (float)p;
+            bool first = true;
+            if (dup) {
+                ps = 0.f;
+                for (int i = 0; i < K; ++i)
+                    if (tok_int(a.ids, a.id64, row * K + i) == id) {
+                        if (i < j) first = false;
+                        ps += (float)exp((double)a.t[row * K + i] - shift);
+                    }
+            }
+            if (first) mine[id] = __float_as_uint(ps);
+            if (a.pk) a.pk[row * K + j] = first && !none ? ps : -1.f;
+        }
+    P = tok_group<G, TokSum>(P);
+    kl = tok_group<G, TokSum>(kl);
+    double A = P, B = P;
+    if (a.bucket) {
+        const double p0 = rest == 0.0 ? 0.0 : 1.0 - P;
+        if (p0 > 0.0) {
+            const double lq0 = listed < rest ? log1p(-listed / sum) : log(rest / sum);
+            kl += p0 * (log(p0) - lq0);
+            A = P + p0;
+            B = A - p0 * (sum / rest);
+        }
+    }
+    DistRow d;
+    d.m = none ? 0.f : m;
+    d.l2S = none ? INFINITY : (float)(lnS * 1.4426950408889634);
+    d.A = (float)A;
+    d.B = (float)B;
+    if (there && gl == 0) {
+        a.loss[row] = live ? (float)((double)w * (double)a.T * (double)a.T * kl) : 0.f;
+        if (a.stat) a.stat[row] = live ? make_float4(d.m, d.l2S, d.A, d.B) : make_float4(0.f, INFINITY, 0.f, 0.f);
+    }
+    __syncthreads();
+    if constexpr (GRAD) {
+        if (there && gl * 8 < V) {
+            const float fw = w * a.T;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const bool is = f[e] == meq, li = mine[gl * 8 + e] != NOT_LISTED;
-            const float ev = is ? 0.f : tok_exp2(__builtin_fmaf(f[e], c, -mc));
-            S += li ? 0.f : ev;
-            Sl += li ? ev : 0.f;
-            n += is && !li ? 1.f : 0.f;
-            nl += is && li ? 1.f : 0.f;
-        }
-        S = tok_group<G, TokSum>(S);
-        Sl = tok_group<G, TokSum>(Sl);
-        n = tok_group<G, TokSum>(n);
-        nl = tok_group<G, TokSum>(nl);
-        const double sc = (double)tok_exp2(-ref.dmax);
-        const double rest = (double)n + (double)S * sc, listed = (double)nl + (double)Sl * sc;
-        double sum = rest + listed;
-        if (m == INFINITY) sum = (double)NAN;
-        const bool none = sum == 0.0;
-        const double lnS = none ? 0.0 : log(sum);
-        double shift = 0.0;
-        if (!a.bucket) {
-            tm = tok_group<G, TokMax>(tm);
-            double tot = 0.0;
-            if (live && tm > -INFINITY)
-                for (int j = gl; j < K; j += G) {
-                    const int64_t id = tok_int(a.ids, a.id64, row * K + j);
-                    if ((uint64_t)id < (uint64_t)V) tot += exp((double)a.t[row * K + j] - (double)tm);
-                }
-            tot = tok_group<G, TokSum>(tot);
-            if (tm > -INFINITY) shift = (double)tm + log(tot);
-        }
-        const bool dup = __ballot(twice) != 0;               // any row of this wave
-        __syncthreads();                                     // the marks have been read
-        double P = 0.0, kl = 0.0;
-        if (live)
-            for (int j = gl; j < K; j += G) {
-                const int64_t id = tok_int(a.ids, a.id64, row * K + j);
-                if ((uint64_t)id >= (uint64_t)V) continue;
-                const double lp = (double)a.t[row * K + j] - shift, p = exp(lp);
-                P += p;
-                if (p != 0.0) {
-                    const double xv = (double)TokElem<T>::one(x[id]);
-                    kl += p * (lp - (none ? -(double)INFINITY : (xv - (double)m) * a.r.dinv_t - lnS));
-                }
-                float ps = (float)p;
-                bool first = true;
-                if (dup) {
-                    ps = 0.f;
-                    for (int i = 0; i < K; ++i)
-                        if (tok_int(a.ids, a.id64, row * K + i) == id) {
-                            if (i < j) first = false;
-                            ps += (float)exp((double)a.t[row * K + i] - shift);
-                        }
-                }
-                if (first) mine[id] = __float_as_uint(ps);
-                if (a.pk) a.pk[row * K + j] = first && !none ? ps : -1.f;
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t pb = mine[gl * 8 + e];
+                const float q = dist_q(d, a.r.c, f[e]);
+                const float g = pb == NOT_LISTED ? d.B * q : none ? 0.f : __builtin_fmaf(d.A, q, -__uint_as_float(pb));
+                f[e] = live ? fw * g : 0.f;
             }
-        P = tok_group<G, TokSum>(P);
-        kl = tok_group<G, TokSum>(kl);
-        double A = P, B = P;
-        if (a.bucket) {
-            const double p0 = rest == 0.0 ? 0.0 : 1.0 - P;
-            if (p0 > 0.0) {
-                const double lq0 = listed < rest ? log1p(-listed / sum) : log(rest / sum);
-                kl += p0 * (log(p0) - lq0);
-                A = P + p0;
-                B = A - p0 * (sum / rest);
-            }
+            tok_narrow_store<T>((tok_out<T>)a.dx + row * V, V, gl * 8, f);
         }
-        DistRow d;
-        d.m = none ? 0.f : m;
-        d.l2S = none ? INFINITY : (float)(lnS * 1.4426950408889634);
-        d.A = (float)A;
-        d.B = (float)B;
-        if (there && gl == 0) {
-            a.loss[row] = live ? (float)((double)w * (double)a.T * (double)a.T * kl) : 0.f;
-            if (a.stat) a.stat[row] = live ? make_float4(d.m, d.l2S, d.A, d.B) : make_float4(0.f, INFINITY, 0.f, 0.f);
-        }
-        __syncthreads();
-        if constexpr (GRAD) {
-            if (there && gl * 8 < V) {
-                const float fw = w * a.T;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t pb = mine[gl * 8 + e];
-                    const float q = dist_q(d, a.r.c, f[e]);
-                    const float g = pb == NOT_LISTED ? d.B * q : none ? 0.f : __builtin_fmaf(d.A, q, -__uint_as_float(pb));
-                    f[e] = live ? fw * g : 0.f;
-                }
-                tok_narrow_store<T>(reinterpret_cast<T*>(a.dx) + row * V, V, gl * 8, f);
-            }
-        }
-        __syncthreads();                                     // the buffer is used again by the next rows
     }
 }
 
@@ -486,56 +494,54 @@ struct DistGradArgs {
     float T;
     const float *w, *g, *pk;     // g: the gradient of each row's loss
     const float4* stat;
-    void* dx;
+    int64_t dx;
 };
 
 template <typename T> __global__ __launch_bounds__(256) void tok_distill_grad_kernel(DistGradArgs a) {
     constexpr int VEC = TokElem<T>::VEC, U = 4;
     const int tid = threadIdx.x;
     const int nvec = a.r.V / VEC, ntail = a.r.V - nvec * VEC;
-    const int64_t units = a.r.rows * a.chunks;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const int64_t row = u / a.chunks;
-        const int ch = (int)(u - row * a.chunks);
-        const float w = a.w ? a.w[row] : 1.f;
-        T* o = reinterpret_cast<T*>(a.dx) + row * a.r.V;
-        const T* x = tok_row<T>(a.r, row);
-        const int b0 = ch * 256 * U;
-        const bool live = w != 0.f;
-        const float4 st = live ? a.stat[row] : make_float4(0.f, INFINITY, 0.f, 0.f);
-        const DistRow d{st.x, st.y, st.z, st.w};
-        const float f = live ? w * a.T * (a.g ? a.g[row] : 1.f) : 0.f, fB = f * d.B;
-        u32x4_t r[U];
+    const int64_t u = a.r.u0 + blockIdx.x;
+    const int64_t row = u / a.chunks;
+    const int ch = (int)(u - row * a.chunks);
+    const float w = a.w ? a.w[row] : 1.f;
+    tok_out<T> o = (tok_out<T>)a.dx + row * a.r.V;
+    tok_in<T> x = tok_row<T>(a.r, row);
+    const int b0 = ch * 256 * U;
+    const bool live = w != 0.f;
+    const float4 st = live ? a.stat[row] : make_float4(0.f, INFINITY, 0.f, 0.f);
+    const DistRow d{st.x, st.y, st.z, st.w};
+    const float f = live ? w * a.T * (a.g ? a.g[row] : 1.f) : 0.f, fB = f * d.B;
+    u32x4_t r[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int v = b0 + i * 256 + tid;
-            r[i] = u32x4_t{0, 0, 0, 0};
-            if (live && v < nvec) r[i] = tok_ld16(x + (int64_t)v * VEC);
-        }
+    for (int i = 0; i < U; ++i) {
+        const int v = b0 + i * 256 + tid;
+        r[i] = u32x4_t{0, 0, 0, 0};
+        if (live && v < nvec) r[i] = tok_ld16<T>(x + (int64_t)v * VEC);
+    }
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int v = b0 + i * 256 + tid;
-            if (v < nvec) {
-                float g[VEC];
+    for (int i = 0; i < U; ++i) {
+        const int v = b0 + i * 256 + tid;
+        if (v < nvec) {
+            float g[VEC];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) g[e] = live ? fB * dist_q(d, a.r.c, TokElem<T>::get(r[i], e)) : 0.f;
-                tok_st16(o + (int64_t)v * VEC, TokElem<T>::pack(g));
-            }
+            for (int e = 0; e < VEC; ++e) g[e] = live ? fB * dist_q(d, a.r.c, TokElem<T>::get(r[i], e)) : 0.f;
+            tok_st16<T>(o + (int64_t)v * VEC, TokElem<T>::pack(g));
         }
-        const bool last = ch == a.chunks - 1;
-        if (last && tid < ntail) {
-            const int e = nvec * VEC + tid;
-            o[e] = TokElem<T>::put(live ? fB * dist_q(d, a.r.c, TokElem<T>::one(x[e])) : 0.f);
-        }
-        __syncthreads();                                     // the listed tokens' stores follow the block's own
-        if (live) {
-            const int64_t lo = (int64_t)b0 * VEC, hi = last ? a.r.V : lo + 256 * U * VEC;
-            for (int j = tid; j < a.K; j += 256) {
-                const int64_t id = tok_int(a.ids, a.id64, row * a.K + j);
-                const float p = a.pk[row * a.K + j];
-                if (id >= lo && id < hi && p >= 0.f)
-                    o[id] = TokElem<T>::put(f * (d.A * dist_q(d, a.r.c, TokElem<T>::one(x[id])) - p));
-            }
+    }
+    const bool last = ch == a.chunks - 1;
+    if (last && tid < ntail) {
+        const int e = nvec * VEC + tid;
+        o[e] = TokElem<T>::put(live ? fB * dist_q(d, a.r.c, TokElem<T>::one(x[e])) : 0.f);
+    }
+    __syncthreads();                                     // the listed tokens' stores follow the block's own
+    if (live) {
+        const int64_t lo = (int64_t)b0 * VEC, hi = last ? a.r.V : lo + 256 * U * VEC;
+        for (int j = tid; j < a.K; j += 256) {
+            const int64_t id = tok_int(a.ids, a.id64, row * a.K + j);
+            const float p = a.pk[row * a.K + j];
+            if (id >= lo && id < hi && p >= 0.f)
+                o[id] = TokElem<T>::put(f * (d.A * dist_q(d, a.r.c, TokElem<T>::one(x[id])) - p));
         }
     }
 }
@@ -546,38 +552,37 @@ template <typename T, int G> __global__ __launch_bounds__(256) void tok_distill_
     const int gl = threadIdx.x & (G - 1), gr = threadIdx.x / G;
     uint32_t* mine = buf + gr * G * 8;
     const int V = a.r.V, K = a.K;
-    for (int64_t r0 = (int64_t)blockIdx.x * RB; r0 < a.r.rows; r0 += (int64_t)gridDim.x * RB) {
-        const int64_t row = r0 + gr;
-        const bool there = row < a.r.rows;
-        const float w = there ? (a.w ? a.w[row] : 1.f) : 0.f;
-        const bool live = there && w != 0.f;
-        float f[8];
-        tok_narrow_load<T>(live ? tok_row<T>(a.r, row) : nullptr, V, gl * 8, live, f);
+    const int64_t r0 = (a.r.u0 + blockIdx.x) * RB;
+    const int64_t row = r0 + gr;
+    const bool there = row < a.r.rows;
+    const float w = there ? (a.w ? a.w[row] : 1.f) : 0.f;
+    const bool live = there && w != 0.f;
+    float f[8];
+    tok_narrow_load<T>(live ? tok_row<T>(a.r, row) : (tok_in<T>)0, V, gl * 8, live, f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mine[gl * 8 + e] = NOT_LISTED;
-        __syncthreads();
-        if (live)
-            for (int j = gl; j < K; j += G) {
-                const int64_t id = tok_int(a.ids, a.id64, row * K + j);
-                const float p = a.pk[row * K + j];
-                if ((uint64_t)id < (uint64_t)V && p >= 0.f) mine[id] = __float_as_uint(p);
-            }
-        __syncthreads();
-        if (there && gl * 8 < V) {
-            const float4 st = live ? a.stat[row] : make_float4(0.f, INFINITY, 0.f, 0.f);
-            const DistRow d{st.x, st.y, st.z, st.w};
-            const float fw = live ? w * a.T * (a.g ? a.g[row] : 1.f) : 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t pb = mine[gl * 8 + e];
-                const float q = dist_q(d, a.r.c, f[e]);
-                const float g = pb == NOT_LISTED ? d.B * q : __builtin_fmaf(d.A, q, -__uint_as_float(pb));
-                f[e] = live ? fw * g : 0.f;
-            }
-            tok_narrow_store<T>(reinterpret_cast<T*>(a.dx) + row * V, V, gl * 8, f);
+    for (int e = 0; e < 8; ++e) mine[gl * 8 + e] = NOT_LISTED;
+    __syncthreads();
+    if (live)
+        for (int j = gl; j < K; j += G) {
+            const int64_t id = tok_int(a.ids, a.id64, row * K + j);
+            const float p = a.pk[row * K + j];
+            if ((uint64_t)id < (uint64_t)V && p >= 0.f) mine[id] = __float_as_uint(p);
         }
-        __syncthreads();
+    __syncthreads();
+    if (there && gl * 8 < V) {
+        const float4 st = live ? a.stat[row] : make_float4(0.f, INFINITY, 0.f, 0.f);
+        const DistRow d{st.x, st.y, st.z, st.w};
+        const float fw = live ? w * a.T * (a.g ? a.g[row] : 1.f) : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t pb = mine[gl * 8 + e];
+            const float q = dist_q(d, a.r.c, f[e]);
+            const float g = pb == NOT_LISTED ? d.B * q : __builtin_fmaf(d.A, q, -__uint_as_float(pb));
+            f[e] = live ? fw * g : 0.f;
+        }
+        tok_narrow_store<T>((tok_out<T>)a.dx + row * V, V, gl * 8, f);
     }
+    __syncthreads();
 }
 
 // ---- launchers -------------------------------------------------------------------------------------------------------------
@@ -596,23 +601,25 @@ int64_t tok_distill_segments(int64_t V, int dtype, int64_t rows, int grad) {
 }
 
 template <typename T, bool GRAD> static void distill_wide(const DistArgs& a, const TokPlan& p, hipStream_t s) {
-    const dim3 grid(tok_blocks(a.r.rows * p.nseg, p.nt)), blk(p.nt);
-    if (p.nt == 64 && p.nv == 2) hipLaunchKernelGGL((tok_distill_kernel<T, 64, 2, GRAD>), grid, blk, 0, s, a);
-    else if (p.nt == 64 && p.nv == 4) hipLaunchKernelGGL((tok_distill_kernel<T, 64, 4, GRAD>), grid, blk, 0, s, a);
-    else if (p.nt == 64) hipLaunchKernelGGL((tok_distill_kernel<T, 64, 8, GRAD>), grid, blk, 0, s, a);
-    else if (p.nv == 4) hipLaunchKernelGGL((tok_distill_kernel<T, 256, 4, GRAD>), grid, blk, 0, s, a);
-    else if (p.nv == 8) hipLaunchKernelGGL((tok_distill_kernel<T, 256, 8, GRAD>), grid, blk, 0, s, a);
-    else if (p.nt == 256) hipLaunchKernelGGL((tok_distill_kernel<T, 256, 16, GRAD>), grid, blk, 0, s, a);
-    else if constexpr (GRAD) hipLaunchKernelGGL((tok_distill_kernel<T, 512, 16, GRAD>), grid, blk, 0, s, a);
+    const int64_t units = a.r.rows * p.nseg;
+    const int nt = p.nt;
+    if (p.nt == 64 && p.nv == 2) tok_launch(tok_distill_kernel<T, 64, 2, GRAD>, units, nt, 0, s, a);
+    else if (p.nt == 64 && p.nv == 4) tok_launch(tok_distill_kernel<T, 64, 4, GRAD>, units, nt, 0, s, a);
+    else if (p.nt == 64) tok_launch(tok_distill_kernel<T, 64, 8, GRAD>, units, nt, 0, s, a);
+    else if (p.nv == 4) tok_launch(tok_distill_kernel<T, 256, 4, GRAD>, units, nt, 0, s, a);
+    else if (p.nv == 8) tok_launch(tok_distill_kernel<T, 256, 8, GRAD>, units, nt, 0, s, a);
+    else if (p.nt == 256) tok_launch(tok_distill_kernel<T, 256, 16, GRAD>, units, nt, 0, s, a);
+    else if constexpr (GRAD) tok_launch(tok_distill_kernel<T, 512, 16, GRAD>, units, nt, 0, s, a);
 }
 template <typename T, bool GRAD> static void distill_narrow(const DistArgs& a, hipStream_t s) {
     const int G = tok_narrow_lanes(a.r.V);
     const int64_t rb = 256 / G;
-    const dim3 grid(tok_blocks((a.r.rows + rb - 1) / rb, 256)), blk(256);
-    if (G == 8) hipLaunchKernelGGL((tok_distill_narrow_kernel<T, 8, GRAD>), grid, blk, 0, s, a);
-    else if (G == 16) hipLaunchKernelGGL((tok_distill_narrow_kernel<T, 16, GRAD>), grid, blk, 0, s, a);
-    else if (G == 32) hipLaunchKernelGGL((tok_distill_narrow_kernel<T, 32, GRAD>), grid, blk, 0, s, a);
-    else hipLaunchKernelGGL((tok_distill_narrow_kernel<T, 64, GRAD>), grid, blk, 0, s, a);
+    const int64_t units = (a.r.rows + rb - 1) / rb;
+    const int nt = 256;
+    if (G == 8) tok_launch(tok_distill_narrow_kernel<T, 8, GRAD>, units, nt, 0, s, a);
+    else if (G == 16) tok_launch(tok_distill_narrow_kernel<T, 16, GRAD>, units, nt, 0, s, a);
+    else if (G == 32) tok_launch(tok_distill_narrow_kernel<T, 32, GRAD>, units, nt, 0, s, a);
+    else tok_launch(tok_distill_narrow_kernel<T, 64, GRAD>, units, nt, 0, s, a);
 }
 template <typename T> static void distill_any(const DistArgs& a, const TokPlan* p, bool grad, hipStream_t s) {
     if (!p) grad ? distill_narrow<T, true>(a, s) : distill_narrow<T, false>(a, s);
@@ -623,15 +630,16 @@ template <typename T> static void distill_grad_any(DistGradArgs a, hipStream_t s
     if (V <= TOK_NARROW_V) {
         const int G = tok_narrow_lanes(V);
         const int64_t rb = 256 / G;
-        const dim3 grid(tok_blocks((a.r.rows + rb - 1) / rb, 256)), blk(256);
-        if (G == 8) hipLaunchKernelGGL((tok_distill_grad_narrow_kernel<T, 8>), grid, blk, 0, s, a);
-        else if (G == 16) hipLaunchKernelGGL((tok_distill_grad_narrow_kernel<T, 16>), grid, blk, 0, s, a);
-        else if (G == 32) hipLaunchKernelGGL((tok_distill_grad_narrow_kernel<T, 32>), grid, blk, 0, s, a);
-        else hipLaunchKernelGGL((tok_distill_grad_narrow_kernel<T, 64>), grid, blk, 0, s, a);
+        const int64_t units = (a.r.rows + rb - 1) / rb;
+        const int nt = 256;
+        if (G == 8) tok_launch(tok_distill_grad_narrow_kernel<T, 8>, units, nt, 0, s, a);
+        else if (G == 16) tok_launch(tok_distill_grad_narrow_kernel<T, 16>, units, nt, 0, s, a);
+        else if (G == 32) tok_launch(tok_distill_grad_narrow_kernel<T, 32>, units, nt, 0, s, a);
+        else tok_launch(tok_distill_grad_narrow_kernel<T, 64>, units, nt, 0, s, a);
         return;
     }
     a.chunks = (V / TokElem<T>::VEC + 1023) / 1024;
-    hipLaunchKernelGGL((tok_distill_grad_kernel<T>), dim3(tok_blocks(a.r.rows * a.chunks, 256)), dim3(256), 0, s, a);
+    tok_launch(tok_distill_grad_kernel<T>, a.r.rows * a.chunks, 256, 0, s, a);
 }
 
 // dtype: 0 fp32, 1 bf16, 2 fp16.  dx = 0: loss, stat and pk (for launch_tok_distill_grad).  dx: the gradient too, for a loss
@@ -652,7 +660,7 @@ void launch_tok_distill(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t
     a.bucket = bucket;
     a.T = (float)temperature;
     a.loss = as_ptr<float>(loss);
-    a.dx = as_ptr<void>(dx);
+    a.dx = (int64_t)dx;
     a.stat = as_ptr<float4>(stat);
     a.pk = as_ptr<float>(pk);
     a.nseg = 1;
@@ -670,14 +678,13 @@ void launch_tok_distill(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t
     if (dtype == 0) distill_any<float>(a, narrow ? nullptr : &p, grad, s);
     else if (dtype == 1) distill_any<bf16_t>(a, narrow ? nullptr : &p, grad, s);
     else distill_any<f16_t>(a, narrow ? nullptr : &p, grad, s);
-    SERANN_CHECK(hipGetLastError());
     if (a.nseg > 1) {
-        const dim3 grid(tok_blocks(rows, 64)), blk(64);
-        if (dtype == 0) hipLaunchKernelGGL((tok_distill_join_kernel<float>), grid, blk, 0, s, a);
-        else if (dtype == 1) hipLaunchKernelGGL((tok_distill_join_kernel<bf16_t>), grid, blk, 0, s, a);
-        else hipLaunchKernelGGL((tok_distill_join_kernel<f16_t>), grid, blk, 0, s, a);
-        SERANN_CHECK(hipGetLastError());
-    }
+        const int64_t units = rows;
+        const int nt = 64;
+        if (dtype == 0) tok_launch(tok_distill_join_kernel<float>, units, nt, 0, s, a);
+        else if (dtype == 1) tok_launch(tok_distill_join_kernel<bf16_t>, units, nt, 0, s, a);
+        else tok_launch(tok_distill_join_kernel<f16_t>, units, nt, 0, s, a);
+        }
     if (dx && !grad)
         launch_tok_distill_grad(x, dtype, rows, n1, s0, s1, V, temperature, ids, id64, w, K, 0, stat, pk, dx, stream);
 }
@@ -699,10 +706,9 @@ void launch_tok_distill_grad(uint64_t x, int dtype, int64_t rows, int64_t n1, in
     a.g = as_ptr<const float>(g);
     a.pk = as_ptr<const float>(pk);
     a.stat = as_ptr<const float4>(stat);
-    a.dx = as_ptr<void>(dx);
+    a.dx = (int64_t)dx;
     const hipStream_t s = as_stream(stream);
     if (dtype == 0) distill_grad_any<float>(a, s);
     else if (dtype == 1) distill_grad_any<bf16_t>(a, s);
     else distill_grad_any<f16_t>(a, s);
-    SERANN_CHECK(hipGetLastError());
 }

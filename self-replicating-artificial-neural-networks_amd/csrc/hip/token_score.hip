@@ -10,9 +10,9 @@
 // nothing is rescaled and nothing is read twice.  What bounds it: HBM, with ~13 of the ~15 lane operations an element that
 // 256 CUs have at 5 TB/s of bf16, so every operation an element counts (one fma to the exponent, v_max3, no canonicalisation).
 // Top k: k threads' maxima are k different elements, so the smallest of the per-wave ceil(k / waves)-th largest thread
-// maxima is a lower bound of the k-th largest element.  Elements at or above it (about 1.5 k) go to LDS and are ranked by
-// counting: no data-dependent loop.  If more than TOK_CAP reach it (thousands of equal values), k exact argmax rounds over
-// the registers replace the list: slower, never wrong.
+// maxima is a lower bound of the k-th largest element.  The vectors that reach it go to an LDS list (about 1.5 k of them);
+// their elements at or above it are ranked by counting: no data-dependent loop.  If the lists overflow (thousands of equal
+// values), k exact argmax rounds over the row replace them: slower, never wrong.
 // Narrow rows (V <= 512, the autoencoder's vocabulary): 8 to 64 lanes a row with 8 elements each; the lane's 8 keys are
 // sorted by a network and k rounds take the best head of the group.
 #include "token.h"
@@ -29,10 +29,9 @@ struct ScoreArgs {
     float4* part;                // nseg > 1: (m, n, S, W) and the sorted keys of each segment
     uint64_t* keys;
 };
-constexpr int TOK_CAP = 1024;
 
 __device__ __forceinline__ int64_t score_target(const ScoreArgs& a, int64_t row) {
-    const int64_t i0 = a.r.n1 == a.r.rows ? 0 : row / a.r.n1;
+    const int64_t i0 = a.r.n1 == a.r.rows ? 0 : (int64_t)((uint32_t)row / (uint32_t)a.r.n1);
     return tok_int(a.y, a.y64, i0 * a.t0 + (row - i0 * a.r.n1) * a.t1);
 }
 // Row statistics -> outputs that do not depend on k.  xt: the target's logit (valid_t: the target is inside the vocabulary)
@@ -65,226 +64,233 @@ __device__ __forceinline__ float score_toplp(const ScoreArgs& a, float x, float 
     return x == -INFINITY ? -INFINITY + lnS : (x - m) * a.r.inv_t - lnS;
 }
 
+// One element's share of the sums
+struct ScoreSums {
+    float S, W, n;
+    __device__ __forceinline__ void add(float x, const TokRef& ref) {
+        const float d = __builtin_fmaf(x, ref.c, -ref.mc);
+        const bool is = x == ref.meq;
+        const float e = is ? 0.f : tok_exp2(d);
+        n += is ? 1.f : 0.f;
+        S += e;
+        W = __builtin_fmaf(e, tok_max(d, -200.f), W);        // -inf: 0 * -200, not 0 * -inf
+    }
+};
+
 template <typename T, int NT, int NV>
-__global__ __launch_bounds__(NT) void tok_score_kernel(ScoreArgs a) {
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4 : 5))) void tok_score_kernel(ScoreArgs a) {
     constexpr int VEC = TokElem<T>::VEC, NW = NT / 64;
-    constexpr int CAP = TOK_CAP;
-    __shared__ float red[NW][4];
-    __shared__ uint64_t cand[CAP];
-    __shared__ int ncand;
+    // one-wave rows: 8 KB of lists a block, or LDS would keep waves away
+    constexpr int SPECIAL = NT == 64 ? 192 : 512, CAND = NT == 64 ? 512 : 1024;
+    __shared__ float red[NW][3];
     __shared__ uint64_t best[NW];
+    __shared__ TokSpecial<SPECIAL> list;
+    __shared__ uint64_t cand[CAND];
+    __shared__ int ncand;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int nvec_row = a.r.V / VEC;
-    const int64_t units = a.r.rows * a.nseg;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const int64_t row = a.nseg == 1 ? u : u / a.nseg;
-        const int seg = (int)(u - row * a.nseg);
-        int64_t tgt = 0;
-        if (a.y) {
-            tgt = score_target(a, row);
-            if (tgt == a.ignore) {
-                if (a.nseg == 1) score_skip(a, row, tid, NT);
-                continue;
+    const int64_t u = a.r.u0 + blockIdx.x;
+    const int64_t row = a.nseg == 1 ? u : u / a.nseg;
+    const int seg = (int)(u - row * a.nseg);
+    int64_t tgt = 0;
+    if (a.y) {
+        tgt = score_target(a, row);
+        if (tgt == a.ignore) {
+            if (a.nseg == 1) score_skip(a, row, tid, NT);
+            return;
+        }
+    }
+    tok_in<T> x = tok_row<T>(a.r, row);
+    const bool valid_t = !a.y || (uint64_t)tgt < (uint64_t)a.r.V;
+    float xt = 0.f;
+    if (a.y && valid_t && a.nseg == 1) xt = TokElem<T>::one(x[tgt]);
+    const int v0 = seg * a.segvec;
+    const int nv = min(a.segvec, nvec_row - v0);
+    const int ntail = seg == a.nseg - 1 ? a.r.V - nvec_row * VEC : 0;
+    const int e0 = v0 * VEC;                             // the segment's first element
+    x += e0;
+    TokSeg<T, NT, NV> s;
+    s.load(x, nv, ntail);
+    const float tm = s.max_of();
+    const float wm0 = tok_group<64, TokMax>(tm);
+    float wb = wm0;
+    if (a.k) {
+        // this wave's share of the bound: its kk-th largest thread maximum (ties counted together)
+        const int kk = NW == 1 ? a.k : (a.k + NW - 1) / NW;
+        if (kk <= 64) {
+            float cur = tm;
+            int left = kk;
+            while (true) {
+                const int hit = (int)__popcll(__ballot(cur == wb));
+                if (hit >= left || hit == 0 || wb == -INFINITY) break;     // 0: NaN
+                left -= hit;
+                cur = cur == wb ? -INFINITY : cur;
+                wb = tok_group<64, TokMax>(cur);
             }
-        }
-        const T* x = tok_row<T>(a.r, row);
-        const bool valid_t = !a.y || (uint64_t)tgt < (uint64_t)a.r.V;
-        float xt = 0.f;
-        if (a.y && valid_t && a.nseg == 1) xt = TokElem<T>::one(x[tgt]);
-        const int v0 = seg * a.segvec;
-        const int nv = min(a.segvec, nvec_row - v0);
-        const int ntail = seg == a.nseg - 1 ? a.r.V - nvec_row * VEC : 0;
-        TokSeg<T, NT, NV> s;
-        s.load(x + (int64_t)v0 * VEC, nv, ntail);
-        const float tm = s.max_of();
-        const float wm0 = tok_group<64, TokMax>(tm);
-        float wb = wm0;
-        if (a.k) {
-            // this wave's share of the bound: its kk-th largest thread maximum (ties counted together)
-            const int kk = NW == 1 ? a.k : (a.k + NW - 1) / NW;
-            if (kk <= 64) {
-                float cur = tm;
-                int left = kk;
-                wb = wm0;
-                while (true) {
-                    const int hit = (int)__popcll(__ballot(cur == wb));
-                    if (hit >= left || hit == 0 || wb == -INFINITY) break;     // 0: NaN
-                    left -= hit;
-                    cur = cur == wb ? -INFINITY : cur;
-                    wb = tok_group<64, TokMax>(cur);
-                }
-            } else {
-                // one wave, k > 64: two elements a lane (the two best vectors' maxima) at or above the smallest second one
-                float b1 = s.xt, b2 = -INFINITY;
+        } else {
+            // one wave, k > 64: two elements a lane (the two best vectors' maxima) at or above the smallest second one
+            float b1 = s.xt, b2 = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    b2 = tok_max(b2, fminf(b1, s.vm[i]));
-                    b1 = tok_max(b1, s.vm[i]);
-                }
-                wb = tok_group<64, TokMin>(b2);
+            for (int i = 0; i < NV; ++i) {
+                b2 = tok_max(b2, fminf(b1, s.vm[i]));
+                b1 = tok_max(b1, s.vm[i]);
             }
+            wb = tok_group<64, TokMin>(b2);
         }
-        if (lane == 0) {
-            red[wave][0] = wm0;
-            red[wave][1] = wb;
-        }
-        if (tid == 0) ncand = 0;
-        __syncthreads();
-        float m = red[0][0], B = red[0][1];
+    }
+    if (lane == 0) {
+        red[wave][0] = wm0;
+        red[wave][1] = wb;
+    }
+    if (tid == 0) list.n = ncand = 0;
+    __syncthreads();
+    float m = red[0][0], B = red[0][1];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) {
-            m = tok_max(m, red[w][0]);
-            B = fminf(B, red[w][1]);
-        }
-        const TokRef ref = tok_ref(m, a.r.c);
-        const float meq = ref.meq, mc = ref.mc, c = ref.c;
-        float S = 0.f, W = 0.f, n = 0.f;
+    for (int w = 1; w < NW; ++w) {
+        m = tok_max(m, red[w][0]);
+        B = fminf(B, red[w][1]);
+    }
+    const TokRef ref = tok_ref(m, a.r.c);
+    ScoreSums sum{0.f, 0.f, 0.f};
+    int chain = -1;
+    if (B > -INFINITY) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (i * NT < nv) {
                 float cs = 0.f, cw = 0.f;
-                if (s.vm[i] == meq) {                        // a few lanes a row: leave the maximum out, count it
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float xv = TokElem<T>::get(s.r[i], e);
-                        const float d = __builtin_fmaf(xv, c, -mc);
-                        const bool is = xv == meq;
-                        const float ev = is ? 0.f : tok_exp2(d);
-                        n += is ? 1.f : 0.f;
-                        cs += ev;
-                        cw = __builtin_fmaf(ev, tok_max(d, -200.f), cw);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float d = __builtin_fmaf(TokElem<T>::get(s.r[i], e), c, -mc);
-                        const float ev = tok_exp2(d);
-                        cs += ev;
-                        cw = __builtin_fmaf(ev, tok_max(d, -200.f), cw);      // -inf: 0 * -200, not 0 * -inf
-                    }
+                for (int e = 0; e < VEC; ++e) {
+                    const float d = __builtin_fmaf(TokElem<T>::get(s.r[i], e), ref.c, -ref.mc);
+                    const float ev = tok_exp2(d);
+                    cs += ev;
+                    cw = __builtin_fmaf(ev, tok_max(d, -200.f), cw);
                 }
-                S += cs;
-                W += cw;
-                if (a.k && s.vm[i] >= B && i * NT + tid < nv) {
-                    const int base = (v0 + i * NT + tid) * VEC;
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float xv = TokElem<T>::get(s.r[i], e);
-                        if (xv >= B) {
-                            const int at = atomicAdd(&ncand, 1);
-                            if (at < CAP) cand[at] = tok_key(xv, base + e);
-                        }
-                    }
-                }
+                const bool top = s.vm[i] == m;
+                if (s.vm[i] >= B) list.push(s.r[i], i * NT + tid, top, chain);
+                sum.S += top ? 0.f : cs;
+                sum.W += top ? 0.f : cw;
             }
         }
-        if (tid < ntail) {
-            const float d = __builtin_fmaf(s.xt, c, -mc);
-            const bool is = s.xt == meq;
-            const float ev = is ? 0.f : tok_exp2(d);
-            n += is ? 1.f : 0.f;
-            S += ev;
-            W = __builtin_fmaf(ev, tok_max(d, -200.f), W);
-            if (a.k && s.xt >= B) {
-                const int at = atomicAdd(&ncand, 1);
-                if (at < CAP) cand[at] = tok_key(s.xt, v0 * VEC + s.tail0 + tid);
+    }
+    __syncthreads();
+    const int nl = list.n;
+    const bool slow = !(B > -INFINITY) || nl > SPECIAL;
+    if (!slow) {
+        for (; chain >= 0; chain = list.next[chain])
+            if (list.at[chain] < 0)
+                for (int e = 0; e < VEC; ++e) sum.add(list.template get<T>(chain, e), ref);
+        if (a.k)
+            for (int i = tid; i < nl * VEC; i += NT) {
+                const int slot = i / VEC, e = i & (VEC - 1);
+                const float xv = list.template get<T>(slot, e);
+                if (xv >= B) {
+                    const int at = atomicAdd(&ncand, 1);
+                    if (at < CAND) cand[at] = tok_key(xv, e0 + list.vec(slot) * VEC + e);
+                }
             }
-        }
-        S = tok_group<64, TokSum>(S);
-        W = tok_group<64, TokSum>(W);
-        n = tok_group<64, TokSum>(n);
-        __syncthreads();                                    // red is read above, written below; the candidates are complete
-        if (lane == 0) {
-            red[wave][0] = S;
-            red[wave][1] = W;
-            red[wave][2] = n;
-        }
-        __syncthreads();
-        S = red[0][0];
-        W = red[0][1];
-        n = red[0][2];
+    } else {
+        // thousands of vectors at the bound (equal values), or fewer than k elements left: element by element, read again
+        sum = ScoreSums{0.f, 0.f, 0.f};
+        for (int v = tid; v < nv; v += NT) {
+            const u32x4_t r = tok_ld16<T>(x + (int64_t)v * VEC);
 #pragma unroll
-        for (int w = 1; w < NW; ++w) {
-            S += red[w][0];
-            W += red[w][1];
-            n += red[w][2];
+            for (int e = 0; e < VEC; ++e) sum.add(TokElem<T>::get(r, e), ref);
         }
-        const float sc = tok_exp2(-ref.dmax);
-        W = (W - ref.dmax * S) * sc;
-        S *= sc;
-        if (m == INFINITY) S = NAN;
-        float lnS = 0.f;
-        if (a.nseg == 1)
-            lnS = score_finish(a, row, m, n, S, W, xt, valid_t, tid == 0);
-        else if (tid == 0)
-            a.part[u] = make_float4(m, n, S, W);
-        if (a.k) {
-            // a row (or segment) with a NaN or +inf logit has no ranking
-            const int nc = S == S ? ncand : 0;
-            if (nc <= CAP) {
-                for (int i = tid; i < nc; i += NT) {
-                    const uint64_t key = cand[i];
-                    int rank = 0;
-                    for (int j = 0; j < nc; ++j) rank += cand[j] > key;
-                    if (rank < a.k) {
-                        if (a.nseg == 1) {
-                            a.ids[row * a.k + rank] = tok_key_index(key);
-                            a.top[row * a.k + rank] = score_toplp(a, tok_key_value(key), m, lnS);
-                        } else {
-                            a.keys[u * a.k + rank] = key;
-                        }
+    }
+    if (tid < ntail) {
+        sum.add(s.xt, ref);
+        if (a.k && s.xt >= B && !slow) {
+            const int at = atomicAdd(&ncand, 1);
+            if (at < CAND) cand[at] = tok_key(s.xt, e0 + nv * VEC + tid);
+        }
+    }
+    float S = tok_group<64, TokSum>(sum.S), W = tok_group<64, TokSum>(sum.W), n = tok_group<64, TokSum>(sum.n);
+    if (lane == 0) {                                     // red was read before the barrier above
+        red[wave][0] = S;
+        red[wave][1] = W;
+        red[wave][2] = n;
+    }
+    __syncthreads();                                     // the sums and the candidates are complete
+    S = red[0][0];
+    W = red[0][1];
+    n = red[0][2];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) {
+        S += red[w][0];
+        W += red[w][1];
+        n += red[w][2];
+    }
+    const float sc = tok_exp2(-ref.dmax);
+    W = (W - ref.dmax * S) * sc;
+    S *= sc;
+    if (m == INFINITY) S = NAN;
+    float lnS = 0.f;
+    if (a.nseg == 1)
+        lnS = score_finish(a, row, m, n, S, W, xt, valid_t, tid == 0);
+    else if (tid == 0)
+        a.part[u] = make_float4(m, n, S, W);
+    if (a.k) {
+        // a row (or segment) with a NaN or +inf logit has no ranking
+        const int nc = S == S ? (slow ? CAND + 1 : ncand) : 0;
+        int done = nc < a.k ? nc : a.k;
+        if (nc <= CAND) {
+            for (int i = tid; i < nc; i += NT) {
+                const uint64_t key = cand[i];
+                int rank = 0;
+                for (int j = 0; j < nc; ++j) rank += cand[j] > key;
+                if (rank < a.k) {
+                    if (a.nseg == 1) {
+                        a.ids[row * a.k + rank] = tok_key_index(key);
+                        a.top[row * a.k + rank] = score_toplp(a, tok_key_value(key), m, lnS);
+                    } else {
+                        a.keys[u * a.k + rank] = key;
                     }
                 }
             }
-            int done = nc < a.k ? nc : a.k;
-            if (nc > CAP) {
-                // too many elements at the bound: k rounds of the largest key below the last one
-                uint64_t last = ~0ull;
-                for (done = 0; done < a.k; ++done) {
-                    uint64_t bk = 0;
+        } else {
+            // k rounds of the largest key below the last one, read again (L2); an exhausted segment yields key 0
+            uint64_t last = ~0ull;
+            for (done = 0; done < a.k; ++done) {
+                uint64_t bk = 0;
+                for (int v = tid; v < nv; v += NT) {
+                    const u32x4_t r = tok_ld16<T>(x + (int64_t)v * VEC);
 #pragma unroll
-                    for (int i = 0; i < NV; ++i)
-                        if (i * NT + tid < nv && s.vm[i] >= B) {
-                            const int base = (v0 + i * NT + tid) * VEC;
-#pragma unroll
-                            for (int e = 0; e < VEC; ++e) {
-                                const float xv = TokElem<T>::get(s.r[i], e);
-                                const uint64_t key = tok_key(xv, base + e);
-                                if (xv >= B && key < last && key > bk) bk = key;
-                            }
-                        }
-                    if (tid < ntail && s.xt >= B) {
-                        const uint64_t key = tok_key(s.xt, v0 * VEC + s.tail0 + tid);
+                    for (int e = 0; e < VEC; ++e) {
+                        const uint64_t key = tok_key(TokElem<T>::get(r, e), e0 + v * VEC + e);
                         if (key < last && key > bk) bk = key;
                     }
-                    bk = tok_group<64, TokTop>(bk);
-                    if (lane == 0) best[wave] = bk;
-                    __syncthreads();
-                    bk = best[0];
+                }
+                if (tid < ntail) {
+                    const uint64_t key = tok_key(s.xt, e0 + nv * VEC + tid);
+                    if (key < last && key > bk) bk = key;
+                }
+                bk = tok_group<64, TokTop>(bk);
+                if (lane == 0) best[wave] = bk;
+                __syncthreads();
+                bk = best[0];
 #pragma unroll
-                    for (int w = 1; w < NW; ++w) bk = best[w] > bk ? best[w] : bk;
-                    __syncthreads();
-                    last = bk;
-                    if (tid == 0) {
-                        if (a.nseg == 1) {
-                            a.ids[row * a.k + done] = tok_key_index(bk);
-                            a.top[row * a.k + done] = score_toplp(a, tok_key_value(bk), m, lnS);
-                        } else {
-                            a.keys[u * a.k + done] = bk;
-                        }
+                for (int w = 1; w < NW; ++w) bk = best[w] > bk ? best[w] : bk;
+                __syncthreads();
+                if (bk == 0) break;
+                last = bk;
+                if (tid == 0) {
+                    if (a.nseg == 1) {
+                        a.ids[row * a.k + done] = tok_key_index(bk);
+                        a.top[row * a.k + done] = score_toplp(a, tok_key_value(bk), m, lnS);
+                    } else {
+                        a.keys[u * a.k + done] = bk;
                     }
                 }
             }
-            for (int j = done + tid; j < a.k; j += NT) {     // fewer than k elements that are not NaN
-                if (a.nseg == 1) {
-                    a.ids[row * a.k + j] = -1;
-                    a.top[row * a.k + j] = NAN;
-                } else {
-                    a.keys[u * a.k + j] = 0;
-                }
+        }
+        for (int j = done + tid; j < a.k; j += NT) {     // fewer than k elements
+            if (a.nseg == 1) {
+                a.ids[row * a.k + j] = -1;
+                a.top[row * a.k + j] = NAN;
+            } else {
+                a.keys[u * a.k + j] = 0;
             }
         }
-        __syncthreads();                                    // LDS is used again by the next row
     }
 }
 
@@ -293,85 +299,84 @@ __global__ __launch_bounds__(NT) void tok_score_kernel(ScoreArgs a) {
 __global__ __launch_bounds__(256) void tok_score_join_kernel(ScoreArgs a, int esize_code) {
     extern __shared__ uint64_t lists[];
     const int tid = threadIdx.x;
-    for (int64_t row = blockIdx.x; row < a.r.rows; row += gridDim.x) {
-        int64_t tgt = 0;
-        if (a.y) {
-            tgt = score_target(a, row);
-            if (tgt == a.ignore) {
-                score_skip(a, row, tid, 256);
-                continue;
-            }
+    const int64_t row = a.r.u0 + blockIdx.x;
+    int64_t tgt = 0;
+    if (a.y) {
+        tgt = score_target(a, row);
+        if (tgt == a.ignore) {
+            score_skip(a, row, tid, 256);
+            return;
         }
-        const bool valid_t = !a.y || (uint64_t)tgt < (uint64_t)a.r.V;
-        float xt = 0.f;
-        if (a.y && valid_t) {
-            xt = esize_code == 0 ? tok_row<float>(a.r, row)[tgt]
-                                 : esize_code == 1 ? bf2f(tok_row<bf16_t>(a.r, row)[tgt]) : (float)tok_row<f16_t>(a.r, row)[tgt];
+    }
+    const bool valid_t = !a.y || (uint64_t)tgt < (uint64_t)a.r.V;
+    float xt = 0.f;
+    if (a.y && valid_t) {
+        xt = esize_code == 0 ? tok_row<float>(a.r, row)[tgt]
+                             : esize_code == 1 ? bf2f(tok_row<bf16_t>(a.r, row)[tgt]) : (float)tok_row<f16_t>(a.r, row)[tgt];
+    }
+    const float4* part = a.part + row * a.nseg;
+    float m = -INFINITY;
+    for (int s = 0; s < a.nseg; ++s) m = tok_max(m, part[s].x);
+    float S = 0.f, W = 0.f, n = 0.f;
+    for (int s = 0; s < a.nseg; ++s) {
+        const float4 p = part[s];
+        if (p.x == m) {
+            n += p.y;
+            S += p.z;
+            W += p.w;
+        } else if (p.x > -INFINITY) {
+            const float d = (p.x - m) * a.r.c, f = tok_exp2(d);
+            S += (p.y + p.z) * f;
+            W += f > 0.f ? f * (p.w + tok_max(d, -200.f) * (p.y + p.z)) : 0.f;
+        } else {
+            S += p.z;                                   // 0, or NaN
         }
-        const float4* part = a.part + row * a.nseg;
-        float m = -INFINITY;
-        for (int s = 0; s < a.nseg; ++s) m = tok_max(m, part[s].x);
-        float S = 0.f, W = 0.f, n = 0.f;
-        for (int s = 0; s < a.nseg; ++s) {
-            const float4 p = part[s];
-            if (p.x == m) {
-                n += p.y;
-                S += p.z;
-                W += p.w;
-            } else if (p.x > -INFINITY) {
-                const float d = (p.x - m) * a.r.c, f = tok_exp2(d);
-                S += (p.y + p.z) * f;
-                W += f > 0.f ? f * (p.w + tok_max(d, -200.f) * (p.y + p.z)) : 0.f;
-            } else {
-                S += p.z;                                   // 0, or NaN
-            }
-        }
-        const float lnS = score_finish(a, row, m, n, S, W, xt, valid_t, tid == 0);
-        if (a.k) {
-            const int nk = a.nseg * a.k;
-            const uint64_t* keys = a.keys + row * nk;
-            for (int i = tid; i < nk; i += 256) lists[i] = keys[i];
-            __syncthreads();
-            for (int i = tid; i < nk; i += 256) {
-                const uint64_t key = lists[i];
-                const int own = i / a.k;
-                if (key == 0 || S != S) continue;
-                int rank = i - own * a.k;
-                for (int s = 0; s < a.nseg && rank < a.k; ++s) {
-                    if (s == own) continue;
-                    const uint64_t* l = lists + s * a.k;
-                    int lo = 0, hi = a.k;                    // keys larger than `key`: a prefix of the sorted list
-                    while (lo < hi) {
-                        const int mid = (lo + hi) >> 1;
-                        if (l[mid] > key) lo = mid + 1;
-                        else hi = mid;
-                    }
-                    rank += lo;
-                }
-                if (rank < a.k) {
-                    a.ids[row * a.k + rank] = tok_key_index(key);
-                    a.top[row * a.k + rank] = score_toplp(a, tok_key_value(key), m, lnS);
-                }
-            }
-            // fewer than k elements that are not NaN: every key that there is has been placed, the rest is filled
-            int have = 0;
-            for (int s = 0; s < a.nseg && S == S; ++s) {
+    }
+    const float lnS = score_finish(a, row, m, n, S, W, xt, valid_t, tid == 0);
+    if (a.k) {
+        const int nk = a.nseg * a.k;
+        const uint64_t* keys = a.keys + row * nk;
+        for (int i = tid; i < nk; i += 256) lists[i] = keys[i];
+        __syncthreads();
+        for (int i = tid; i < nk; i += 256) {
+            const uint64_t key = lists[i];
+            const int own = i / a.k;
+            if (key == 0 || S != S) continue;
+            int rank = i - own * a.k;
+            for (int s = 0; s < a.nseg && rank < a.k; ++s) {
+                if (s == own) continue;
                 const uint64_t* l = lists + s * a.k;
-                int lo = 0, hi = a.k;
+                int lo = 0, hi = a.k;                    // keys larger than `key`: a prefix of the sorted list
                 while (lo < hi) {
                     const int mid = (lo + hi) >> 1;
-                    if (l[mid] != 0) lo = mid + 1;
+                    if (l[mid] > key) lo = mid + 1;
                     else hi = mid;
                 }
-                have += lo;
-                if (have >= a.k) break;
+                rank += lo;
             }
-            for (int j = have + tid; j < a.k; j += 256) {
-                a.ids[row * a.k + j] = -1;
-                a.top[row * a.k + j] = NAN;
+            if (rank < a.k) {
+                a.ids[row * a.k + rank] = tok_key_index(key);
+                a.top[row * a.k + rank] = score_toplp(a, tok_key_value(key), m, lnS);
             }
-            __syncthreads();
         }
+        // fewer than k elements that are not NaN: every key that there is has been placed, the rest is filled
+        int have = 0;
+        for (int s = 0; s < a.nseg && S == S; ++s) {
+            const uint64_t* l = lists + s * a.k;
+            int lo = 0, hi = a.k;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (l[mid] != 0) lo = mid + 1;
+                else hi = mid;
+            }
+            have += lo;
+            if (have >= a.k) break;
+        }
+        for (int j = have + tid; j < a.k; j += 256) {
+            a.ids[row * a.k + j] = -1;
+            a.top[row * a.k + j] = NAN;
+        }
+        __syncthreads();
     }
 }
 
@@ -419,73 +424,62 @@ __global__ __launch_bounds__(256) void tok_score_narrow_kernel(ScoreArgs a) {
     constexpr int RB = 256 / G;
     const int gl = threadIdx.x & (G - 1), gr = threadIdx.x / G;
     const int V = a.r.V;
-    for (int64_t r0 = (int64_t)blockIdx.x * RB; r0 < a.r.rows; r0 += (int64_t)gridDim.x * RB) {
-        const int64_t row = r0 + gr;
-        const bool there = row < a.r.rows;
-        int64_t tgt = 0;
-        if (a.y && there) tgt = score_target(a, row);
-        const bool skip = a.y && tgt == a.ignore;
-        const bool live = there && !skip;
-        const bool valid_t = !a.y || (uint64_t)tgt < (uint64_t)V;
-        const T* x = live ? tok_row<T>(a.r, row) : nullptr;
-        float xt = 0.f;
-        if (live && a.y && valid_t && gl == 0) xt = TokElem<T>::one(x[tgt]);
-        float f[8];
-        tok_narrow_load<T>(x, V, gl * 8, live, f);
-        float m = tok_max(tok_max3(tok_max3(f[0], f[1], f[2]), f[3], f[4]), tok_max3(f[5], f[6], f[7]));
-        m = tok_group<G, TokMax>(m);
-        const TokRef ref = tok_ref(m, a.r.c);
-        const float meq = ref.meq, mc = ref.mc, c = ref.c;
-        float S = 0.f, W = 0.f, n = 0.f;
+    const int64_t r0 = (a.r.u0 + blockIdx.x) * RB;
+    const int64_t row = r0 + gr;
+    const bool there = row < a.r.rows;
+    int64_t tgt = 0;
+    if (a.y && there) tgt = score_target(a, row);
+    const bool skip = a.y && tgt == a.ignore;
+    const bool live = there && !skip;
+    const bool valid_t = !a.y || (uint64_t)tgt < (uint64_t)V;
+    tok_in<T> x = live ? tok_row<T>(a.r, row) : (tok_in<T>)0;
+    float xt = 0.f;
+    if (live && a.y && valid_t && gl == 0) xt = TokElem<T>::one(x[tgt]);
+    float f[8];
+    tok_narrow_load<T>(x, V, gl * 8, live, f);
+    float m = tok_max(tok_max3(tok_max3(f[0], f[1], f[2]), f[3], f[4]), tok_max3(f[5], f[6], f[7]));
+    m = tok_group<G, TokMax>(m);
+    const TokRef ref = tok_ref(m, a.r.c);
+    ScoreSums sum{0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum.add(f[e], ref);
+    float S = tok_group<G, TokSum>(sum.S), W = tok_group<G, TokSum>(sum.W), n = tok_group<G, TokSum>(sum.n);
+    const float sc = tok_exp2(-ref.dmax);
+    W = (W - ref.dmax * S) * sc;
+    S *= sc;
+    if (m == INFINITY) S = NAN;
+    float lnS = 0.f;
+    if (live) lnS = score_finish(a, row, m, n, S, W, xt, valid_t, gl == 0);
+    else if (there) score_skip(a, row, gl, G);
+    if (a.k) {
+        K h[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float d = __builtin_fmaf(f[e], c, -mc);
-            const bool is = f[e] == meq;
-            const float ev = is ? 0.f : tok_exp2(d);
-            n += is ? 1.f : 0.f;
-            S += ev;
-            W = __builtin_fmaf(ev, tok_max(d, -200.f), W);
+            // NaN and what lies behind the row are not ranked: key 0
+            const bool in = gl * 8 + e < V && f[e] == f[e];
+            h[e] = in ? NK::make(f[e], gl * 8 + e) : (K)0;
         }
-        S = tok_group<G, TokSum>(S);
-        W = tok_group<G, TokSum>(W);
-        n = tok_group<G, TokSum>(n);
-        const float sc = tok_exp2(-ref.dmax);
-        W = (W - ref.dmax * S) * sc;
-        S *= sc;
-        if (m == INFINITY) S = NAN;
-        float lnS = 0.f;
-        if (live) lnS = score_finish(a, row, m, n, S, W, xt, valid_t, gl == 0);
-        else if (there) score_skip(a, row, gl, G);
-        if (a.k) {
-            K h[8];
+        // Batcher's odd-even merge sort of 8, largest first
+        order2(h[0], h[1]); order2(h[2], h[3]); order2(h[4], h[5]); order2(h[6], h[7]);
+        order2(h[0], h[2]); order2(h[1], h[3]); order2(h[4], h[6]); order2(h[5], h[7]);
+        order2(h[1], h[2]); order2(h[5], h[6]);
+        order2(h[0], h[4]); order2(h[1], h[5]); order2(h[2], h[6]); order2(h[3], h[7]);
+        order2(h[2], h[4]); order2(h[3], h[5]);
+        order2(h[1], h[2]); order2(h[3], h[4]); order2(h[5], h[6]);
+        K keep = 0;
+        for (int j = 0; j < a.k; ++j) {
+            const K top = tok_group<G, TokTop>(h[0]);
+            if (top == h[0]) {                           // keys differ, so one lane's head goes (or all are 0)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                // NaN and what lies behind the row are not ranked: key 0
-                const bool in = gl * 8 + e < V && f[e] == f[e];
-                h[e] = in ? NK::make(f[e], gl * 8 + e) : (K)0;
+                for (int e = 0; e < 7; ++e) h[e] = h[e + 1];
+                h[7] = 0;
             }
-            // Batcher's odd-even merge sort of 8, largest first
-            order2(h[0], h[1]); order2(h[2], h[3]); order2(h[4], h[5]); order2(h[6], h[7]);
-            order2(h[0], h[2]); order2(h[1], h[3]); order2(h[4], h[6]); order2(h[5], h[7]);
-            order2(h[1], h[2]); order2(h[5], h[6]);
-            order2(h[0], h[4]); order2(h[1], h[5]); order2(h[2], h[6]); order2(h[3], h[7]);
-            order2(h[2], h[4]); order2(h[3], h[5]);
-            order2(h[1], h[2]); order2(h[3], h[4]); order2(h[5], h[6]);
-            K keep = 0;
-            for (int j = 0; j < a.k; ++j) {
-                const K top = tok_group<G, TokTop>(h[0]);
-                if (top == h[0]) {                           // keys differ, so one lane's head goes (or all are 0)
-#pragma unroll
-                    for (int e = 0; e < 7; ++e) h[e] = h[e + 1];
-                    h[7] = 0;
-                }
-                if ((j & (G - 1)) == gl) keep = S == S ? top : (K)0;
-                if ((j & (G - 1)) == G - 1 || j == a.k - 1) {
-                    const int at = (j & ~(G - 1)) + gl;      // G results at a time, one a lane
-                    if (live && at <= j) {
-                        a.ids[row * a.k + at] = keep ? NK::index(keep) : -1;
-                        a.top[row * a.k + at] = keep ? score_toplp(a, NK::value(keep), m, lnS) : NAN;
-                    }
+            if ((j & (G - 1)) == gl) keep = S == S ? top : (K)0;
+            if ((j & (G - 1)) == G - 1 || j == a.k - 1) {
+                const int at = (j & ~(G - 1)) + gl;      // G results at a time, one a lane
+                if (live && at <= j) {
+                    a.ids[row * a.k + at] = keep ? NK::index(keep) : -1;
+                    a.top[row * a.k + at] = keep ? score_toplp(a, NK::value(keep), m, lnS) : NAN;
                 }
             }
         }
@@ -499,7 +493,7 @@ struct ScoreGradArgs {
     int y64, chunks;
     const float *glp, *gent, *ent;   // glp / gent: 0 = no such gradient
     const float2* stat;
-    void* dx;                        // [rows][V]
+    int64_t dx;                      // [rows][V]
 };
 // dx = ( gl [v = target] - q (gl + gh (ln q + H)) ) / T,  log2 q = fma(x - m, c, -l2S)
 struct ScoreCoef {
@@ -530,44 +524,42 @@ __global__ __launch_bounds__(256) void tok_score_grad_kernel(ScoreGradArgs a) {
     constexpr int VEC = TokElem<T>::VEC, U = 4;
     const int tid = threadIdx.x;
     const int nvec = a.r.V / VEC, ntail = a.r.V - nvec * VEC;
-    const int64_t units = a.r.rows * a.chunks;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const int64_t row = u / a.chunks;
-        const int ch = (int)(u - row * a.chunks);
-        const int64_t i0 = a.r.n1 == a.r.rows ? 0 : row / a.r.n1;
-        const int64_t tgt = a.y ? tok_int(a.y, a.y64, i0 * a.t0 + (row - i0 * a.r.n1) * a.t1) : 0;
-        const bool skip = a.y && tgt == a.ignore, valid_t = !a.y || (uint64_t)tgt < (uint64_t)a.r.V;
-        T* o = reinterpret_cast<T*>(a.dx) + row * a.r.V;
-        const T* x = tok_row<T>(a.r, row);
-        const int b0 = ch * 256 * U;
-        ScoreCoef k{};
-        if (!skip) k = score_coef(a, row, valid_t);
-        const int tv = a.y ? (int)tgt / VEC : -1, te = a.y ? (int)tgt - tv * VEC : 0;
-        u32x4_t r[U];
+    const int64_t u = a.r.u0 + blockIdx.x;
+    const int64_t row = u / a.chunks;
+    const int ch = (int)(u - row * a.chunks);
+    const int64_t i0 = a.r.n1 == a.r.rows ? 0 : (int64_t)((uint32_t)row / (uint32_t)a.r.n1);
+    const int64_t tgt = a.y ? tok_int(a.y, a.y64, i0 * a.t0 + (row - i0 * a.r.n1) * a.t1) : 0;
+    const bool skip = a.y && tgt == a.ignore, valid_t = !a.y || (uint64_t)tgt < (uint64_t)a.r.V;
+    tok_out<T> o = (tok_out<T>)a.dx + row * a.r.V;
+    tok_in<T> x = tok_row<T>(a.r, row);
+    const int b0 = ch * 256 * U;
+    ScoreCoef k{};
+    if (!skip) k = score_coef(a, row, valid_t);
+    const int tv = a.y ? (int)tgt / VEC : -1, te = a.y ? (int)tgt - tv * VEC : 0;
+    u32x4_t r[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int v = b0 + i * 256 + tid;
-            if (!skip && v < nvec) r[i] = tok_ld16(x + (int64_t)v * VEC);
+    for (int i = 0; i < U; ++i) {
+        const int v = b0 + i * 256 + tid;
+        if (!skip && v < nvec) r[i] = tok_ld16<T>(x + (int64_t)v * VEC);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int v = b0 + i * 256 + tid;
+        if (v < nvec) {
+            float f[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) f[e] = skip ? 0.f : score_dx(k, a.r.c, TokElem<T>::get(r[i], e));
+            if (!skip && v == tv)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) f[e] += e == te ? k.gl : 0.f;
+            tok_st16<T>(o + (int64_t)v * VEC, TokElem<T>::pack(f));
         }
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int v = b0 + i * 256 + tid;
-            if (v < nvec) {
-                float f[VEC];
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) f[e] = skip ? 0.f : score_dx(k, a.r.c, TokElem<T>::get(r[i], e));
-                if (!skip && v == tv)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) f[e] += e == te ? k.gl : 0.f;
-                tok_st16(o + (int64_t)v * VEC, TokElem<T>::pack(f));
-            }
-        }
-        if (ch == a.chunks - 1 && tid < ntail) {
-            const int e = nvec * VEC + tid;
-            float f = 0.f;
-            if (!skip) f = score_dx(k, a.r.c, TokElem<T>::one(x[e])) + (a.y && e == (int)tgt ? k.gl : 0.f);
-            o[e] = TokElem<T>::put(f);
-        }
+    }
+    if (ch == a.chunks - 1 && tid < ntail) {
+        const int e = nvec * VEC + tid;
+        float f = 0.f;
+        if (!skip) f = score_dx(k, a.r.c, TokElem<T>::one(x[e])) + (a.y && e == (int)tgt ? k.gl : 0.f);
+        o[e] = TokElem<T>::put(f);
     }
 }
 
@@ -576,28 +568,27 @@ __global__ __launch_bounds__(256) void tok_score_grad_narrow_kernel(ScoreGradArg
     constexpr int RB = 256 / G;
     const int gl = threadIdx.x & (G - 1), gr = threadIdx.x / G;
     const int V = a.r.V;
-    for (int64_t r0 = (int64_t)blockIdx.x * RB; r0 < a.r.rows; r0 += (int64_t)gridDim.x * RB) {
-        const int64_t row = r0 + gr;
-        if (row >= a.r.rows) continue;
-        const int64_t i0 = a.r.n1 == a.r.rows ? 0 : row / a.r.n1;
-        const int64_t tgt = a.y ? tok_int(a.y, a.y64, i0 * a.t0 + (row - i0 * a.r.n1) * a.t1) : 0;
-        const bool skip = a.y && tgt == a.ignore, valid_t = !a.y || (uint64_t)tgt < (uint64_t)V;
-        if (gl * 8 >= V) continue;
-        float f[8];
-        tok_narrow_load<T>(tok_row<T>(a.r, row), V, gl * 8, !skip, f);
-        if (skip) {
+    const int64_t r0 = (a.r.u0 + blockIdx.x) * RB;
+    const int64_t row = r0 + gr;
+    if (row >= a.r.rows) return;
+    const int64_t i0 = a.r.n1 == a.r.rows ? 0 : (int64_t)((uint32_t)row / (uint32_t)a.r.n1);
+    const int64_t tgt = a.y ? tok_int(a.y, a.y64, i0 * a.t0 + (row - i0 * a.r.n1) * a.t1) : 0;
+    const bool skip = a.y && tgt == a.ignore, valid_t = !a.y || (uint64_t)tgt < (uint64_t)V;
+    if (gl * 8 >= V) return;
+    float f[8];
+    tok_narrow_load<T>(tok_row<T>(a.r, row), V, gl * 8, !skip, f);
+    if (skip) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = 0.f;
-        } else {
-            const ScoreCoef k = score_coef(a, row, valid_t);
+        for (int e = 0; e < 8; ++e) f[e] = 0.f;
+    } else {
+        const ScoreCoef k = score_coef(a, row, valid_t);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                f[e] = score_dx(k, a.r.c, f[e]);
-                if (a.y && gl * 8 + e == (int)tgt) f[e] += k.gl;
-            }
+        for (int e = 0; e < 8; ++e) {
+            f[e] = score_dx(k, a.r.c, f[e]);
+            if (a.y && gl * 8 + e == (int)tgt) f[e] += k.gl;
         }
-        tok_narrow_store<T>(reinterpret_cast<T*>(a.dx) + row * V, V, gl * 8, f);
     }
+    tok_narrow_store<T>((tok_out<T>)a.dx + row * V, V, gl * 8, f);
 }
 
 // ---- launchers ---------------------------------------------------------------------------------------------------------
@@ -609,32 +600,35 @@ int64_t tok_score_segments(int64_t V, int dtype, int64_t rows) {
 }
 
 template <typename T> static void score_wide(const ScoreArgs& a, const TokPlan& p, hipStream_t s) {
-    const dim3 grid(tok_blocks(a.r.rows * p.nseg, p.nt)), blk(p.nt);
-    if (p.nt == 64 && p.nv == 2) hipLaunchKernelGGL((tok_score_kernel<T, 64, 2>), grid, blk, 0, s, a);
-    else if (p.nt == 64 && p.nv == 4) hipLaunchKernelGGL((tok_score_kernel<T, 64, 4>), grid, blk, 0, s, a);
-    else if (p.nt == 64) hipLaunchKernelGGL((tok_score_kernel<T, 64, 8>), grid, blk, 0, s, a);
-    else if (p.nv == 4) hipLaunchKernelGGL((tok_score_kernel<T, 256, 4>), grid, blk, 0, s, a);
-    else if (p.nv == 8) hipLaunchKernelGGL((tok_score_kernel<T, 256, 8>), grid, blk, 0, s, a);
-    else hipLaunchKernelGGL((tok_score_kernel<T, 256, 16>), grid, blk, 0, s, a);
+    const int64_t units = a.r.rows * p.nseg;
+    const int nt = p.nt;
+    if (p.nt == 64 && p.nv == 2) tok_launch(tok_score_kernel<T, 64, 2>, units, nt, 0, s, a);
+    else if (p.nt == 64 && p.nv == 4) tok_launch(tok_score_kernel<T, 64, 4>, units, nt, 0, s, a);
+    else if (p.nt == 64) tok_launch(tok_score_kernel<T, 64, 8>, units, nt, 0, s, a);
+    else if (p.nv == 4) tok_launch(tok_score_kernel<T, 256, 4>, units, nt, 0, s, a);
+    else if (p.nv == 8) tok_launch(tok_score_kernel<T, 256, 8>, units, nt, 0, s, a);
+    else tok_launch(tok_score_kernel<T, 256, 16>, units, nt, 0, s, a);
 }
 template <typename T> static void score_narrow(const ScoreArgs& a, hipStream_t s) {
     const int G = tok_narrow_lanes(a.r.V);
     const int64_t rb = 256 / G;
-    const dim3 grid(tok_blocks((a.r.rows + rb - 1) / rb, 256)), blk(256);
-    if (G == 8) hipLaunchKernelGGL((tok_score_narrow_kernel<T, 8>), grid, blk, 0, s, a);
-    else if (G == 16) hipLaunchKernelGGL((tok_score_narrow_kernel<T, 16>), grid, blk, 0, s, a);
-    else if (G == 32) hipLaunchKernelGGL((tok_score_narrow_kernel<T, 32>), grid, blk, 0, s, a);
-    else hipLaunchKernelGGL((tok_score_narrow_kernel<T, 64>), grid, blk, 0, s, a);
+    const int64_t units = (a.r.rows + rb - 1) / rb;
+    const int nt = 256;
+    if (G == 8) tok_launch(tok_score_narrow_kernel<T, 8>, units, nt, 0, s, a);
+    else if (G == 16) tok_launch(tok_score_narrow_kernel<T, 16>, units, nt, 0, s, a);
+    else if (G == 32) tok_launch(tok_score_narrow_kernel<T, 32>, units, nt, 0, s, a);
+    else tok_launch(tok_score_narrow_kernel<T, 64>, units, nt, 0, s, a);
 }
 
 template <typename T> static void score_grad_narrow(const ScoreGradArgs& a, hipStream_t s) {
     const int G = tok_narrow_lanes(a.r.V);
     const int64_t rb = 256 / G;
-    const dim3 grid(tok_blocks((a.r.rows + rb - 1) / rb, 256)), blk(256);
-    if (G == 8) hipLaunchKernelGGL((tok_score_grad_narrow_kernel<T, 8>), grid, blk, 0, s, a);
-    else if (G == 16) hipLaunchKernelGGL((tok_score_grad_narrow_kernel<T, 16>), grid, blk, 0, s, a);
-    else if (G == 32) hipLaunchKernelGGL((tok_score_grad_narrow_kernel<T, 32>), grid, blk, 0, s, a);
-    else hipLaunchKernelGGL((tok_score_grad_narrow_kernel<T, 64>), grid, blk, 0, s, a);
+    const int64_t units = (a.r.rows + rb - 1) / rb;
+    const int nt = 256;
+    if (G == 8) tok_launch(tok_score_grad_narrow_kernel<T, 8>, units, nt, 0, s, a);
+    else if (G == 16) tok_launch(tok_score_grad_narrow_kernel<T, 16>, units, nt, 0, s, a);
+    else if (G == 32) tok_launch(tok_score_grad_narrow_kernel<T, 32>, units, nt, 0, s, a);
+    else tok_launch(tok_score_grad_narrow_kernel<T, 64>, units, nt, 0, s, a);
 }
 
 // dtype: 0 fp32, 1 bf16, 2 fp16.  y = 0: no targets (lp is not written).  ws: rows * segments * (16 + 8 k) bytes, 16-aligned.
@@ -663,8 +657,7 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
         if (dtype == 0) score_narrow<float>(a, s);
         else if (dtype == 1) score_narrow<bf16_t>(a, s);
         else score_narrow<f16_t>(a, s);
-        SERANN_CHECK(hipGetLastError());
-        return;
+            return;
     }
     const TokPlan p = score_plan(V, dtype, rows);
     a.nseg = p.nseg;
@@ -677,10 +670,8 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
     if (dtype == 0) score_wide<float>(a, p, s);
     else if (dtype == 1) score_wide<bf16_t>(a, p, s);
     else score_wide<f16_t>(a, p, s);
-    SERANN_CHECK(hipGetLastError());
     if (p.nseg > 1) {
-        hipLaunchKernelGGL(tok_score_join_kernel, dim3(tok_blocks(rows, 256)), dim3(256), (size_t)p.nseg * k * 8, s, a, dtype);
-        SERANN_CHECK(hipGetLastError());
+        tok_launch(tok_score_join_kernel, rows, 256, (size_t)p.nseg * k * 8, s, a, dtype);
     }
 }
 
@@ -700,7 +691,7 @@ void launch_tok_score_grad(uint64_t x, int dtype, int64_t rows, int64_t n1, int6
     a.gent = as_ptr<const float>(gent);
     a.ent = as_ptr<const float>(ent);
     a.stat = as_ptr<const float2>(stat);
-    a.dx = as_ptr<void>(dx);
+    a.dx = (int64_t)dx;
     const hipStream_t s = as_stream(stream);
     if (V <= TOK_NARROW_V) {
         if (dtype == 0) score_grad_narrow<float>(a, s);
@@ -709,10 +700,10 @@ void launch_tok_score_grad(uint64_t x, int dtype, int64_t rows, int64_t n1, int6
     } else {
         const int64_t nvec = V / (16 / tok_esize(dtype));
         a.chunks = (int)((nvec + 1023) / 1024);
-        const dim3 grid(tok_blocks(rows * a.chunks, 256)), blk(256);
-        if (dtype == 0) hipLaunchKernelGGL((tok_score_grad_kernel<float>), grid, blk, 0, s, a);
-        else if (dtype == 1) hipLaunchKernelGGL((tok_score_grad_kernel<bf16_t>), grid, blk, 0, s, a);
-        else hipLaunchKernelGGL((tok_score_grad_kernel<f16_t>), grid, blk, 0, s, a);
+        const int64_t units = rows * a.chunks;
+        const int nt = 256;
+        if (dtype == 0) tok_launch(tok_score_grad_kernel<float>, units, nt, 0, s, a);
+        else if (dtype == 1) tok_launch(tok_score_grad_kernel<bf16_t>, units, nt, 0, s, a);
+        else tok_launch(tok_score_grad_kernel<f16_t>, units, nt, 0, s, a);
     }
-    SERANN_CHECK(hipGetLastError());
 }
