@@ -191,7 +191,7 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
                       uint64_t ids, uint64_t top, uint64_t stat, uint64_t ws, uint64_t stream);
 void launch_tok_score_grad(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s0, int64_t s1, int64_t V,
                            double temperature, uint64_t y, int y64, int64_t t0, int64_t t1, int64_t ignore, uint64_t glp,
-                           uint64_t gent, uint64_t ent, uint64_t stat, uint64_t dx, uint64_t stream);
+                           uint64_t gent, uint64_t stat, uint64_t dx, uint64_t stream);
 int64_t tok_distill_segments(int64_t V, int dtype, int64_t rows, int grad);
 void launch_tok_distill(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s0, int64_t s1, int64_t V, double temperature,
                         uint64_t ids, int id64, uint64_t t, uint64_t w, int K, int bucket, uint64_t loss, uint64_t dx,

@@ -25,7 +25,7 @@ struct ScoreArgs {
     float *lp, *ent;
     int64_t* ids;
     float* top;
-    float2* stat;                // for the backward pass: (m, log2 sum), 0: not wanted
+    float* stat;                 // for the backward pass: (m, log2 sum, entropy) a row, 0: not wanted
     float4* part;                // nseg > 1: (m, n, S, W) and the sorted keys of each segment
     uint64_t* keys;
 };
@@ -44,7 +44,9 @@ __device__ __forceinline__ float score_finish(const ScoreArgs& a, int64_t row, f
         const float H = none ? 0.f : lnS - 0.6931471805599453f * (W / (n + S));
         a.ent[row] = H;
         if (a.stat) {
-            a.stat[row] = none ? make_float2(0.f, INFINITY) : make_float2(m, lnS * 1.4426950408889634f);
+            a.stat[row * 3] = none ? 0.f : m;
+            a.stat[row * 3 + 1] = none ? INFINITY : lnS * 1.4426950408889634f;
+            a.stat[row * 3 + 2] = H;
         }
     }
     return none ? 0.f : lnS;
@@ -53,7 +55,6 @@ __device__ __forceinline__ void score_skip(const ScoreArgs& a, int64_t row, int 
     if (lane == 0) {
         if (a.lp) a.lp[row] = 0.f;
         a.ent[row] = 0.f;
-        if (a.stat) a.stat[row] = make_float2(0.f, INFINITY);
     }
     for (int j = lane; j < a.k; j += lanes) {
         a.ids[row * a.k + j] = -1;
@@ -491,8 +492,7 @@ struct ScoreGradArgs {
     TokRows r;
     int64_t y, t0, t1, ignore;
     int y64, chunks;
-    const float *glp, *gent, *ent;   // glp / gent: 0 = no such gradient
-    const float2* stat;
+    const float *glp, *gent, *stat;  // glp / gent: 0 = no such gradient
     int64_t dx;                      // [rows][V]
 };
 // dx = ( gl [v = target] - q (gl + gh (ln q + H)) ) / T,  log2 q = fma(x - m, c, -l2S)
@@ -500,17 +500,17 @@ struct ScoreCoef {
     float m, l2S, a, b, gl;          // -q (a + b log2 q) + [target] gl
 };
 __device__ __forceinline__ ScoreCoef score_coef(const ScoreGradArgs& a, int64_t row, bool valid_t) {
-    const float2 st = a.stat[row];
+    const float* st = a.stat + row * 3;
     float gl = a.glp ? a.glp[row] : 0.f;
     const float gh = a.gent ? a.gent[row] : 0.f;
     if (!valid_t && a.glp) gl = NAN;                         // a target outside the vocabulary: loud
     ScoreCoef k;
-    k.m = st.x;
-    k.l2S = st.y;
+    k.m = st[0];
+    k.l2S = st[1];
     k.gl = gl * a.r.inv_t;
-    k.a = (gl + gh * a.ent[row]) * a.r.inv_t;
+    k.a = (gl + gh * st[2]) * a.r.inv_t;
     k.b = gh * 0.6931471805599453f * a.r.inv_t;
-    if (st.y == INFINITY) k.a = k.b = k.gl = 0.f;            // an empty row has no gradient
+    if (k.l2S == INFINITY) k.a = k.b = k.gl = 0.f;            // an empty row has no gradient
     return k;
 }
 __device__ __forceinline__ float score_dx(const ScoreCoef& k, float c, float x) {
@@ -650,7 +650,7 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
     a.ent = as_ptr<float>(ent);
     a.ids = as_ptr<int64_t>(ids);
     a.top = as_ptr<float>(top);
-    a.stat = as_ptr<float2>(stat);
+    a.stat = as_ptr<float>(stat);
     a.nseg = 1;
     const hipStream_t s = as_stream(stream);
     if (V <= TOK_NARROW_V) {
@@ -677,7 +677,7 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
 
 void launch_tok_score_grad(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s0, int64_t s1, int64_t V,
                            double temperature, uint64_t y, int y64, int64_t t0, int64_t t1, int64_t ignore, uint64_t glp,
-                           uint64_t gent, uint64_t ent, uint64_t stat, uint64_t dx, uint64_t stream) {
+                           uint64_t gent, uint64_t stat, uint64_t dx, uint64_t stream) {
     if (rows <= 0) return;
     if (dtype < 0 || dtype > 2) throw std::runtime_error("token operators: unknown logits type");
     ScoreGradArgs a{};
@@ -689,8 +689,7 @@ void launch_tok_score_grad(uint64_t x, int dtype, int64_t rows, int64_t n1, int6
     a.ignore = ignore;
     a.glp = as_ptr<const float>(y ? glp : 0);
     a.gent = as_ptr<const float>(gent);
-    a.ent = as_ptr<const float>(ent);
-    a.stat = as_ptr<const float2>(stat);
+    a.stat = as_ptr<const float>(stat);
     a.dx = (int64_t)dx;
     const hipStream_t s = as_stream(stream);
     if (V <= TOK_NARROW_V) {

@@ -148,63 +148,98 @@ def _distill_segments(V, code, rows, grad):
     return H.lib().tok_distill_segments(V, code, rows, grad)
 
 
+# the current stream of a device as the launchers take it; torch.cuda.current_stream() builds a Stream object first (2 of the
+# 16 us that a small call took)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _on_device(f):
+    """f(logits, ...) with the logits' device as the current one; entering a device context costs more than to ask."""
+    @functools.wraps(f)
+    def run(logits, *args):
+        if torch.cuda.current_device() == logits.device.index:
+            return f(logits, *args)
+        with torch.cuda.device(logits.device):
+            return f(logits, *args)
+    return run
+
+
+def _once(backward):
+    """``once_differentiable`` whose wrapping is paid for only under create_graph (5 us a call otherwise)."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
+
+
 # ------------------------------------------------------------------------------------------------
 # log-probabilities
 # ------------------------------------------------------------------------------------------------
+@_on_device
 def _score_hip(logits, targets, temperature, top_k, ignore_index, want_stat):
+    """(logprob, entropy, top ids, top log-probabilities, what the backward pass needs)."""
     x, rows, n1, s0, s1 = _rows(logits)
-    lead, dev, V, code = logits.shape[:-1], logits.device, logits.shape[-1], _DTYPES[logits.dtype]
-    lp = ids = top = stat = ws = None
-    y, t0, t1 = None, 0, 0
+    shape, V, code = logits.shape, logits.shape[-1], _DTYPES[logits.dtype]
+    lead = shape[:-1]
+    lp = ids = top = saved = ws = None
+    y, y64, t0, t1, yp, lpp = None, False, 0, 0, 0, 0
     if targets is not None:
         y, t0, t1 = _same_rows(targets, n1, rows)
-        lp = torch.empty(lead, dtype=torch.float32, device=dev)
-    ent = torch.empty(lead, dtype=torch.float32, device=dev)
+        y64 = y.dtype == torch.int64
+        lp = x.new_empty(lead, dtype=torch.float32)
+        yp, lpp = y.data_ptr(), lp.data_ptr()
+    ent = x.new_empty(lead, dtype=torch.float32)
+    idp = topp = stp = wsp = 0
     if top_k:
-        ids = torch.empty(lead + (top_k,), dtype=torch.int64, device=dev)
-        top = torch.empty(lead + (top_k,), dtype=torch.float32, device=dev)
+        ids = x.new_empty(lead + (top_k,), dtype=torch.int64)
+        top = x.new_empty(lead + (top_k,), dtype=torch.float32)
+        idp, topp = ids.data_ptr(), top.data_ptr()
+    layout = (code, rows, n1, s0, s1, V, temperature, yp, y64, t0, t1, ignore_index)
     if want_stat:
-        stat = torch.empty((rows, 2), dtype=torch.float32, device=dev)
+        stat = x.new_empty((rows, 3), dtype=torch.float32)
+        stp = stat.data_ptr()
+        saved = (x, y, stat, layout)
     nseg = _score_segments(V, code, rows)
     if nseg > 1:
-        ws = torch.empty(rows * nseg * (2 + top_k), dtype=torch.int64, device=dev)
-    H.lib().tok_score(x.data_ptr(), code, rows, n1, s0, s1, V, temperature, H.ptr(y), y is not None and y.dtype == torch.int64,
-                      t0, t1, ignore_index, top_k, H.ptr(lp), ent.data_ptr(), H.ptr(ids), H.ptr(top), H.ptr(stat), H.ptr(ws),
-                      torch.cuda.current_stream(dev).cuda_stream)
-    return lp, ent, ids, top, stat
+        ws = x.new_empty(rows * nseg * (2 + top_k), dtype=torch.int64)
+        wsp = ws.data_ptr()
+    H.lib().tok_score(x.data_ptr(), *layout, top_k, lpp, ent.data_ptr(), idp, topp, stp, wsp,
+                      _raw_stream(logits.device.index))
+    return lp, ent, ids, top, saved
+
+
+@_on_device
+def _score_grad_hip(x, layout, stat, glp, gent, shape):
+    dx = x.new_empty(shape)
+    H.lib().tok_score_grad(x.data_ptr(), *layout, H.ptr(glp), H.ptr(gent), stat.data_ptr(), dx.data_ptr(),
+                           _raw_stream(x.device.index))
+    return dx
+
+
+def _f32(g):
+    return g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) else g.float().contiguous()
 
 
 class _Score(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, targets, temperature, top_k, ignore_index):
-        with torch.cuda.device(logits.device):
-            lp, ent, ids, top, stat = _score_hip(logits, targets, temperature, top_k, ignore_index, True)
-        ctx.save_for_backward(logits, targets, ent, stat)
-        ctx.args = (temperature, ignore_index)
+    def forward(ctx, logits, targets, temperature, top_k, ignore_index, extra):
+        lp, ent, ids, top, (x, y, stat, ctx.layout) = _score_hip(logits, targets, temperature, top_k, ignore_index, True)
+        ctx.save_for_backward(x, y, stat)
+        ctx.shape = logits.shape
         ctx.set_materialize_grads(False)
-        if top_k:
-            ctx.mark_non_differentiable(ids, top)
-        return lp, ent, ids, top
+        extra += (ids, top)                     # no gradients: kept out of the graph
+        return ent if lp is None else (ent, lp)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, glp, gent, _ids, _top):
-        logits, targets, ent, stat = ctx.saved_tensors
+    @_once
+    def backward(ctx, gent, glp=None):
         if glp is None and gent is None:
-            return None, None, None, None, None
-        temperature, ignore_index = ctx.args
-        dev, V = logits.device, logits.shape[-1]
-        with torch.cuda.device(dev):
-            x, rows, n1, s0, s1 = _rows(logits)
-            y, t0, t1 = _same_rows(targets, n1, rows) if targets is not None else (None, 0, 0)
-            glp = glp.float().contiguous() if glp is not None else None
-            gent = gent.float().contiguous() if gent is not None else None
-            dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-            H.lib().tok_score_grad(x.data_ptr(), _DTYPES[logits.dtype], rows, n1, s0, s1, V, temperature, H.ptr(y),
-                                   y is not None and y.dtype == torch.int64, t0, t1, ignore_index, H.ptr(glp), H.ptr(gent),
-                                   ent.data_ptr(), stat.data_ptr(), dx.data_ptr(),
-                                   torch.cuda.current_stream(dev).cuda_stream)
-        return dx, None, None, None, None
+            return None, None, None, None, None, None
+        x, _, stat = ctx.saved_tensors
+        return _score_grad_hip(x, ctx.layout, stat, _f32(glp), _f32(gent), ctx.shape), None, None, None, None, None
 
 
 def _log_softmax(logits, temperature):
@@ -260,57 +295,62 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     if not logits.is_cuda:
         return _score_torch(logits, targets, temperature, top_k, ignore_index)
     if torch.is_grad_enabled() and logits.requires_grad:
-        return TokenLogprobs(*_Score.apply(logits, targets, temperature, top_k, ignore_index))
-    if torch.cuda.current_device() == logits.device.index:
-        return TokenLogprobs(*_score_hip(logits, targets, temperature, top_k, ignore_index, False)[:4])
-    with torch.cuda.device(logits.device):
-        return TokenLogprobs(*_score_hip(logits, targets, temperature, top_k, ignore_index, False)[:4])
+        extra = []
+        out = _Score.apply(logits, targets, temperature, top_k, ignore_index, extra)
+        return TokenLogprobs(None, out, *extra) if targets is None else TokenLogprobs(out[1], out[0], *extra)
+    return TokenLogprobs(*_score_hip(logits, targets, temperature, top_k, ignore_index, False)[:4])
 
 
 # ------------------------------------------------------------------------------------------------
 # distillation
 # ------------------------------------------------------------------------------------------------
+@_on_device
 def _distill_hip(logits, ids, logprobs, temperature, bucket, weight, dx, save):
-    """(loss, stat, pk); the gradient goes to ``dx`` when given (for a loss gradient of 1 a row)."""
+    """(loss, what the backward pass needs).  dx: None, or where the gradient for a loss gradient of 1 a row goes (True: into
+    a new tensor); returned in the second place then."""
     x, rows, n1, s0, s1 = _rows(logits)
-    dev, V, K, code = logits.device, logits.shape[-1], ids.shape[-1], _DTYPES[logits.dtype]
-    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-    stat = pk = ws = None
+    V, K, code = logits.shape[-1], ids.shape[-1], _DTYPES[logits.dtype]
+    loss = x.new_empty(logits.shape[:-1], dtype=torch.float32)
+    if dx is True:
+        dx = x.new_empty(logits.shape)
+    stp = pkp = wsp = 0
     nseg = _distill_segments(V, code, rows, dx is not None)
+    stat = pk = None
     if save or dx is not None and nseg > 0:
-        stat = torch.empty((rows, 4), dtype=torch.float32, device=dev)
-        pk = torch.empty((rows, K), dtype=torch.float32, device=dev)
+        stat = x.new_empty((rows, 4), dtype=torch.float32)
+        pk = x.new_empty((rows, K), dtype=torch.float32)
+        stp, pkp = stat.data_ptr(), pk.data_ptr()
     if nseg > 1:
-        ws = torch.empty((rows * nseg, 4), dtype=torch.float32, device=dev)
-    H.lib().tok_distill(x.data_ptr(), code, rows, n1, s0, s1, V, temperature, ids.data_ptr(), ids.dtype == torch.int64,
-                        logprobs.data_ptr(), H.ptr(weight), K, bucket, loss.data_ptr(), H.ptr(dx), H.ptr(stat), H.ptr(pk),
-                        H.ptr(ws), torch.cuda.current_stream(dev).cuda_stream)
-    return loss, stat, pk
+        ws = x.new_empty((rows * nseg, 4), dtype=torch.float32)
+        wsp = ws.data_ptr()
+    layout = (code, rows, n1, s0, s1, V, temperature, ids.data_ptr(), ids.dtype == torch.int64)
+    wp = 0 if weight is None else weight.data_ptr()
+    H.lib().tok_distill(x.data_ptr(), *layout, logprobs.data_ptr(), wp, K, bucket, loss.data_ptr(),
+                        0 if dx is None else dx.data_ptr(), stp, pkp, wsp, _raw_stream(logits.device.index))
+    return loss, (x, stat, pk, layout) if dx is None else dx
+
+
+@_on_device
+def _distill_grad_hip(x, layout, ids, weight, g, stat, pk, shape):
+    dx = x.new_empty(shape)
+    H.lib().tok_distill_grad(x.data_ptr(), *layout, H.ptr(weight), ids.shape[-1], g.data_ptr(), stat.data_ptr(),
+                             pk.data_ptr(), dx.data_ptr(), _raw_stream(x.device.index))
+    return dx
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, logprobs, temperature, bucket, weight):
-        with torch.cuda.device(logits.device):
-            loss, stat, pk = _distill_hip(logits, ids, logprobs, temperature, bucket, weight, None, True)
-        ctx.save_for_backward(logits, ids, weight, stat, pk)
-        ctx.temperature = temperature
+        loss, (x, stat, pk, ctx.layout) = _distill_hip(logits, ids, logprobs, temperature, bucket, weight, None, True)
+        ctx.save_for_backward(x, ids, weight, stat, pk)
+        ctx.shape = logits.shape
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
-        logits, ids, weight, stat, pk = ctx.saved_tensors
-        dev, V = logits.device, logits.shape[-1]
-        with torch.cuda.device(dev):
-            x, rows, n1, s0, s1 = _rows(logits)
-            g = g.float().contiguous()
-            dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-            H.lib().tok_distill_grad(x.data_ptr(), _DTYPES[logits.dtype], rows, n1, s0, s1, V, ctx.temperature,
-                                     ids.data_ptr(), ids.dtype == torch.int64, H.ptr(weight), ids.shape[-1], g.data_ptr(),
-                                     stat.data_ptr(), pk.data_ptr(), dx.data_ptr(),
-                                     torch.cuda.current_stream(dev).cuda_stream)
-        return dx, None, None, None, None, None
+        x, ids, weight, stat, pk = ctx.saved_tensors
+        return _distill_grad_hip(x, ctx.layout, ids, weight, _f32(g), stat, pk, ctx.shape), None, None, None, None, None
 
 
 def _distill_torch(logits, ids, logprobs, temperature, tail, weight):
@@ -360,12 +400,10 @@ def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     _check_teacher(logits, teacher_ids, teacher_logprobs, tail, weight)
     if not logits.is_cuda:
         return _distill_torch(logits, teacher_ids, teacher_logprobs, temperature, tail, weight)
-    ids, lp = teacher_ids.contiguous(), teacher_logprobs.float().contiguous()
-    weight = None if weight is None else weight.float().contiguous()
+    ids, lp, weight = teacher_ids.contiguous(), _f32(teacher_logprobs), _f32(weight)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _Distill.apply(logits, ids, lp, temperature, _TAILS[tail], weight)
-    with torch.cuda.device(logits.device):
-        return _distill_hip(logits, ids, lp, temperature, _TAILS[tail], weight, None, False)[0]
+    return _distill_hip(logits, ids, lp, temperature, _TAILS[tail], weight, None, False)[0]
 
 
 def topk_distill_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, *,
@@ -388,9 +426,5 @@ def topk_distill_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
             loss = _distill_torch(x, teacher_ids, teacher_logprobs, temperature, tail, weight)
             dx, = torch.autograd.grad(loss.sum(), x)
         return loss.detach(), dx.contiguous() if out is None else out.copy_(dx)
-    ids, lp = teacher_ids.contiguous(), teacher_logprobs.float().contiguous()
-    weight = None if weight is None else weight.float().contiguous()
-    with torch.cuda.device(logits.device):
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
-        loss = _distill_hip(logits, ids, lp, temperature, _TAILS[tail], weight, dx, False)[0]
-    return loss, dx
+    ids, lp, weight = teacher_ids.contiguous(), _f32(teacher_logprobs), _f32(weight)
+    return _distill_hip(logits, ids, lp, temperature, _TAILS[tail], weight, True if out is None else out, False)
