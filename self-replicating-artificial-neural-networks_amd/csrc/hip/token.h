@@ -20,8 +20,8 @@ typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16_t;
 
 constexpr int TOK_MAX_K = 128;        // top alternatives / teacher entries a row
-constexpr int TOK_MAX_SEG = 64;       // segments a row is split into at most
-constexpr int64_t TOK_MAX_V = 1 << 20;
+constexpr int64_t TOK_MAX_V = 1000000;
+constexpr int TOK_MAX_SEG = 62;       // segments a row is cut into at most: 10^6 fp32 logits in 64 KB pieces; a lane each to join
 constexpr int TOK_NARROW_V = 512;     // rows of up to 64 x 8 elements: a group of 8-64 lanes a row, no LDS reduction
 
 // Rows of a [n0][n1][V] tensor with strides s0, s1 (elements) and unit stride inside a row; row r = (r / n1, r % n1)
@@ -113,25 +113,55 @@ template <int CTRL> __device__ __forceinline__ double tok_dpp(double v) {
     return __builtin_bit_cast(double, tok_dpp<CTRL>(__builtin_bit_cast(uint64_t, v)));
 }
 struct TokMax { static __device__ __forceinline__ float f(float a, float b) { return tok_max(a, b); } };
-struct TokMin { static __device__ __forceinline__ float f(float a, float b) { return fminf(a, b); } };
+struct TokMin {
+    static __device__ __forceinline__ float f(float a, float b) { return fminf(a, b); }
+    static __device__ __forceinline__ uint64_t f(uint64_t a, uint64_t b) { return a < b ? a : b; }
+};
 struct TokSum {
     static __device__ __forceinline__ float f(float a, float b) { return a + b; }
     static __device__ __forceinline__ double f(double a, double b) { return a + b; }
+    static __device__ __forceinline__ uint32_t f(uint32_t a, uint32_t b) { return a + b; }
 };
 struct TokTop {
     static __device__ __forceinline__ uint32_t f(uint32_t a, uint32_t b) { return a > b ? a : b; }
     static __device__ __forceinline__ uint64_t f(uint64_t a, uint64_t b) { return a > b ? a : b; }
     static __device__ __forceinline__ double f(double a, double b) { return a > b ? a : b; }
 };
+// (a, b) of lanes 16 (32) apart: the even row of 16 lanes (the lower half) of v in every lane, and the odd row (upper half)
+template <int D> __device__ __forceinline__ void tok_halves(uint32_t v, uint32_t& a, uint32_t& b) {
+    static_assert(D == 16 || D == 32, "rows or halves");
+    if constexpr (D == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        a = r[0];
+        b = r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        a = r[0];
+        b = r[1];
+    }
+}
+template <int D, typename OP, typename V> __device__ __forceinline__ V tok_across(V v) {
+    if constexpr (sizeof(V) == 4) {
+        uint32_t a, b;
+        tok_halves<D>(__builtin_bit_cast(uint32_t, v), a, b);
+        return OP::f(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b));
+    } else {
+        const uint64_t w = __builtin_bit_cast(uint64_t, v);
+        uint32_t al, bl, ah, bh;
+        tok_halves<D>((uint32_t)w, al, bl);
+        tok_halves<D>((uint32_t)(w >> 32), ah, bh);
+        return OP::f(__builtin_bit_cast(V, (uint64_t)ah << 32 | al), __builtin_bit_cast(V, (uint64_t)bh << 32 | bl));
+    }
+}
 // Reduction over aligned groups of G lanes, every lane gets the result: lanes 1 and 2 apart (quad_perm), then the mirrored
-// half row and row (their quads / halves are uniform by then), then across rows of 16
+// half row and row (their quads / halves are uniform by then), then across rows of 16: all on the vector ALU, no LDS trip
 template <int G, typename OP, typename V> __device__ __forceinline__ V tok_group(V v) {
     if constexpr (G > 1) v = OP::f(v, tok_dpp<0xB1>(v));
     if constexpr (G > 2) v = OP::f(v, tok_dpp<0x4E>(v));
     if constexpr (G > 4) v = OP::f(v, tok_dpp<0x141>(v));
     if constexpr (G > 8) v = OP::f(v, tok_dpp<0x140>(v));
-    if constexpr (G > 16) v = OP::f(v, (V)__shfl_xor(v, 16, 64));
-    if constexpr (G > 32) v = OP::f(v, (V)__shfl_xor(v, 32, 64));
+    if constexpr (G > 16) v = tok_across<16, OP>(v);
+    if constexpr (G > 32) v = tok_across<32, OP>(v);
     return v;
 }
 
@@ -149,6 +179,25 @@ __device__ __forceinline__ uint64_t tok_key(float x, int i) {
 }
 __device__ __forceinline__ int tok_key_index(uint64_t k) { return (int)~(uint32_t)k; }
 __device__ __forceinline__ float tok_key_value(uint64_t k) { return tok_unorder((uint32_t)(k >> 32)); }
+
+// Ranks the n distinct keys of an LDS list by counting the larger ones, 8 lanes a key: f(rank, key) for ranks below k, from one
+// lane.  n is the same in every thread; NT threads call.
+template <int NT, typename F> __device__ __forceinline__ void tok_rank(uint64_t* keys, int n, int k, const F& f) {
+    const int tid = threadIdx.x, l = tid & 7;
+    for (int i0 = 0; i0 < n; i0 += NT / 8) {
+        const int i = i0 + (tid >> 3);
+        const uint64_t key = i < n ? keys[i] : 0;
+        uint32_t c = 0;
+        int j = l;
+        for (; j + 24 < n; j += 32) {
+            const uint64_t a = keys[j], b = keys[j + 8], d = keys[j + 16], e = keys[j + 24];
+            c += (a > key) + (b > key) + (d > key) + (e > key);
+        }
+        for (; j < n; j += 8) c += keys[j] > key;
+        c = tok_group<8, TokSum>(c);
+        if (l == 0 && i < n && (int)c < k) f((int)c, key);
+    }
+}
 
 template <typename T> __device__ __forceinline__ tok_in<T> tok_row(const TokRows& r, int64_t row) {
     const int64_t i0 = r.n1 == r.rows ? 0 : (int64_t)((uint32_t)row / (uint32_t)r.n1);      // fewer than 2^31 rows
@@ -319,7 +368,7 @@ inline void tok_launch(void (*kernel)(A, X...), int64_t units, int nt, size_t ld
     }
 }
 inline TokRows tok_rows_of(uint64_t x, int64_t rows, int64_t n1, int64_t s0, int64_t s1, int64_t V, double temperature) {
-    if (rows < 0 || V < 1 || V > TOK_MAX_V) throw std::runtime_error("token operators: vocabulary must be in [1, 2^20]");
+    if (rows < 0 || V < 1 || V > TOK_MAX_V) throw std::runtime_error("token operators: vocabulary must be in [1, 10^6]");
     if (n1 < 1 || (rows && rows % n1)) throw std::runtime_error("token operators: rows must be a multiple of n1");
     if (!(temperature > 0)) throw std::runtime_error("token operators: temperature must be positive");
     TokRows r;

@@ -235,19 +235,14 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
         const int nc = S == S ? (slow ? CAND + 1 : ncand) : 0;
         int done = nc < a.k ? nc : a.k;
         if (nc <= CAND) {
-            for (int i = tid; i < nc; i += NT) {
-                const uint64_t key = cand[i];
-                int rank = 0;
-                for (int j = 0; j < nc; ++j) rank += cand[j] > key;
-                if (rank < a.k) {
-                    if (a.nseg == 1) {
-                        a.ids[row * a.k + rank] = tok_key_index(key);
-                        a.top[row * a.k + rank] = score_toplp(a, tok_key_value(key), m, lnS);
-                    } else {
-                        a.keys[u * a.k + rank] = key;
-                    }
+            tok_rank<NT>(cand, nc, a.k, [&](int rank, uint64_t key) {
+                if (a.nseg == 1) {
+                    a.ids[row * a.k + rank] = tok_key_index(key);
+                    a.top[row * a.k + rank] = score_toplp(a, tok_key_value(key), m, lnS);
+                } else {
+                    a.keys[u * a.k + rank] = key;
                 }
-            }
+            });
         } else {
             // k rounds of the largest key below the last one, read again (L2); an exhausted segment yields key 0
             uint64_t last = ~0ull;
@@ -295,93 +290,84 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
     }
 }
 
-// Joins the segments of a row: one wave a row.  The sums are rescaled to the row's maximum in segment order; a key's rank is
-// its place in its own sorted list plus, by binary search, the number of larger keys in every other list.
-__global__ __launch_bounds__(256) void tok_score_join_kernel(ScoreArgs a, int esize_code) {
+// Joins the segments of a row.  The sums are rescaled to the row's maximum, a segment a lane, and added by a fixed tree.  Of
+// the sorted lists of keys: with j = ceil(k / lists), the smallest of the j-th keys has at least k keys at or above it, and so
+// has the largest of the k-th keys; what lies below both is dropped, the rest (about 1.5 k) ranked by counting.
+// NT = 64 without alternatives: one wave a row.
+template <int NT> __global__ __launch_bounds__(NT) void tok_score_join_kernel(ScoreArgs a, int dtype) {
     extern __shared__ uint64_t lists[];
-    const int tid = threadIdx.x;
+    __shared__ int ncand;
+    const int tid = threadIdx.x, lane = tid & 63;
     const int64_t row = a.r.u0 + blockIdx.x;
+    // every load that the row needs is under way before the first is waited for
+    float4 p = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    if (lane < a.nseg) p = a.part[row * a.nseg + lane];
     int64_t tgt = 0;
-    if (a.y) {
-        tgt = score_target(a, row);
-        if (tgt == a.ignore) {
-            score_skip(a, row, tid, 256);
-            return;
-        }
+    if (a.y) tgt = score_target(a, row);
+    const int nk = a.nseg * a.k;
+    const uint64_t* keys = a.keys + row * nk;
+    if (a.k) {
+        if (tid == 0) ncand = 0;
+        for (int i = tid; i < nk; i += NT) lists[i] = keys[i];
+    }
+    if (a.y && tgt == a.ignore) {
+        score_skip(a, row, tid, NT);
+        return;
     }
     const bool valid_t = !a.y || (uint64_t)tgt < (uint64_t)a.r.V;
     float xt = 0.f;
-    if (a.y && valid_t) {
-        xt = esize_code == 0 ? tok_row<float>(a.r, row)[tgt]
-                             : esize_code == 1 ? bf2f(tok_row<bf16_t>(a.r, row)[tgt]) : (float)tok_row<f16_t>(a.r, row)[tgt];
+    if (a.y && valid_t)
+        xt = dtype == 0 ? tok_row<float>(a.r, row)[tgt]
+             : dtype == 1 ? bf2f(tok_row<bf16_t>(a.r, row)[tgt]) : (float)tok_row<f16_t>(a.r, row)[tgt];
+    const float m = tok_group<64, TokMax>(p.x);
+    float n = 0.f, S = p.z, W = 0.f;                         // a segment of nothing but -inf: 0, or NaN
+    if (p.x == m) {
+        n = p.y;
+        W = p.w;
+    } else if (p.x > -INFINITY) {
+        const float d = (p.x - m) * a.r.c, f = tok_exp2(d);
+        S = (p.y + p.z) * f;
+        W = f > 0.f ? f * (p.w + tok_max(d, -200.f) * (p.y + p.z)) : 0.f;
     }
-    const float4* part = a.part + row * a.nseg;
-    float m = -INFINITY;
-    for (int s = 0; s < a.nseg; ++s) m = tok_max(m, part[s].x);
-    float S = 0.f, W = 0.f, n = 0.f;
-    for (int s = 0; s < a.nseg; ++s) {
-        const float4 p = part[s];
-        if (p.x == m) {
-            n += p.y;
-            S += p.z;
-            W += p.w;
-        } else if (p.x > -INFINITY) {
-            const float d = (p.x - m) * a.r.c, f = tok_exp2(d);
-            S += (p.y + p.z) * f;
-            W += f > 0.f ? f * (p.w + tok_max(d, -200.f) * (p.y + p.z)) : 0.f;
-        } else {
-            S += p.z;                                   // 0, or NaN
-        }
-    }
+    n = tok_group<64, TokSum>(n);
+    S = tok_group<64, TokSum>(S);
+    W = tok_group<64, TokSum>(W);
     const float lnS = score_finish(a, row, m, n, S, W, xt, valid_t, tid == 0);
-    if (a.k) {
-        const int nk = a.nseg * a.k;
-        const uint64_t* keys = a.keys + row * nk;
-        for (int i = tid; i < nk; i += 256) lists[i] = keys[i];
+    if constexpr (NT > 64) {
         __syncthreads();
-        for (int i = tid; i < nk; i += 256) {
-            const uint64_t key = lists[i];
-            const int own = i / a.k;
-            if (key == 0 || S != S) continue;
-            int rank = i - own * a.k;
-            for (int s = 0; s < a.nseg && rank < a.k; ++s) {
-                if (s == own) continue;
-                const uint64_t* l = lists + s * a.k;
-                int lo = 0, hi = a.k;                    // keys larger than `key`: a prefix of the sorted list
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1;
-                    if (l[mid] > key) lo = mid + 1;
-                    else hi = mid;
-                }
-                rank += lo;
-            }
-            if (rank < a.k) {
-                a.ids[row * a.k + rank] = tok_key_index(key);
-                a.top[row * a.k + rank] = score_toplp(a, tok_key_value(key), m, lnS);
-            }
-        }
-        // fewer than k elements that are not NaN: every key that there is has been placed, the rest is filled
-        int have = 0;
-        for (int s = 0; s < a.nseg && S == S; ++s) {
-            const uint64_t* l = lists + s * a.k;
-            int lo = 0, hi = a.k;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (l[mid] != 0) lo = mid + 1;
-                else hi = mid;
-            }
-            have += lo;
-            if (have >= a.k) break;
-        }
-        for (int j = have + tid; j < a.k; j += 256) {
-            a.ids[row * a.k + j] = -1;
-            a.top[row * a.k + j] = NAN;
+        // each wave works the bound out for itself
+        const uint64_t first = lane < a.nseg ? lists[lane * a.k] : 0;
+        const int live = (int)__popcll(__ballot(first != 0));
+        const int j = live ? (a.k + live - 1) / live : 1;
+        const uint64_t jth = first ? lists[lane * a.k + j - 1] : ~0ull, kth = lane < a.nseg ? lists[lane * a.k + a.k - 1] : 0;
+        uint64_t B = tok_group<64, TokMin>(jth);
+        const uint64_t Bk = tok_group<64, TokTop>(kth);
+        if (Bk > B) B = Bk;
+        if (B == 0) B = 1;                                   // key 0: no element
+        // candidates move to the front of the lists' memory: read, then written
+        uint64_t mine[(TOK_MAX_SEG * TOK_MAX_K + NT - 1) / NT];
+#pragma unroll
+        for (int q = 0; q < (TOK_MAX_SEG * TOK_MAX_K + NT - 1) / NT; ++q) {
+            const int i = q * NT + tid;
+            mine[q] = i < nk ? lists[i] : 0;
         }
         __syncthreads();
+#pragma unroll
+        for (int q = 0; q < (TOK_MAX_SEG * TOK_MAX_K + NT - 1) / NT; ++q)
+            if (mine[q] >= B) lists[atomicAdd(&ncand, 1)] = mine[q];
+        __syncthreads();
+        const int nc = S == S ? ncand : 0;                   // a row with a NaN or +inf logit has no ranking
+        tok_rank<NT>(lists, nc, a.k, [&](int rank, uint64_t key) {
+            a.ids[row * a.k + rank] = tok_key_index(key);
+            a.top[row * a.k + rank] = score_toplp(a, tok_key_value(key), m, lnS);
+        });
+        for (int r = nc + tid; r < a.k; r += NT) {           // fewer than k elements
+            a.ids[row * a.k + r] = -1;
+            a.top[row * a.k + r] = NAN;
+        }
     }
 }
 
-// ---- narrow rows -------------------------------------------------------------------------------------------------------
 // Keys of a narrow row (index < 512): 16-bit types fit (order, index) in 32 bits, fp32 takes 64
 template <typename T> struct NarrowKey {
     typedef uint32_t type;
@@ -671,7 +657,8 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
     else if (dtype == 1) score_wide<bf16_t>(a, p, s);
     else score_wide<f16_t>(a, p, s);
     if (p.nseg > 1) {
-        tok_launch(tok_score_join_kernel, rows, 256, (size_t)p.nseg * k * 8, s, a, dtype);
+        if (k) tok_launch(tok_score_join_kernel<256>, rows, 256, (size_t)p.nseg * k * 8, s, a, dtype);
+        else tok_launch(tok_score_join_kernel<64>, rows, 64, 0, s, a, dtype);
     }
 }
 

@@ -10,7 +10,7 @@ tokens come next -- and train a model from another one's answers:
 * :func:`topk_distill_grad`  -- the same loss and its gradient in one pass over the logits, for trainers that run their own
   backward (``riboae.hip_trainer``).
 
-Logits are ``(..., V)``, float32, bfloat16 or float16, 1 <= V <= 2**20.  Leading dimensions may have any strides (a slice
+Logits are ``(..., V)``, float32, bfloat16 or float16, 1 <= V <= 1,000,000.  Leading dimensions may have any strides (a slice
 ``logits[:, :-1]`` is read in place); the last one is copied if it is not contiguous.  Sums are taken in float32 or wider,
 whatever the logits' type; results are float32, gradients have the logits' type.  ``-inf`` logits are tokens ruled out: they
 have probability and gradient 0.  A row of nothing but ``-inf`` has log-probabilities ``-inf``, entropy 0 and no gradient.  A
@@ -31,7 +31,7 @@ from . import hip_ops as H
 
 MAX_TOP_K = 128          # csrc/hip/token.h TOK_MAX_K
 MAX_TEACHER_K = 256      # csrc/hip/token_distill.hip DIST_MAX_K
-MAX_VOCAB = 1 << 20      # csrc/hip/token.h TOK_MAX_V
+MAX_VOCAB = 1_000_000    # csrc/hip/token.h TOK_MAX_V
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TAILS = {"drop": 0, "bucket": 1}
 

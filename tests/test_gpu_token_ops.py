@@ -104,7 +104,7 @@ def test_score_sizes(V, dtype):
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("V,k", [(40, 40), (130, 128), (512, 65), (600, 128), (1500, 64), (4000, 128), (9000, 128), (20000, 33),
-                                 (70001, 128), (100003, 1)])
+                                 (70001, 128), (100003, 1), (1000000, 128), (999999, 20)])
 def test_score_top_k(V, k, dtype):
     x, at, _ = _logits(5, V, dtype, k)
     _check_score(x, at, 2.0, k, grad=False)
