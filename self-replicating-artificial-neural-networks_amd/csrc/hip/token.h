@@ -328,6 +328,109 @@ template <typename T> __device__ __forceinline__ void tok_narrow_store(tok_out<T
     }
 }
 
+// Many short rows (up to 64 elements): a wave takes 64 of them, a row a lane -- no reductions between lanes, no idle lanes.
+// The rows pass through LDS on the way in and out, so that HBM sees whole lines; a lane's own row there also answers the
+// look-ups by token.  LDS holds [64][V] elements; everything is the wave's own, so fences of the wave order it.
+__device__ __forceinline__ void tok_wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+// n contiguous elements between global memory and LDS, 16 bytes a lane
+template <typename T> __device__ __forceinline__ void tok_stage_in(tok_in<T> x, T* lds, int n) {
+    constexpr int VEC = TokElem<T>::VEC;
+    const int lane = threadIdx.x, nv = n / VEC;
+    u32x4_t* l = reinterpret_cast<u32x4_t*>(lds);
+    int v = lane;
+    for (; v + 192 < nv; v += 256) {
+        u32x4_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = tok_ld16<T>(x + (v + i * 64) * VEC);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[v + i * 64] = r[i];
+    }
+    for (; v < nv; v += 64) l[v] = tok_ld16<T>(x + v * VEC);
+    for (int e = nv * VEC + lane; e < n; e += 64) lds[e] = x[e];
+}
+template <typename T> __device__ __forceinline__ void tok_stage_out(const T* lds, tok_out<T> o, int n) {
+    constexpr int VEC = TokElem<T>::VEC;
+    const int lane = threadIdx.x, nv = n / VEC;
+    const u32x4_t* l = reinterpret_cast<const u32x4_t*>(lds);
+    for (int v = lane; v < nv; v += 64) tok_st16<T>(o + v * VEC, l[v]);
+    for (int e = nv * VEC + lane; e < n; e += 64) o[e] = lds[e];
+}
+// rows [row0, row0 + n) of the logits to LDS
+template <typename T> __device__ __forceinline__ void tok_stage_rows(const TokRows& r, int64_t row0, int n, T* lds) {
+    if (r.n1 == r.rows && r.s1 == r.V) {
+        tok_stage_in<T>(tok_row<T>(r, row0), lds, n * r.V);
+    } else {
+        const int lane = threadIdx.x;
+        for (int i = 0; i < n; ++i) {
+            tok_in<T> x = tok_row<T>(r, row0 + i);
+            if (lane < r.V) lds[i * r.V + lane] = x[lane];
+        }
+    }
+    tok_wave_fence();
+}
+template <typename T> struct TokLane {
+    static constexpr int VEC = TokElem<T>::VEC, NVL = 64 / VEC;
+    float f[64];
+    // the lane's row in LDS; `pad` behind its end
+    __device__ __forceinline__ void load(const T* x, int V, float pad) {
+        const bool vec = V % VEC == 0;                       // rows start at multiples of 16 bytes
+#pragma unroll
+        for (int i = 0; i < NVL; ++i) {
+            if (i * VEC < V) {                               // uniform
+                if (vec) {
+                    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(x + i * VEC);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) f[i * VEC + e] = TokElem<T>::get(v, e);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        f[i * VEC + e] = pad;
+                        if (i * VEC + e < V) f[i * VEC + e] = TokElem<T>::one(x[i * VEC + e]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) f[i * VEC + e] = pad;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* o, int V) const {
+        const bool vec = V % VEC == 0;
+#pragma unroll
+        for (int i = 0; i < NVL; ++i)
+            if (i * VEC < V) {
+                if (vec) {
+                    *reinterpret_cast<u32x4_t*>(o + i * VEC) = TokElem<T>::pack(f + i * VEC);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        if (i * VEC + e < V) o[i * VEC + e] = TokElem<T>::put(f[i * VEC + e]);
+                }
+            }
+    }
+    // over the elements of the row, VEC at a time (the last chunk's pads among them)
+    template <typename F> __device__ __forceinline__ void each(int V, const F& g) {
+#pragma unroll
+        for (int i = 0; i < NVL; ++i)
+            if (i * VEC < V) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) g(i * VEC + e, f[i * VEC + e]);
+            }
+    }
+    __device__ __forceinline__ float max_of(int V, float m) const {
+#pragma unroll
+        for (int i = 0; i < NVL; ++i)
+            if (i * VEC < V) {
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) m = tok_max3(m, f[i * VEC + e], f[i * VEC + e + 1]);
+            }
+        return m;
+    }
+};
+
 // How a row is cut: NT threads x NV vectors a segment.  Whole rows of up to 4096 vectors (64 KB: 16 of 64 registers' vectors
 // a thread) stay one block; longer ones, and rows too few to fill 256 CUs, are cut and joined by a second, small launch.
 struct TokPlan {
@@ -387,3 +490,6 @@ inline TokRows tok_rows_of(uint64_t x, int64_t rows, int64_t n1, int64_t s0, int
 inline int tok_esize(int dtype) { return dtype == 0 ? 4 : 2; }
 // lanes a narrow row takes: 8 elements a lane
 inline int tok_narrow_lanes(int64_t V) { return V <= 64 ? 8 : V <= 128 ? 16 : V <= 256 ? 32 : 64; }
+// one lane a row instead of 8: from TOK_LANE_ROWS rows of up to 64 elements on
+constexpr int64_t TOK_LANE_ROWS = 16384;
+inline bool tok_lane_rows(int64_t V, int64_t rows) { return V <= 64 && rows >= TOK_LANE_ROWS; }

@@ -45,118 +45,124 @@ struct DistRow {
 };
 
 __device__ __forceinline__ double group_sum64(double v) { return tok_group<64, TokSum>(v); }
-// LDS writes of this wave's lanes before its later reads (one wave: in order in hardware, so a compiler fence)
-__device__ __forceinline__ void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
 
-// The first wave's work on a row: p, the loss, and the gradient's factors.  n, S: the sums relative to m (tok_ln) over all
-// elements, or in bucket mode over the unlisted ones.  dup: some id may occur twice.
-__device__ __forceinline__ DistRow dist_epilogue(const DistArgs& a, DistEntries& E, int64_t row, float w, float m, float n,
-                                                 float S, bool dup, int lane) {
-    const int K = a.K;
-    // teacher: drop mode normalises over the entries that are there
-    double shift = 0.0;
-    if (!a.bucket) {
-        float tm = -INFINITY;
-        for (int j = lane; j < K; j += 64)
-            if (E.id[j] >= 0) tm = tok_max(tm, E.t[j]);
-        tm = tok_group<64, TokMax>(tm);
-        double tot = 0.0;
-        if (tm > -INFINITY) {
-            for (int j = lane; j < K; j += 64)
-                if (E.id[j] >= 0) tot += exp((double)E.t[j] - (double)tm);
-            tot = group_sum64(tot);
-            shift = (double)tm + log(tot);
-        }
+// Sums over a row's entries: with s = the largest t (drop mode) or 0 (bucket), e_k = exp(t_k - s),
+//   tot = sum e_k,   acc = sum e_k ( (t_k - s) - (x_k - m) / T )
+// one fp64 exponential an entry; p_k = e_k / tot (drop) or e_k (bucket).
+struct DistTeach {
+    double tot, acc;
+    __device__ __forceinline__ void add(float t, float s, float x, float m, double inv_t) {
+        const double l = (double)t - (double)s, e = exp(l);
+        tot += e;
+        if (e != 0.0) acc += e * (l - (x == -INFINITY ? -(double)INFINITY : ((double)x - (double)m) * inv_t));
     }
-    double P = 0.0;
-    for (int j = lane; j < K; j += 64) {
-        const double p = E.id[j] < 0 ? 0.0 : exp((double)E.t[j] - shift);
-        E.p[j] = (float)p;
-        P += p;
-    }
-    P = group_sum64(P);
-    wave_fence();
-    // ids that occur again: the first occurrence carries the gradient's sum, the others none
-    float psum[DIST_MAX_K / 64];
-#pragma unroll
-    for (int s = 0; s < DIST_MAX_K / 64; ++s) {
-        const int j = s * 64 + lane;
-        psum[s] = -1.f;
-        if (j < K && E.id[j] >= 0) {
-            psum[s] = E.p[j];
-            if (dup) {
-                float sum = 0.f;
-                bool first = true;
-                for (int i = 0; i < K; ++i)
-                    if (E.id[i] == E.id[j]) {
-                        if (i < j) first = false;
-                        sum += E.p[i];
-                    }
-                psum[s] = first ? sum : -1.f;
-            }
-        }
-    }
-    // sums over the vocabulary
-    double nl = 0.0, Sl = 0.0;
-    if (a.bucket) {
-#pragma unroll
-        for (int s = 0; s < DIST_MAX_K / 64; ++s) {
-            const int j = s * 64 + lane;
-            if (j < K && !(psum[s] < 0.f)) {
-                if (E.x[j] == m) nl += m > -INFINITY ? 1.0 : 0.0;
-                else if (m > -INFINITY) Sl += exp(((double)E.x[j] - (double)m) * a.r.dinv_t);
-            }
-        }
-        nl = group_sum64(nl);
-        Sl = group_sum64(Sl);
-    }
-    const double rest = (double)n + (double)S, listed = nl + Sl;
+};
+// A row's loss and the gradient's factors.  rest / listed: the student's sums relative to m over the elements outside / inside
+// the list (drop mode: their sum counts).  shift: ln p_k = t_k - shift.
+struct DistDone {
+    DistRow d;
+    double kl, shift;
+    bool none;
+};
+__device__ __forceinline__ DistDone dist_finish(const DistArgs& a, float m, double rest, double listed, double tot, double acc,
+                                                float s) {
+    DistDone r;
     double sum = rest + listed;
     if (m == INFINITY) sum = (double)NAN;
-    const bool none = sum == 0.0;
-    const double lnS = none ? 0.0 : log(sum);
-    // the loss
-    double kl = 0.0;
-    for (int j = lane; j < K; j += 64) {
-        if (E.id[j] < 0) continue;
-        const double lp = (double)E.t[j] - shift, p = exp(lp);
-        if (p != 0.0) {
-            const double lq = none ? -(double)INFINITY : ((double)E.x[j] - (double)m) * a.r.dinv_t - lnS;
-            kl += p * (lp - lq);
-        }
-    }
-    kl = group_sum64(kl);
-    double A = P, B = P;
+    r.none = sum == 0.0;                                     // nothing left of the student: infinite loss, no gradient
+    const double lnS = r.none ? 0.0 : log(sum);
+    double P, A, B;
     if (a.bucket) {
+        r.shift = 0.0;
+        P = tot;
+        r.kl = acc + (tot != 0.0 ? tot * lnS : 0.0);
+        A = B = P;
         const double p0 = rest == 0.0 ? 0.0 : 1.0 - P;
         if (p0 > 0.0) {
             const double lq0 = listed < rest ? log1p(-listed / sum) : log(rest / sum);
-            kl += p0 * (log(p0) - lq0);
+            r.kl += p0 * (log(p0) - lq0);
             A = P + p0;
             B = A - p0 * (sum / rest);
         }
+    } else {
+        const double lt = tot == 0.0 ? 0.0 : log(tot);
+        r.shift = (tot == 0.0 ? 0.0 : (double)s) + lt;
+        r.kl = tot == 0.0 ? 0.0 : acc / tot - lt + lnS;
+        A = B = tot == 0.0 ? 0.0 : 1.0 + (tot - tot);        // NaN stays NaN
     }
-    DistRow d;
-    d.m = none ? 0.f : m;
-    d.l2S = none ? INFINITY : (float)(lnS * 1.4426950408889634);
-    d.A = (float)A;
-    d.B = (float)B;
-    wave_fence();
+    r.d.m = r.none ? 0.f : m;
+    r.d.l2S = r.none ? INFINITY : (float)(lnS * 1.4426950408889634);
+    r.d.A = (float)A;
+    r.d.B = (float)B;
+    return r;
+}
+// an entry's p for the gradient, in fp32
+__device__ __forceinline__ float dist_p(float t, double shift) {
+    return tok_exp2((float)(((double)t - shift) * 1.4426950408889634));
+}
+
+// The first wave's work on a row: the loss, and each entry's p.  n, S: the student's sums relative to m over all elements, or
+// in bucket mode over the unlisted ones.  dup: some id may occur twice; the first occurrence carries the sum then.
+__device__ __forceinline__ DistRow dist_epilogue(const DistArgs& a, DistEntries& E, int64_t row, float w, float m, float n,
+                                                 float S, bool dup, int lane) {
+    const int K = a.K;
+    float s = -INFINITY;
+    if (!a.bucket) {
+        for (int j = lane; j < K; j += 64)
+            if (E.id[j] >= 0) s = tok_max(s, E.t[j]);
+        s = tok_group<64, TokMax>(s);
+    }
+    if (!(s > -INFINITY)) s = 0.f;
+    DistTeach te{0.0, 0.0};
+    for (int j = lane; j < K; j += 64)
+        if (E.id[j] >= 0) te.add(E.t[j], s, E.x[j], m, a.r.dinv_t);
+    te.tot = group_sum64(te.tot);
+    te.acc = group_sum64(te.acc);
+    bool first[DIST_MAX_K / 64];
+    float nl = 0.f, Sl = 0.f;
 #pragma unroll
-    for (int s = 0; s < DIST_MAX_K / 64; ++s) {
-        const int j = s * 64 + lane;
-        if (j < K) E.p[j] = none ? -1.f : psum[s];
+    for (int q = 0; q < DIST_MAX_K / 64; ++q) {
+        const int j = q * 64 + lane;
+        first[q] = j < K && E.id[j] >= 0;
+        if (dup && first[q])
+            for (int i = 0; i < j; ++i) first[q] &= E.id[i] != E.id[j];
+        if (a.bucket && first[q]) {
+            if (E.x[j] == m) nl += m > -INFINITY ? 1.f : 0.f;
+            else if (m > -INFINITY) Sl += tok_exp2((E.x[j] - m) * a.r.c);
+        }
+    }
+    nl = tok_group<64, TokSum>(nl);
+    Sl = tok_group<64, TokSum>(Sl);
+    const DistDone r = dist_finish(a, m, (double)n + (double)S, (double)nl + (double)Sl, te.tot, te.acc, s);
+    for (int j = lane; j < K; j += 64) E.p[j] = dist_p(E.t[j], r.shift);
+    if (dup) {
+        tok_wave_fence();
+        float sum[DIST_MAX_K / 64];
+#pragma unroll
+        for (int q = 0; q < DIST_MAX_K / 64; ++q) {
+            const int j = q * 64 + lane;
+            sum[q] = 0.f;
+            if (first[q])
+                for (int i = j; i < K; ++i) sum[q] += E.id[i] == E.id[j] ? E.p[i] : 0.f;
+        }
+        tok_wave_fence();
+#pragma unroll
+        for (int q = 0; q < DIST_MAX_K / 64; ++q)
+            if (q * 64 + lane < K) E.p[q * 64 + lane] = sum[q];
+    }
+#pragma unroll
+    for (int q = 0; q < DIST_MAX_K / 64; ++q) {
+        const int j = q * 64 + lane;
+        if (j < K) {
+            if (!first[q] || r.none) E.p[j] = -1.f;
+            if (a.pk) a.pk[row * K + j] = E.p[j];
+        }
     }
     if (lane == 0) {
-        a.loss[row] = (float)((double)w * (double)a.T * (double)a.T * kl);
-        if (a.stat) a.stat[row] = make_float4(d.m, d.l2S, d.A, d.B);
+        a.loss[row] = (float)((double)w * (double)a.T * (double)a.T * r.kl);
+        if (a.stat) a.stat[row] = make_float4(r.d.m, r.d.l2S, r.d.A, r.d.B);
     }
-    if (a.pk)
-        for (int j = lane; j < K; j += 64) a.pk[row * K + j] = E.p[j];
-    return d;
+    return r.d;
 }
 
 __device__ __forceinline__ float dist_q(const DistRow& d, float c, float x) {
@@ -367,12 +373,11 @@ constexpr uint32_t NOT_LISTED = 0xffffffffu;
 template <typename T, int G, bool GRAD>
 __global__ __launch_bounds__(256) void tok_distill_narrow_kernel(DistArgs a) {
     constexpr int RB = 256 / G;
-    __shared__ uint32_t buf[256 * 8];
+    __shared__ uint32_t buf[256 * 8];                        // a row's words belong to its group of lanes: fences of the wave
     const int gl = threadIdx.x & (G - 1), gr = threadIdx.x / G;
     uint32_t* mine = buf + gr * G * 8;
     const int V = a.r.V, K = a.K;
-    const int64_t r0 = (a.r.u0 + blockIdx.x) * RB;
-    const int64_t row = r0 + gr;
+    const int64_t row = (a.r.u0 + blockIdx.x) * RB + gr;
     const bool there = row < a.r.rows;
     const float w = there ? (a.w ? a.w[row] : 1.f) : 0.f;
     const bool live = there && w != 0.f;
@@ -381,22 +386,22 @@ __global__ __launch_bounds__(256) void tok_distill_narrow_kernel(DistArgs a) {
     tok_narrow_load<T>(x, V, gl * 8, live, f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) mine[gl * 8 + e] = NOT_LISTED;
-    __syncthreads();
+    tok_wave_fence();
     bool twice = false;
-    float tm = -INFINITY;
+    float s = -INFINITY;
     if (live)
         for (int j = gl; j < K; j += G) {
             const int64_t id = tok_int(a.ids, a.id64, row * K + j);
             if ((uint64_t)id < (uint64_t)V) {
                 twice |= atomicExch(&mine[id], 0u) != NOT_LISTED;
-                tm = tok_max(tm, a.t[row * K + j]);
+                s = tok_max(s, a.t[row * K + j]);
             }
         }
-    __syncthreads();
+    tok_wave_fence();
     float m = tok_max(tok_max3(tok_max3(f[0], f[1], f[2]), f[3], f[4]), tok_max3(f[5], f[6], f[7]));
     m = tok_group<G, TokMax>(m);
     const TokRef ref = tok_ref(m, a.r.c);
-    DistSums un{0.f, 0.f}, li{0.f, 0.f};                 // unlisted, listed (drop mode needs their sum alone)
+    DistSums un{0.f, 0.f}, li{0.f, 0.f};                     // unlisted, listed (drop mode needs their sum alone)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const bool l = mine[gl * 8 + e] != NOT_LISTED;
@@ -406,83 +411,145 @@ __global__ __launch_bounds__(256) void tok_distill_narrow_kernel(DistArgs a) {
     const float S = tok_group<G, TokSum>(un.S), Sl = tok_group<G, TokSum>(li.S);
     const float n = tok_group<G, TokSum>(un.n), nl = tok_group<G, TokSum>(li.n);
     const double sc = (double)tok_exp2(-ref.dmax);
-    const double rest = (double)n + (double)S * sc, listed = (double)nl + (double)Sl * sc;
-    double sum = rest + listed;
-    if (m == INFINITY) sum = (double)NAN;
-    const bool none = sum == 0.0;
-    const double lnS = none ? 0.0 : log(sum);
-    double shift = 0.0;
-    if (!a.bucket) {
-        tm = tok_group<G, TokMax>(tm);
-        double tot = 0.0;
-        if (live && tm > -INFINITY)
-            for (int j = gl; j < K; j += G) {
-                const int64_t id = tok_int(a.ids, a.id64, row * K + j);
-                if ((uint64_t)id < (uint64_t)V) tot += exp((double)a.t[row * K + j] - (double)tm);
-            }
-        tot = tok_group<G, TokSum>(tot);
-        if (tm > -INFINITY) shift = (double)tm + log(tot);
-    }
-    const bool dup = __ballot(twice) != 0;               // any row of this wave
-    __syncthreads();                                     // the marks have been read
-    double P = 0.0, kl = 0.0;
+    s = a.bucket ? 0.f : tok_group<G, TokMax>(s);
+    if (!(s > -INFINITY)) s = 0.f;
+    const bool dup = __ballot(twice) != 0;                   // any row of this wave
+    DistTeach te{0.0, 0.0};
     if (live)
         for (int j = gl; j < K; j += G) {
             const int64_t id = tok_int(a.ids, a.id64, row * K + j);
+            if ((uint64_t)id < (uint64_t)V) te.add(a.t[row * K + j], s, TokElem<T>::one(x[id]), m, a.r.dinv_t);
+        }
+    te.tot = tok_group<G, TokSum>(te.tot);
+    te.acc = tok_group<G, TokSum>(te.acc);
+    const DistDone r = dist_finish(a, m, (double)n + (double)S * sc, (double)nl + (double)Sl * sc, te.tot, te.acc, s);
+    tok_wave_fence();                                        // the marks have been read
+    if (live && (GRAD || a.pk))
+        for (int j = gl; j < K; j += G) {
+            const int64_t id = tok_int(a.ids, a.id64, row * K + j);
             if ((uint64_t)id >= (uint64_t)V) continue;
-            const double lp = (double)a.t[row * K + j] - shift, p = exp(lp);
-            P += p;
-            if (p != 0.0) {
-                const double xv = (double)TokElem<T>::one(x[id]);
-                kl += p * (lp - (none ? -(double)INFINITY : (xv - (double)m) * a.r.dinv_t - lnS));
-            }
-            float ps = (float)p;
+            float p = dist_p(a.t[row * K + j], r.shift);
             bool first = true;
             if (dup) {
-                ps = 0.f;
+                p = 0.f;
                 for (int i = 0; i < K; ++i)
                     if (tok_int(a.ids, a.id64, row * K + i) == id) {
                         if (i < j) first = false;
-                        ps += (float)exp((double)a.t[row * K + i] - shift);
+                        p += dist_p(a.t[row * K + i], r.shift);
                     }
             }
-            if (first) mine[id] = __float_as_uint(ps);
-            if (a.pk) a.pk[row * K + j] = first && !none ? ps : -1.f;
+            if (first) mine[id] = __float_as_uint(p);
+            if (a.pk) a.pk[row * K + j] = first && !r.none ? p : -1.f;
         }
-    P = tok_group<G, TokSum>(P);
-    kl = tok_group<G, TokSum>(kl);
-    double A = P, B = P;
-    if (a.bucket) {
-        const double p0 = rest == 0.0 ? 0.0 : 1.0 - P;
-        if (p0 > 0.0) {
-            const double lq0 = listed < rest ? log1p(-listed / sum) : log(rest / sum);
-            kl += p0 * (log(p0) - lq0);
-            A = P + p0;
-            B = A - p0 * (sum / rest);
-        }
-    }
-    DistRow d;
-    d.m = none ? 0.f : m;
-    d.l2S = none ? INFINITY : (float)(lnS * 1.4426950408889634);
-    d.A = (float)A;
-    d.B = (float)B;
     if (there && gl == 0) {
-        a.loss[row] = live ? (float)((double)w * (double)a.T * (double)a.T * kl) : 0.f;
-        if (a.stat) a.stat[row] = live ? make_float4(d.m, d.l2S, d.A, d.B) : make_float4(0.f, INFINITY, 0.f, 0.f);
+        a.loss[row] = live ? (float)((double)w * (double)a.T * (double)a.T * r.kl) : 0.f;
+        if (a.stat) a.stat[row] = live ? make_float4(r.d.m, r.d.l2S, r.d.A, r.d.B) : make_float4(0.f, INFINITY, 0.f, 0.f);
     }
-    __syncthreads();
+    tok_wave_fence();
     if constexpr (GRAD) {
         if (there && gl * 8 < V) {
             const float fw = w * a.T;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const uint32_t pb = mine[gl * 8 + e];
-                const float q = dist_q(d, a.r.c, f[e]);
-                const float g = pb == NOT_LISTED ? d.B * q : none ? 0.f : __builtin_fmaf(d.A, q, -__uint_as_float(pb));
+                const float q = dist_q(r.d, a.r.c, f[e]);
+                const float g = pb == NOT_LISTED ? r.d.B * q : r.none ? 0.f : __builtin_fmaf(r.d.A, q, -__uint_as_float(pb));
                 f[e] = live ? fw * g : 0.f;
             }
             tok_narrow_store<T>((tok_out<T>)a.dx + row * V, V, gl * 8, f);
         }
+    }
+}
+
+// Many short rows: a row a lane; the listed tokens are the bits of a 64-bit word, the entries wait in LDS, and so does the
+// gradient's row while the listed tokens are put into it.
+constexpr int DIST_LANE_K = 16;       // 64 rows' entries in 8 KB of LDS
+
+template <typename T, bool GRAD> __global__ __launch_bounds__(64) void tok_distill_lane_kernel(DistArgs a) {
+    extern __shared__ uint64_t lane_lds[];
+    const int V = a.r.V, K = a.K, lane = threadIdx.x;
+    T* rows = reinterpret_cast<T*>(lane_lds);
+    float* ts = reinterpret_cast<float*>(reinterpret_cast<char*>(lane_lds) + (64 * V * sizeof(T) + 15) / 16 * 16);
+    signed char* is = reinterpret_cast<signed char*>(ts + 64 * K);
+    const int64_t row0 = (a.r.u0 + blockIdx.x) * 64, row = row0 + lane;
+    const int nrow = a.r.rows - row0 < 64 ? (int)(a.r.rows - row0) : 64;
+    const bool there = lane < nrow;
+    const float w = there ? (a.w ? a.w[row] : 1.f) : 0.f;
+    const bool live = w != 0.f;
+    for (int i = lane; i < nrow * K; i += 64) {
+        const int64_t id = tok_int(a.ids, a.id64, row0 * K + i);
+        is[i] = (uint64_t)id < (uint64_t)V ? (signed char)id : (signed char)-1;
+        ts[i] = a.t[row0 * K + i];
+    }
+    tok_stage_rows<T>(a.r, row0, nrow, rows);
+    T* x = rows + lane * V;
+    TokLane<T> l;
+    l.load(x, V, -INFINITY);
+    uint64_t in = 0;
+    bool dup = false;
+    float s = -INFINITY;
+    for (int j = 0; live && j < K; ++j) {
+        const int id = is[lane * K + j];
+        if (id < 0) continue;
+        dup |= (in >> id) & 1;
+        in |= 1ull << id;
+        s = tok_max(s, ts[lane * K + j]);
+    }
+    if (a.bucket || !(s > -INFINITY)) s = 0.f;
+    const float m = l.max_of(V, -INFINITY);
+    const TokRef ref = tok_ref(m, a.r.c);
+    DistSums un{0.f, 0.f}, li{0.f, 0.f};
+    if (a.bucket)
+        l.each(V, [&](int e, float f) {
+            const bool listed = (in >> e) & 1;
+            un.add(f, ref, listed);
+            li.add(f, ref, !listed);
+        });
+    else
+        l.each(V, [&](int, float f) { un.add(f, ref, false); });
+    const double sc = (double)tok_exp2(-ref.dmax);
+    DistTeach te{0.0, 0.0};
+    for (int j = 0; live && j < K; ++j) {
+        const int id = is[lane * K + j];
+        if (id >= 0) te.add(ts[lane * K + j], s, TokElem<T>::one(x[id]), m, a.r.dinv_t);
+    }
+    const DistDone r = dist_finish(a, m, (double)un.n + (double)un.S * sc, (double)li.n + (double)li.S * sc, te.tot, te.acc, s);
+    if (there) {
+        a.loss[row] = live ? (float)((double)w * (double)a.T * (double)a.T * r.kl) : 0.f;
+        if (a.stat) a.stat[row] = live ? make_float4(r.d.m, r.d.l2S, r.d.A, r.d.B) : make_float4(0.f, INFINITY, 0.f, 0.f);
+    }
+    const float f = w * a.T, fB = f * r.d.B;
+    float g[DIST_LANE_K];                                    // the entries' gradients, the student's row still in LDS
+#pragma unroll
+    for (int j = 0; j < DIST_LANE_K; ++j) {
+        g[j] = 0.f;
+        const int id = (GRAD || a.pk) && j < K ? is[lane * K + j] : -1;
+        if (id >= 0 && live) {
+            float p = 0.f;
+            bool first = true;
+            if (!dup) {
+                p = dist_p(ts[lane * K + j], r.shift);
+            } else {
+                for (int i = 0; i < K; ++i)
+                    if (is[lane * K + i] == id) {
+                        first &= i >= j;
+                        p += dist_p(ts[lane * K + i], r.shift);
+                    }
+            }
+            if (a.pk) a.pk[row * K + j] = first && !r.none ? p : -1.f;
+            if (!r.none) g[j] = f * __builtin_fmaf(r.d.A, dist_q(r.d, a.r.c, TokElem<T>::one(x[id])), -p);
+        }
+    }
+    if constexpr (GRAD) {
+        l.each(V, [&](int, float& v) { v = live ? fB * dist_q(r.d, a.r.c, v) : 0.f; });
+        if (there) {
+            l.store(x, V);
+#pragma unroll
+            for (int j = 0; j < DIST_LANE_K; ++j)            // an id that occurs twice is stored twice, the same value
+                if (j < K && live && is[lane * K + j] >= 0) x[is[lane * K + j]] = TokElem<T>::put(g[j]);
+        }
+        tok_wave_fence();
+        tok_stage_out<T>(rows, (tok_out<T>)a.dx + row0 * V, nrow * V);
     }
 }
 
@@ -582,7 +649,6 @@ template <typename T, int G> __global__ __launch_bounds__(256) void tok_distill_
         }
         tok_narrow_store<T>((tok_out<T>)a.dx + row * V, V, gl * 8, f);
     }
-    __syncthreads();
 }
 
 // ---- launchers -------------------------------------------------------------------------------------------------------------
@@ -612,6 +678,11 @@ template <typename T, bool GRAD> static void distill_wide(const DistArgs& a, con
     else if constexpr (GRAD) tok_launch(tok_distill_kernel<T, 512, 16, GRAD>, units, nt, 0, s, a);
 }
 template <typename T, bool GRAD> static void distill_narrow(const DistArgs& a, hipStream_t s) {
+    if (tok_lane_rows(a.r.V, a.r.rows) && a.K <= DIST_LANE_K) {
+        const size_t lds = (64 * a.r.V * sizeof(T) + 15) / 16 * 16 + 64 * a.K * 5;
+        tok_launch(tok_distill_lane_kernel<T, GRAD>, (a.r.rows + 63) / 64, 64, lds, s, a);
+        return;
+    }
     const int G = tok_narrow_lanes(a.r.V);
     const int64_t rb = 256 / G;
     const int64_t units = (a.r.rows + rb - 1) / rb;

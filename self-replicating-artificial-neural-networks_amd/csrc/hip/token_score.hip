@@ -51,12 +51,13 @@ __device__ __forceinline__ float score_finish(const ScoreArgs& a, int64_t row, f
     }
     return none ? 0.f : lnS;
 }
+// lanes = 0: without the alternatives
 __device__ __forceinline__ void score_skip(const ScoreArgs& a, int64_t row, int lane, int lanes) {
     if (lane == 0) {
         if (a.lp) a.lp[row] = 0.f;
         a.ent[row] = 0.f;
     }
-    for (int j = lane; j < a.k; j += lanes) {
+    for (int j = lane; lanes && j < a.k; j += lanes) {
         a.ids[row * a.k + j] = -1;
         a.top[row * a.k + j] = -INFINITY;
     }
@@ -473,6 +474,75 @@ __global__ __launch_bounds__(256) void tok_score_narrow_kernel(ScoreArgs a) {
     }
 }
 
+// Many short rows: a row a lane.  The k-th round takes the lowest index that holds the maximum of what is left (taken ones, and
+// what lies behind the row, are NaN, which no maximum and no comparison sees).  The alternatives go out through LDS when
+// they fit the rows' place there (out != 0).
+template <typename T> __global__ __launch_bounds__(64) void tok_score_lane_kernel(ScoreArgs a, int out) {
+    extern __shared__ uint64_t lane_lds[];
+    T* rows = reinterpret_cast<T*>(lane_lds);
+    const int V = a.r.V, k = a.k, lane = threadIdx.x;
+    const int64_t row0 = (a.r.u0 + blockIdx.x) * 64, row = row0 + lane;
+    const int nrow = a.r.rows - row0 < 64 ? (int)(a.r.rows - row0) : 64;
+    const bool there = lane < nrow;
+    int64_t tgt = 0;
+    if (a.y && there) tgt = score_target(a, row);
+    tok_stage_rows<T>(a.r, row0, nrow, rows);
+    const bool skip = a.y && tgt == a.ignore, valid_t = !a.y || (uint64_t)tgt < (uint64_t)V;
+    const T* x = rows + lane * V;                            // lanes behind the last row read what is there, and write nothing
+    float xt = 0.f;
+    if (a.y && valid_t && !skip) xt = TokElem<T>::one(x[tgt]);
+    TokLane<T> l;
+    l.load(x, V, -INFINITY);
+    const float m = l.max_of(V, -INFINITY);
+    const TokRef ref = tok_ref(m, a.r.c);
+    ScoreSums sum{0.f, 0.f, 0.f};
+    l.each(V, [&](int, float f) { sum.add(f, ref); });
+    const float sc = tok_exp2(-ref.dmax);
+    const float W = (sum.W - ref.dmax * sum.S) * sc, S = m == INFINITY ? NAN : sum.S * sc;
+    float lnS = 0.f;
+    if (there && !skip) lnS = score_finish(a, row, m, sum.n, S, W, xt, valid_t, true);
+    else if (there) score_skip(a, row, 0, 0);
+    if (k) {
+        tok_wave_fence();                                    // the rows' place in LDS is free
+        int* ids = reinterpret_cast<int*>(lane_lds);
+        float* lps = reinterpret_cast<float*>(ids + 64 * k);
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+            if (e >= V) l.f[e] = NAN;
+        float top = m;
+        for (int j = 0; j < k; ++j) {
+            int at = -1;
+            bool found = !(S == S);                          // a row with a NaN or +inf logit has no ranking
+            l.each(V, [&](int e, float& f) {
+                const bool hit = f == top && !found;
+                found |= hit;
+                at = hit ? e : at;
+                f = hit ? NAN : f;
+            });
+            float lp = at < 0 ? NAN : score_toplp(a, top, m, lnS);
+            if (skip) {
+                at = -1;
+                lp = -INFINITY;
+            }
+            if (out) {
+                ids[lane * k + j] = at;
+                lps[lane * k + j] = lp;
+            } else if (there) {
+                a.ids[row * k + j] = at;
+                a.top[row * k + j] = lp;
+            }
+            top = l.max_of(V, NAN);
+        }
+        if (out) {
+            tok_wave_fence();
+            for (int i = lane; i < nrow * k; i += 64) {
+                a.ids[row0 * k + i] = ids[i];
+                a.top[row0 * k + i] = lps[i];
+            }
+        }
+    }
+}
+
 // ---- backward ----------------------------------------------------------------------------------------------------------
 struct ScoreGradArgs {
     TokRows r;
@@ -596,6 +666,12 @@ template <typename T> static void score_wide(const ScoreArgs& a, const TokPlan& 
     else tok_launch(tok_score_kernel<T, 256, 16>, units, nt, 0, s, a);
 }
 template <typename T> static void score_narrow(const ScoreArgs& a, hipStream_t s) {
+    if (tok_lane_rows(a.r.V, a.r.rows)) {
+        const size_t rows = (size_t)64 * a.r.V * sizeof(T), out = (size_t)64 * a.k * 8;
+        const bool fits = out <= 16384;
+        tok_launch(tok_score_lane_kernel<T>, (a.r.rows + 63) / 64, 64, fits && out > rows ? out : rows, s, a, fits ? 1 : 0);
+        return;
+    }
     const int G = tok_narrow_lanes(a.r.V);
     const int64_t rb = 256 / G;
     const int64_t units = (a.r.rows + rb - 1) / rb;

@@ -50,14 +50,25 @@ def _score_tols(x, ref, T):
     return lp, h
 
 
-def _check_score(x, y, T, k, grad=True, seed=0):
+def _first(t, tile):
+    """The first of ``tile`` copies of the rows, after a look that all of them came out the same."""
+    if t is None or tile == 1:
+        return t
+    t = t.reshape((tile, -1) + t.shape[1:])
+    assert _same(t.float(), t[:1].float().expand_as(t))
+    return t[0]
+
+
+def _check_score(x, y, T, k, grad=True, seed=0, tile=1):
+    """``tile``: the rows are given that many times over (launch shapes that only many rows take)."""
     R, V = x.shape[0], x.shape[-1]
     g = torch.Generator().manual_seed(seed + 99)
     gl, gh = torch.randn(R, generator=g), torch.randn(R, generator=g)
     ref = O.score(x, y, T, k, IGN, gl if grad else None, gh if grad else None)
-    xd = x.cuda().requires_grad_(grad)
-    yd = None if y is None else y.cuda()
-    r = TO.token_logprobs(xd, yd, temperature=T, top_k=k, ignore_index=IGN)
+    xd = x.repeat(tile, 1).cuda().requires_grad_(grad)
+    yd = None if y is None else y.repeat(tile).cuda()
+    r = full = TO.token_logprobs(xd, yd, temperature=T, top_k=k, ignore_index=IGN)
+    r = TO.TokenLogprobs(*(_first(v, tile) for v in r))
     tl, th = _score_tols(x, ref, T)
     if y is not None:
         _close(r.logprob, ref["logprob"], tl, "logprob")
@@ -67,11 +78,12 @@ def _check_score(x, y, T, k, grad=True, seed=0):
         tt = O.sum_error(x, T) + 6 * O.U * ref["top_logprobs"].abs().nan_to_num(0, 0, 0)
         _close(r.top_logprobs, ref["top_logprobs"], tt, "top_logprobs")
     if grad:
-        outs, gs = [r.entropy], [gh.cuda()]
+        outs, gs = [full.entropy], [gh.repeat(tile).cuda()]
         if y is not None:
-            outs.append(r.logprob)
-            gs.append(gl.cuda())
+            outs.append(full.logprob)
+            gs.append(gl.repeat(tile).cuda())
         dx, = torch.autograd.grad(outs, [xd], gs)
+        dx = _first(dx, tile)
         assert dx.dtype == x.dtype and dx.shape == x.shape
         # q carries the sum's error and its exponent's (|log2 q| U, three roundings); log q + H carries both bounds
         lq, _ = O.log_q(x, T)
@@ -257,7 +269,7 @@ def _teacher(x, K, T, g, truncated=False):
     return ids, lp
 
 
-def _check_distill(x, ids, t, T, tail, w):
+def _check_distill(x, ids, t, T, tail, w, tile=1):
     R, V = x.shape
     loss, dx = O.distill(x, ids, t, T, tail, w)
     lq, none = O.log_q(x, T)
@@ -279,16 +291,16 @@ def _check_distill(x, ids, t, T, tail, w):
     big = (dx.abs() / (wv.abs()[:, None] * T).clamp_min(1e-300)).nan_to_num(0, 0, 0)
     tg = wv.abs()[:, None] * T * ((q * 2 + big) * (2 * e + 8 * O.U) + 6 * O.U * p)
     tg = tg.nan_to_num() + O.half_ulp(dx.nan_to_num(), x.dtype) * (1 + 1e-6)
-    xd = x.cuda().requires_grad_(True)
-    i, tt, wd = ids.cuda(), t.cuda(), None if w is None else w.cuda()
+    xd = x.repeat(tile, 1).cuda().requires_grad_(True)
+    i, tt, wd = ids.repeat(tile, 1).cuda(), t.repeat(tile, 1).cuda(), None if w is None else w.repeat(tile).cuda()
     got = TO.topk_distill_loss(xd, i, tt, temperature=T, tail=tail, weight=wd)
-    _close(got, loss, tl, "loss")
-    ones = torch.ones(R, device="cuda")
+    _close(_first(got, tile), loss, tl, "loss")
+    ones = torch.ones(R * tile, device="cuda")
     d1, = torch.autograd.grad(got, xd, ones)
-    _close(d1, dx, tg, "autograd gradient")
+    _close(_first(d1, tile), dx, tg, "autograd gradient")
     l2, d2 = TO.topk_distill_grad(xd, i, tt, temperature=T, tail=tail, weight=wd)
-    _close(l2, loss, tl, "loss (one pass)")
-    _close(d2, dx, tg, "gradient (one pass)")
+    _close(_first(l2, tile), loss, tl, "loss (one pass)")
+    _close(_first(d2, tile), dx, tg, "gradient (one pass)")
     assert not l2.requires_grad and not d2.requires_grad
     out = torch.full_like(xd, 3.0)
     l3, d3 = TO.topk_distill_grad(xd, i, tt, temperature=T, tail=tail, weight=wd, out=out)
@@ -380,6 +392,52 @@ def test_distill_gradient_against_differences():
             e[v] = h
             up, dn = (TO.topk_distill_loss((x + s * e).cuda(), ids.cuda(), t.cuda(), tail=tail) for s in (1, -1))
             assert float(((up - dn) / (2 * h) - dx[:, v]).abs().max()) <= tol
+
+
+# ---- many short rows (a row a lane) --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("V", [1, 2, 7, 8, 9, 12, 31, 33, 40, 63, 64])
+def test_many_short_rows(V, dtype):
+    R, tile = 52, 400
+    x, at, g = _logits(R, V, dtype, V)
+    at[1] = IGN
+    if V > 6:
+        x[2] = -math.inf
+        x[3] = torch.finfo(DTYPES[dtype]).min
+        x[4, 2:] = -math.inf
+        x[5, 3] = math.nan
+        x[6, 3] = math.inf
+        x[7] = 0.5
+        x[8, ::2], x[8, 1::2] = 0.0, -0.0
+        at[9] = V
+    _check_score(x, at, 0.7, min(V, 9), tile=tile)
+    _check_score(x, None, 1.0, V, grad=False, tile=tile)
+    x = x[9:]
+    ids, t = _teacher(x, min(V, 8), 2.0, g, truncated=V == 33)
+    w = torch.rand(R - 9, generator=g) + 0.5
+    w[2] = 0
+    x[2] = math.nan
+    for tail in ("drop", "bucket"):
+        _check_distill(x, ids, t, 2.0, tail, w, tile=tile)
+
+
+@pytest.mark.parametrize("tail", ["drop", "bucket"])
+def test_many_short_rows_with_odd_entries(tail):
+    V, tile = 40, 600
+    x, _, g = _logits(31, V, "fp32", 11)
+    ids = torch.randint(0, V, (31, 12), generator=g)
+    t = torch.log_softmax(torch.randn(31, 20, generator=g), -1)[:, :12].contiguous()
+    ids[0, 1:4] = ids[0, 0]
+    ids[1, ::2] = -1
+    ids[2, 3:] = V + torch.arange(9) * (1 << 33)
+    t[3, 2:5] = -math.inf
+    ids[4] = -1
+    ids[5] = ids[5, 0]
+    x[6] = -math.inf
+    x[7, ids[7, 0]] = -math.inf
+    x[8] = torch.where(torch.zeros(V, dtype=torch.bool).scatter_(0, ids[8], True), x[8], -math.inf)
+    x[9, 4] = math.inf
+    _check_distill(x, ids, t, 1.5, tail, None, tile=tile)
 
 
 # ---- together, streams, graphs --------------------------------------------------------------------------------------------
