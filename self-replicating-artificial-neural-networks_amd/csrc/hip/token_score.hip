@@ -474,9 +474,10 @@ __global__ __launch_bounds__(256) void tok_score_narrow_kernel(ScoreArgs a) {
     }
 }
 
-// Many short rows: a row a lane.  The k-th round takes the lowest index that holds the maximum of what is left (taken ones, and
-// what lies behind the row, are NaN, which no maximum and no comparison sees).  The alternatives go out through LDS when
-// they fit the rows' place there (out != 0).
+// Many short rows: a row a lane.  The row's eighths keep their maxima in registers; a round takes the lowest one that holds the
+// maximum, reads those 8 elements of the row in LDS, and marks the lowest that holds it as taken (NaN, which no maximum and no
+// comparison sees).  ~65 operations a round; a pass over the row's registers takes ~180.  The alternatives go out through
+// LDS too when they are few (out = 1).
 template <typename T> __global__ __launch_bounds__(64) void tok_score_lane_kernel(ScoreArgs a, int out) {
     extern __shared__ uint64_t lane_lds[];
     T* rows = reinterpret_cast<T*>(lane_lds);
@@ -503,35 +504,53 @@ template <typename T> __global__ __launch_bounds__(64) void tok_score_lane_kerne
     if (there && !skip) lnS = score_finish(a, row, m, sum.n, S, W, xt, valid_t, true);
     else if (there) score_skip(a, row, 0, 0);
     if (k) {
-        tok_wave_fence();                                    // the rows' place in LDS is free
-        int* ids = reinterpret_cast<int*>(lane_lds);
+        T* mine = rows + lane * V;
+        int* ids = reinterpret_cast<int*>(reinterpret_cast<char*>(lane_lds) + (64 * V * sizeof(T) + 15) / 16 * 16);
         float* lps = reinterpret_cast<float*>(ids + 64 * k);
+        float cm[8];
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
-            if (e >= V) l.f[e] = NAN;
-        float top = m;
+        for (int i = 0; i < 8; ++i) {
+            cm[i] = NAN;
+            if (i * 8 < V) {                                 // pads are -inf: an eighth of nothing else has maximum -inf
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) cm[i] = tok_max3(cm[i], l.f[i * 8 + e], l.f[i * 8 + e + 1]);
+            }
+        }
         for (int j = 0; j < k; ++j) {
+            float top = NAN;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i * 8 < V) top = tok_max(top, cm[i]);
+            int c = 0;
+#pragma unroll
+            for (int i = 7; i >= 0; --i)
+                if (i * 8 < V) c = cm[i] == top ? i : c;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = c * 8 + e < V ? TokElem<T>::one(mine[c * 8 + e]) : NAN;
             int at = -1;
-            bool found = !(S == S);                          // a row with a NaN or +inf logit has no ranking
-            l.each(V, [&](int e, float& f) {
-                const bool hit = f == top && !found;
-                found |= hit;
-                at = hit ? e : at;
-                f = hit ? NAN : f;
-            });
-            float lp = at < 0 ? NAN : score_toplp(a, top, m, lnS);
+#pragma unroll
+            for (int e = 7; e >= 0; --e) at = v[e] == top ? e : at;
+            float rest = NAN;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) rest = tok_max(rest, e == at ? NAN : v[e]);
+            if (at >= 0) mine[c * 8 + at] = TokElem<T>::put(NAN);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i * 8 < V) cm[i] = i == c ? rest : cm[i];
+            int id = at < 0 || !(S == S) ? -1 : c * 8 + at;  // a row with a NaN or +inf logit has no ranking
+            float lp = id < 0 ? NAN : score_toplp(a, top, m, lnS);
             if (skip) {
-                at = -1;
+                id = -1;
                 lp = -INFINITY;
             }
             if (out) {
-                ids[lane * k + j] = at;
+                ids[lane * k + j] = id;
                 lps[lane * k + j] = lp;
             } else if (there) {
-                a.ids[row * k + j] = at;
+                a.ids[row * k + j] = id;
                 a.top[row * k + j] = lp;
             }
-            top = l.max_of(V, NAN);
         }
         if (out) {
             tok_wave_fence();
@@ -667,9 +686,9 @@ template <typename T> static void score_wide(const ScoreArgs& a, const TokPlan& 
 }
 template <typename T> static void score_narrow(const ScoreArgs& a, hipStream_t s) {
     if (tok_lane_rows(a.r.V, a.r.rows)) {
-        const size_t rows = (size_t)64 * a.r.V * sizeof(T), out = (size_t)64 * a.k * 8;
-        const bool fits = out <= 16384;
-        tok_launch(tok_score_lane_kernel<T>, (a.r.rows + 63) / 64, 64, fits && out > rows ? out : rows, s, a, fits ? 1 : 0);
+        const int out = a.k && a.k <= 16;                    // 8 KB of LDS at most
+        const size_t lds = (64 * a.r.V * sizeof(T) + 15) / 16 * 16 + (out ? 64 * a.k * 8 : 0);
+        tok_launch(tok_score_lane_kernel<T>, (a.r.rows + 63) / 64, 64, lds, s, a, out);
         return;
     }
     const int G = tok_narrow_lanes(a.r.V);
