@@ -180,20 +180,25 @@ __device__ __forceinline__ uint64_t tok_key(float x, int i) {
 __device__ __forceinline__ int tok_key_index(uint64_t k) { return (int)~(uint32_t)k; }
 __device__ __forceinline__ float tok_key_value(uint64_t k) { return tok_unorder((uint32_t)(k >> 32)); }
 
-// Ranks the n distinct keys of an LDS list by counting the larger ones, 8 lanes a key: f(rank, key) for ranks below k, from one
-// lane.  n is the same in every thread; NT threads call.
-template <int NT, typename F> __device__ __forceinline__ void tok_rank(uint64_t* keys, int n, int k, const F& f) {
+// Ranks the n distinct keys of an LDS list (16-byte aligned) by counting the larger ones, 8 lanes a key, two keys a read: f(rank,
+// key) for ranks below k, from one lane.  n is the same in every thread; NT threads call.
+template <int NT, typename F> __device__ __forceinline__ void tok_rank(const uint64_t* keys, int n, int k, const F& f) {
     const int tid = threadIdx.x, l = tid & 7;
+    const ulonglong2* two = reinterpret_cast<const ulonglong2*>(keys);
     for (int i0 = 0; i0 < n; i0 += NT / 8) {
         const int i = i0 + (tid >> 3);
         const uint64_t key = i < n ? keys[i] : 0;
         uint32_t c = 0;
         int j = l;
-        for (; j + 24 < n; j += 32) {
-            const uint64_t a = keys[j], b = keys[j + 8], d = keys[j + 16], e = keys[j + 24];
-            c += (a > key) + (b > key) + (d > key) + (e > key);
+        for (; j + 24 < n / 2; j += 32) {
+            const ulonglong2 a = two[j], b = two[j + 8], d = two[j + 16], e = two[j + 24];
+            c += (a.x > key) + (a.y > key) + (b.x > key) + (b.y > key) + (d.x > key) + (d.y > key) + (e.x > key) + (e.y > key);
         }
-        for (; j < n; j += 8) c += keys[j] > key;
+        for (; j < n / 2; j += 8) {
+            const ulonglong2 a = two[j];
+            c += (a.x > key) + (a.y > key);
+        }
+        if ((n & 1) && l == 0) c += keys[n - 1] > key;
         c = tok_group<8, TokSum>(c);
         if (l == 0 && i < n && (int)c < k) f((int)c, key);
     }
@@ -225,27 +230,54 @@ __device__ __forceinline__ TokRef tok_ref(float m, float c) {
 // ln(n + S) of a row's sums (n elements at the maximum, S over the others)
 __device__ __forceinline__ float tok_ln(float n, float S) { return n == 1.f ? log1pf(S) : logf(n + S); }
 
+// lanes below this one whose bit is set
+__device__ __forceinline__ int tok_below(uint64_t mask) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
 // Vectors that need a look at each element (one with the maximum, with candidates of the top k, with listed tokens) go, data
-// and place, to this LDS list, out of the unrolled pass.  Slots are handed out by an atomic, in any order; what is summed is
-// summed by the thread that pushed the vector, along its own chain of slots, so the sums do not depend on that order.
+// and place, to their wave's list in LDS, out of the unrolled pass.  Slots are counted by ballots: no atomics, one order.
+// What is summed is summed by the thread that pushed the vector, along its own chain of slots.
 template <int CAP> struct TokSpecial {
     u32x4_t data[CAP];
     int at[CAP], next[CAP];      // vector of the segment (bit 31: to be summed), the thread's slot before this one
-    int n;
-    __device__ __forceinline__ void push(const u32x4_t& v, int where, bool sum, int& chain) {
-        const int i = atomicAdd(&n, 1);
-        if (i < CAP) {
+    // all lanes of the wave; n: the list's length so far (over CAP: it did not fit)
+    __device__ __forceinline__ void push(bool hit, const u32x4_t& v, int where, bool sum, int& chain, int& n) {
+        const uint64_t mask = __ballot(hit);
+        if (mask == 0) return;
+        const int i = n + tok_below(mask);
+        if (hit && i < CAP) {
             data[i] = v;
             at[i] = where | (sum ? (int)0x80000000 : 0);
             next[i] = chain;
             chain = i;
         }
+        n += (int)__popcll(mask);
     }
     __device__ __forceinline__ int vec(int slot) const { return at[slot] & 0x7fffffff; }
     template <typename T> __device__ __forceinline__ float get(int slot, int e) const {
         return TokElem<T>::one(reinterpret_cast<const T*>(&data[slot])[e]);
     }
 };
+
+// A lower bound of the k-th largest of the wave's lanes' values (1 <= k <= 64): at least k of them are at or above it, seldom
+// many more.  Bisection on the value, counted by ballots; -inf where fewer than k lanes have more.
+__device__ __forceinline__ float tok_kth_bound(float v, int k) {
+    const float hi0 = tok_group<64, TokMax>(v);
+    float lo = tok_group<64, TokMin>(v > -INFINITY ? v : INFINITY), hi = hi0;
+    if (k == 1) return hi0;
+    if ((int)__popcll(__ballot(v >= lo)) < k || !(hi < INFINITY)) return -INFINITY;
+    for (int it = 0; it < 10; ++it) {
+        const float mid = 0.5f * lo + 0.5f * hi;
+        const int c = (int)__popcll(__ballot(v >= mid));
+        if (c >= k) {
+            lo = mid;
+            if (c <= k + (k >> 2) + 1) break;
+        } else {
+            hi = mid;
+        }
+    }
+    return lo;
+}
 
 // A segment of a row in registers: NV 16-byte vectors a thread and one of the < VEC last elements of the row.  Vector
 // i * NT + tid of the segment is r[i]; vm[i] its maximum.
@@ -490,6 +522,9 @@ inline TokRows tok_rows_of(uint64_t x, int64_t rows, int64_t n1, int64_t s0, int
 inline int tok_esize(int dtype) { return dtype == 0 ? 4 : 2; }
 // lanes a narrow row takes: 8 elements a lane
 inline int tok_narrow_lanes(int64_t V) { return V <= 64 ? 8 : V <= 128 ? 16 : V <= 256 ? 32 : 64; }
-// one lane a row instead of 8: from TOK_LANE_ROWS rows of up to 64 elements on
-constexpr int64_t TOK_LANE_ROWS = 16384;
-inline bool tok_lane_rows(int64_t V, int64_t rows) { return V <= 64 && rows >= TOK_LANE_ROWS; }
+// A row a lane instead of a row on 8 lanes: where 8 lanes of 8 elements would idle (rows of up to 160 bytes, which also keeps 15
+// waves' rows in a CU's LDS) and waves of 64 rows still fill the chip.  A single such wave takes longer (8.4 us with five
+// alternatives, 4.9 on 8 lanes); at V = 40 the two meet near 50,000 rows (fp32, 65,536 rows: 9.6 us against 13.3), at V = 64
+// in fp32 the 8 lanes stay ahead (179,200 rows: 12.9 us against 17.9 without alternatives).
+constexpr int64_t TOK_LANE_ROWS = 65536;
+inline bool tok_lane_rows(int64_t V, int esize, int64_t rows) { return V <= 64 && V * esize <= 160 && rows >= TOK_LANE_ROWS; }

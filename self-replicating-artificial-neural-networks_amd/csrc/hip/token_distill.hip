@@ -193,13 +193,14 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void to
     constexpr int WORDS = NT * NV * VEC / 32 + 1;
     __shared__ DistEntries E;
     __shared__ uint32_t bits[WORDS];                         // listed tokens of the segment
-    constexpr int SPECIAL = NT == 64 ? 192 : 512;
-    __shared__ TokSpecial<SPECIAL> list;
+    constexpr int SPECIAL = NT == 64 ? 192 : NT == 256 ? 128 : 96;     // a wave
+    __shared__ TokSpecial<SPECIAL> lists[NW];
     __shared__ float red[NW][3];
-    __shared__ int dup;
+    __shared__ int dup, over;                                // an id occurs twice; some wave's list did not fit
     __shared__ DistRow rowd;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    TokSpecial<SPECIAL>& list = lists[wave];
     const int nvec_row = a.r.V / VEC, ntail_row = a.r.V - nvec_row * VEC;
     const int64_t u = a.r.u0 + blockIdx.x;
     const int64_t row = a.nseg == 1 ? u : u / a.nseg;
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void to
     TokSeg<T, NT, NV> s;
     s.load(x + e0, nv, ntail);
     for (int i = tid; i < WORDS; i += NT) bits[i] = 0;
-    if (tid == 0) dup = list.n = 0;
+    if (tid == 0) dup = over = 0;
     for (int j = tid; j < a.K; j += NT) dist_load_entry<T>(a, E, row, x, j);
     __syncthreads();
     // mark this segment's listed tokens; a bit found set already means an id that occurs twice
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void to
     for (int k = 1; k < NW; ++k) m = tok_max(m, red[k][0]);
     const TokRef ref = tok_ref(m, a.r.c);
     DistSums sum{0.f, 0.f};
-    int chain = -1;
+    int chain = -1, nl = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         if (i * NT < nv) {
@@ -257,19 +258,19 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void to
                 const uint8_t by = reinterpret_cast<const uint8_t*>(bits)[VEC == 8 ? at : at >> 1];
                 special |= (VEC == 8 ? by : by & (15u << ((at & 1) * 4))) != 0;
             }
-            if (special) list.push(s.r[i], i * NT + tid, true, chain);
+            list.push(special, s.r[i], i * NT + tid, true, chain, nl);
             sum.S += special ? 0.f : cs;
         }
     }
+    if (nl > SPECIAL && lane == 0) over = 1;
+    tok_wave_fence();
+    for (; chain >= 0; chain = list.next[chain]) {
+        const int at = list.vec(chain) * VEC;
+        const uint32_t out = a.bucket ? bits[at >> 5] >> (at & 31) : 0;          // a vector's bits lie in one word
+        for (int e = 0; e < VEC; ++e) sum.add(list.template get<T>(chain, e), ref, (out >> e) & 1);
+    }
     __syncthreads();
-    const int nl = list.n;
-    if (nl <= SPECIAL) {
-        for (; chain >= 0; chain = list.next[chain]) {
-            const int at = list.vec(chain) * VEC;
-            const uint32_t out = a.bucket ? bits[at >> 5] >> (at & 31) : 0;      // a vector's bits lie in one word
-            for (int e = 0; e < VEC; ++e) sum.add(list.template get<T>(chain, e), ref, (out >> e) & 1);
-        }
-    } else {                                             // thousands of elements at the maximum: one by one, read again
+    if (over) {                                              // thousands of elements at the maximum: one by one, read again
         sum = DistSums{0.f, 0.f};
         for (int v = tid; v < nv; v += NT) {
             const u32x4_t r = tok_ld16<T>(x + e0 + (int64_t)v * VEC);
@@ -466,7 +467,7 @@ __global__ __launch_bounds__(256) void tok_distill_narrow_kernel(DistArgs a) {
 constexpr int DIST_LANE_K = 16;       // 64 rows' entries in 8 KB of LDS
 
 template <typename T, bool GRAD> __global__ __launch_bounds__(64) void tok_distill_lane_kernel(DistArgs a) {
-    extern __shared__ uint64_t lane_lds[];
+    extern __shared__ __attribute__((aligned(16))) uint64_t lane_lds[];
     const int V = a.r.V, K = a.K, lane = threadIdx.x;
     T* rows = reinterpret_cast<T*>(lane_lds);
     float* ts = reinterpret_cast<float*>(reinterpret_cast<char*>(lane_lds) + (64 * V * sizeof(T) + 15) / 16 * 16);
@@ -678,7 +679,7 @@ template <typename T, bool GRAD> static void distill_wide(const DistArgs& a, con
     else if constexpr (GRAD) tok_launch(tok_distill_kernel<T, 512, 16, GRAD>, units, nt, 0, s, a);
 }
 template <typename T, bool GRAD> static void distill_narrow(const DistArgs& a, hipStream_t s) {
-    if (tok_lane_rows(a.r.V, a.r.rows) && a.K <= DIST_LANE_K) {
+    if (tok_lane_rows(a.r.V, sizeof(T), a.r.rows) && a.K <= DIST_LANE_K) {
         const size_t lds = (64 * a.r.V * sizeof(T) + 15) / 16 * 16 + 64 * a.K * 5;
         tok_launch(tok_distill_lane_kernel<T, GRAD>, (a.r.rows + 63) / 64, 64, lds, s, a);
         return;

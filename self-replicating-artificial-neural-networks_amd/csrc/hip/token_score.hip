@@ -83,13 +83,15 @@ template <typename T, int NT, int NV>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4 : 5))) void tok_score_kernel(ScoreArgs a) {
     constexpr int VEC = TokElem<T>::VEC, NW = NT / 64;
     // one-wave rows: 8 KB of lists a block, or LDS would keep waves away
-    constexpr int SPECIAL = NT == 64 ? 192 : 512, CAND = NT == 64 ? 512 : 1024;
+    constexpr int SPECIAL = NT == 64 ? 192 : 128;     // vectors a wave
+    constexpr int CAND = NT == 64 ? 512 : 1024;
     __shared__ float red[NW][3];
     __shared__ uint64_t best[NW];
-    __shared__ TokSpecial<SPECIAL> list;
-    __shared__ uint64_t cand[CAND];
-    __shared__ int ncand;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ TokSpecial<SPECIAL> lists[NW];
+    __shared__ __attribute__((aligned(16))) uint64_t cand[CAND];
+    __shared__ int ncand;                                    // over CAND: some list did not fit
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    TokSpecial<SPECIAL>& list = lists[wave];
     const int nvec_row = a.r.V / VEC;
     const int64_t u = a.r.u0 + blockIdx.x;
     const int64_t row = a.nseg == 1 ? u : u / a.nseg;
@@ -116,19 +118,11 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
     const float tm = s.max_of();
     const float wm0 = tok_group<64, TokMax>(tm);
     float wb = wm0;
-    if (a.k) {
-        // this wave's share of the bound: its kk-th largest thread maximum (ties counted together)
+    if (a.k > 1) {
+        // this wave's share of the bound
         const int kk = NW == 1 ? a.k : (a.k + NW - 1) / NW;
         if (kk <= 64) {
-            float cur = tm;
-            int left = kk;
-            while (true) {
-                const int hit = (int)__popcll(__ballot(cur == wb));
-                if (hit >= left || hit == 0 || wb == -INFINITY) break;     // 0: NaN
-                left -= hit;
-                cur = cur == wb ? -INFINITY : cur;
-                wb = tok_group<64, TokMax>(cur);
-            }
+            wb = tok_kth_bound(tm, kk);
         } else {
             // one wave, k > 64: two elements a lane (the two best vectors' maxima) at or above the smallest second one
             float b1 = s.xt, b2 = -INFINITY;
@@ -144,7 +138,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
         red[wave][0] = wm0;
         red[wave][1] = wb;
     }
-    if (tid == 0) list.n = ncand = 0;
+    if (tid == 0) ncand = 0;
     __syncthreads();
     float m = red[0][0], B = red[0][1];
 #pragma unroll
@@ -152,9 +146,10 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
         m = tok_max(m, red[w][0]);
         B = fminf(B, red[w][1]);
     }
+    if (a.k <= 1) B = m;
     const TokRef ref = tok_ref(m, a.r.c);
     ScoreSums sum{0.f, 0.f, 0.f};
-    int chain = -1;
+    int chain = -1, nl = 0;                                  // the wave's vectors
     if (B > -INFINITY) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -168,29 +163,47 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
                     cw = __builtin_fmaf(ev, tok_max(d, -200.f), cw);
                 }
                 const bool top = s.vm[i] == m;
-                if (s.vm[i] >= B) list.push(s.r[i], i * NT + tid, top, chain);
+                list.push(s.vm[i] >= B, s.r[i], i * NT + tid, top, chain, nl);
                 sum.S += top ? 0.f : cs;
                 sum.W += top ? 0.f : cw;
             }
         }
-    }
-    __syncthreads();
-    const int nl = list.n;
-    const bool slow = !(B > -INFINITY) || nl > SPECIAL;
-    if (!slow) {
+        tok_wave_fence();
         for (; chain >= 0; chain = list.next[chain])
             if (list.at[chain] < 0)
                 for (int e = 0; e < VEC; ++e) sum.add(list.template get<T>(chain, e), ref);
-        if (a.k)
-            for (int i = tid; i < nl * VEC; i += NT) {
-                const int slot = i / VEC, e = i & (VEC - 1);
+        if (tid < ntail) sum.add(s.xt, ref);
+        if (nl > SPECIAL) {
+            if (lane == 0) atomicAdd(&ncand, CAND + 1);
+        } else if (a.k) {
+            // the wave's candidates, one atomic for all that a step finds; their order does not matter
+            const auto put = [&](bool hit, uint64_t key) {
+                const uint64_t mask = __ballot(hit);
+                if (mask == 0) return;
+                int base = 0;
+                if (lane == 0) base = atomicAdd(&ncand, (int)__popcll(mask));
+                const int at = __builtin_amdgcn_readfirstlane(base) + tok_below(mask);
+                if (hit && at < CAND) cand[at] = key;
+            };
+            for (int b = 0; b < nl * VEC; b += 64) {
+                const int i = b + lane, slot = min(i / VEC, nl - 1), e = i & (VEC - 1);
                 const float xv = list.template get<T>(slot, e);
-                if (xv >= B) {
-                    const int at = atomicAdd(&ncand, 1);
-                    if (at < CAND) cand[at] = tok_key(xv, e0 + list.vec(slot) * VEC + e);
-                }
+                put(i < nl * VEC && xv >= B, tok_key(xv, e0 + list.vec(slot) * VEC + e));
             }
-    } else {
+            if (ntail && wave == 0) put(tid < ntail && s.xt >= B, tok_key(s.xt, e0 + nv * VEC + tid));
+        }
+    }
+    float S = tok_group<64, TokSum>(sum.S), W = tok_group<64, TokSum>(sum.W), n = tok_group<64, TokSum>(sum.n);
+    __syncthreads();                                         // red has been read
+    if (lane == 0) {
+        red[wave][0] = S;
+        red[wave][1] = W;
+        red[wave][2] = n;
+    }
+    __syncthreads();                                         // the sums and the candidates are complete
+    const int nc = ncand;
+    const bool slow = !(B > -INFINITY) || nc > CAND;
+    if (slow) {
         // thousands of vectors at the bound (equal values), or fewer than k elements left: element by element, read again
         sum = ScoreSums{0.f, 0.f, 0.f};
         for (int v = tid; v < nv; v += NT) {
@@ -198,21 +211,18 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
 #pragma unroll
             for (int e = 0; e < VEC; ++e) sum.add(TokElem<T>::get(r, e), ref);
         }
-    }
-    if (tid < ntail) {
-        sum.add(s.xt, ref);
-        if (a.k && s.xt >= B && !slow) {
-            const int at = atomicAdd(&ncand, 1);
-            if (at < CAND) cand[at] = tok_key(s.xt, e0 + nv * VEC + tid);
+        if (tid < ntail) sum.add(s.xt, ref);
+        S = tok_group<64, TokSum>(sum.S);
+        W = tok_group<64, TokSum>(sum.W);
+        n = tok_group<64, TokSum>(sum.n);
+        __syncthreads();
+        if (lane == 0) {
+            red[wave][0] = S;
+            red[wave][1] = W;
+            red[wave][2] = n;
         }
+        __syncthreads();
     }
-    float S = tok_group<64, TokSum>(sum.S), W = tok_group<64, TokSum>(sum.W), n = tok_group<64, TokSum>(sum.n);
-    if (lane == 0) {                                     // red was read before the barrier above
-        red[wave][0] = S;
-        red[wave][1] = W;
-        red[wave][2] = n;
-    }
-    __syncthreads();                                     // the sums and the candidates are complete
     S = red[0][0];
     W = red[0][1];
     n = red[0][2];
@@ -232,10 +242,11 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
     else if (tid == 0)
         a.part[u] = make_float4(m, n, S, W);
     if (a.k) {
-        // a row (or segment) with a NaN or +inf logit has no ranking
-        const int nc = S == S ? (slow ? CAND + 1 : ncand) : 0;
-        int done = nc < a.k ? nc : a.k;
-        if (nc <= CAND) {
+        int done = 0;
+        if (!(S == S)) {
+            // a row (or segment) with a NaN or +inf logit has no ranking
+        } else if (!slow) {
+            done = nc < a.k ? nc : a.k;
             tok_rank<NT>(cand, nc, a.k, [&](int rank, uint64_t key) {
                 if (a.nseg == 1) {
                     a.ids[row * a.k + rank] = tok_key_index(key);
@@ -293,24 +304,29 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
 
 // Joins the segments of a row.  The sums are rescaled to the row's maximum, a segment a lane, and added by a fixed tree.  Of
 // the sorted lists of keys: with j = ceil(k / lists), the smallest of the j-th keys has at least k keys at or above it, and so
-// has the largest of the k-th keys; what lies below both is dropped, the rest (about 1.5 k) ranked by counting.
-// NT = 64 without alternatives: one wave a row.
+// has the largest of the k-th keys; what lies below both is dropped, the rest (about 1.5 k) ranked by counting.  One wave for
+// up to 512 keys a row (2,000 rows of 4 lists of 32: 9.4 us, with four waves and their barriers 12.4), four for more.
+constexpr int JOIN_CAND = 1024;
 template <int NT> __global__ __launch_bounds__(NT) void tok_score_join_kernel(ScoreArgs a, int dtype) {
-    extern __shared__ uint64_t lists[];
+    __shared__ __attribute__((aligned(16))) uint64_t cand[JOIN_CAND];
+    __shared__ uint64_t best[NT / 64];
     __shared__ int ncand;
     const int tid = threadIdx.x, lane = tid & 63;
     const int64_t row = a.r.u0 + blockIdx.x;
-    // every load that the row needs is under way before the first is waited for
-    float4 p = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-    if (lane < a.nseg) p = a.part[row * a.nseg + lane];
-    int64_t tgt = 0;
-    if (a.y) tgt = score_target(a, row);
     const int nk = a.nseg * a.k;
     const uint64_t* keys = a.keys + row * nk;
-    if (a.k) {
-        if (tid == 0) ncand = 0;
-        for (int i = tid; i < nk; i += NT) lists[i] = keys[i];
+    // every load that the row needs is under way before the first is waited for
+    float4 p = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    uint64_t first = 0, kth = 0;
+    if (lane < a.nseg) {
+        p = a.part[row * a.nseg + lane];
+        if (a.k) {
+            first = keys[lane * a.k];
+            kth = keys[lane * a.k + a.k - 1];
+        }
     }
+    int64_t tgt = 0;
+    if (a.y) tgt = score_target(a, row);
     if (a.y && tgt == a.ignore) {
         score_skip(a, row, tid, NT);
         return;
@@ -320,6 +336,7 @@ template <int NT> __global__ __launch_bounds__(NT) void tok_score_join_kernel(Sc
     if (a.y && valid_t)
         xt = dtype == 0 ? tok_row<float>(a.r, row)[tgt]
              : dtype == 1 ? bf2f(tok_row<bf16_t>(a.r, row)[tgt]) : (float)tok_row<f16_t>(a.r, row)[tgt];
+    if (tid == 0) ncand = 0;
     const float m = tok_group<64, TokMax>(p.x);
     float n = 0.f, S = p.z, W = 0.f;                         // a segment of nothing but -inf: 0, or NaN
     if (p.x == m) {
@@ -334,38 +351,59 @@ template <int NT> __global__ __launch_bounds__(NT) void tok_score_join_kernel(Sc
     S = tok_group<64, TokSum>(S);
     W = tok_group<64, TokSum>(W);
     const float lnS = score_finish(a, row, m, n, S, W, xt, valid_t, tid == 0);
-    if constexpr (NT > 64) {
-        __syncthreads();
+    if (a.k == 0) return;
+    int done = 0;
+    if (S == S) {                                            // a row with a NaN or +inf logit has no ranking
         // each wave works the bound out for itself
-        const uint64_t first = lane < a.nseg ? lists[lane * a.k] : 0;
         const int live = (int)__popcll(__ballot(first != 0));
         const int j = live ? (a.k + live - 1) / live : 1;
-        const uint64_t jth = first ? lists[lane * a.k + j - 1] : ~0ull, kth = lane < a.nseg ? lists[lane * a.k + a.k - 1] : 0;
-        uint64_t B = tok_group<64, TokMin>(jth);
-        const uint64_t Bk = tok_group<64, TokTop>(kth);
-        if (Bk > B) B = Bk;
+        uint64_t B = tok_group<64, TokMin>(first ? keys[lane * a.k + j - 1] : ~(uint64_t)0);
+        kth = tok_group<64, TokTop>(kth);
+        if (kth > B) B = kth;
         if (B == 0) B = 1;                                   // key 0: no element
-        // candidates move to the front of the lists' memory: read, then written
-        uint64_t mine[(TOK_MAX_SEG * TOK_MAX_K + NT - 1) / NT];
-#pragma unroll
-        for (int q = 0; q < (TOK_MAX_SEG * TOK_MAX_K + NT - 1) / NT; ++q) {
-            const int i = q * NT + tid;
-            mine[q] = i < nk ? lists[i] : 0;
+        __syncthreads();
+        for (int i0 = 0; i0 < nk; i0 += NT) {
+            const uint64_t key = i0 + tid < nk ? keys[i0 + tid] : 0;
+            const uint64_t mask = __ballot(key >= B);
+            if (mask) {
+                int base = 0;
+                if (lane == 0) base = atomicAdd(&ncand, (int)__popcll(mask));
+                const int at = __builtin_amdgcn_readfirstlane(base) + tok_below(mask);
+                if (key >= B && at < JOIN_CAND) cand[at] = key;
+            }
         }
         __syncthreads();
-#pragma unroll
-        for (int q = 0; q < (TOK_MAX_SEG * TOK_MAX_K + NT - 1) / NT; ++q)
-            if (mine[q] >= B) lists[atomicAdd(&ncand, 1)] = mine[q];
-        __syncthreads();
-        const int nc = S == S ? ncand : 0;                   // a row with a NaN or +inf logit has no ranking
-        tok_rank<NT>(lists, nc, a.k, [&](int rank, uint64_t key) {
+        const int nc = ncand;
+        const auto put = [&](int rank, uint64_t key) {
             a.ids[row * a.k + rank] = tok_key_index(key);
             a.top[row * a.k + rank] = score_toplp(a, tok_key_value(key), m, lnS);
-        });
-        for (int r = nc + tid; r < a.k; r += NT) {           // fewer than k elements
-            a.ids[row * a.k + r] = -1;
-            a.top[row * a.k + r] = NAN;
+        };
+        if (nc <= JOIN_CAND) {
+            done = nc < a.k ? nc : a.k;
+            tok_rank<NT>(cand, nc, a.k, put);
+        } else {                                             // lists that lie across each other: k rounds of the next largest
+            uint64_t last = ~0ull;
+            for (; done < a.k; ++done) {
+                uint64_t bk = 0;
+                for (int i = tid; i < nk; i += NT) {
+                    const uint64_t key = keys[i];
+                    if (key < last && key > bk) bk = key;
+                }
+                bk = tok_group<64, TokTop>(bk);
+                if (lane == 0) best[tid >> 6] = bk;
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < NT / 64; ++w) bk = best[w] > bk ? best[w] : bk;
+                __syncthreads();
+                if (bk == 0) break;
+                last = bk;
+                if (tid == 0) put(done, bk);
+            }
         }
+    }
+    for (int r = done + tid; r < a.k; r += NT) {             // fewer than k elements
+        a.ids[row * a.k + r] = -1;
+        a.top[row * a.k + r] = NAN;
     }
 }
 
@@ -477,9 +515,9 @@ __global__ __launch_bounds__(256) void tok_score_narrow_kernel(ScoreArgs a) {
 // Many short rows: a row a lane.  The row's eighths keep their maxima in registers; a round takes the lowest one that holds the
 // maximum, reads those 8 elements of the row in LDS, and marks the lowest that holds it as taken (NaN, which no maximum and no
 // comparison sees).  ~65 operations a round; a pass over the row's registers takes ~180.  The alternatives go out through
-// LDS too when they are few (out = 1).
-template <typename T> __global__ __launch_bounds__(64) void tok_score_lane_kernel(ScoreArgs a, int out) {
-    extern __shared__ uint64_t lane_lds[];
+// LDS too.
+template <typename T> __global__ __launch_bounds__(64) void tok_score_lane_kernel(ScoreArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint64_t lane_lds[];
     T* rows = reinterpret_cast<T*>(lane_lds);
     const int V = a.r.V, k = a.k, lane = threadIdx.x;
     const int64_t row0 = (a.r.u0 + blockIdx.x) * 64, row = row0 + lane;
@@ -544,20 +582,13 @@ template <typename T> __global__ __launch_bounds__(64) void tok_score_lane_kerne
                 id = -1;
                 lp = -INFINITY;
             }
-            if (out) {
-                ids[lane * k + j] = id;
-                lps[lane * k + j] = lp;
-            } else if (there) {
-                a.ids[row * k + j] = id;
-                a.top[row * k + j] = lp;
-            }
+            ids[lane * k + j] = id;
+            lps[lane * k + j] = lp;
         }
-        if (out) {
-            tok_wave_fence();
-            for (int i = lane; i < nrow * k; i += 64) {
-                a.ids[row0 * k + i] = ids[i];
-                a.top[row0 * k + i] = lps[i];
-            }
+        tok_wave_fence();
+        for (int i = lane; i < nrow * k; i += 64) {
+            a.ids[row0 * k + i] = ids[i];
+            a.top[row0 * k + i] = lps[i];
         }
     }
 }
@@ -685,10 +716,9 @@ template <typename T> static void score_wide(const ScoreArgs& a, const TokPlan& 
     else tok_launch(tok_score_kernel<T, 256, 16>, units, nt, 0, s, a);
 }
 template <typename T> static void score_narrow(const ScoreArgs& a, hipStream_t s) {
-    if (tok_lane_rows(a.r.V, a.r.rows)) {
-        const int out = a.k && a.k <= 16;                    // 8 KB of LDS at most
-        const size_t lds = (64 * a.r.V * sizeof(T) + 15) / 16 * 16 + (out ? 64 * a.k * 8 : 0);
-        tok_launch(tok_score_lane_kernel<T>, (a.r.rows + 63) / 64, 64, lds, s, a, out);
+    if (tok_lane_rows(a.r.V, sizeof(T), a.r.rows) && a.k <= 8) {        // more alternatives: rounds on 8 lanes cost less
+        const size_t lds = (64 * a.r.V * sizeof(T) + 15) / 16 * 16 + 64 * a.k * 8;
+        tok_launch(tok_score_lane_kernel<T>, (a.r.rows + 63) / 64, 64, lds, s, a);
         return;
     }
     const int G = tok_narrow_lanes(a.r.V);
@@ -752,8 +782,8 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
     else if (dtype == 1) score_wide<bf16_t>(a, p, s);
     else score_wide<f16_t>(a, p, s);
     if (p.nseg > 1) {
-        if (k) tok_launch(tok_score_join_kernel<256>, rows, 256, (size_t)p.nseg * k * 8, s, a, dtype);
-        else tok_launch(tok_score_join_kernel<64>, rows, 64, 0, s, a, dtype);
+        if (p.nseg * k <= 512) tok_launch(tok_score_join_kernel<64>, rows, 64, 0, s, a, dtype);
+        else tok_launch(tok_score_join_kernel<256>, rows, 256, 0, s, a, dtype);
     }
 }
 

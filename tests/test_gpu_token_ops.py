@@ -134,6 +134,21 @@ def test_score_ties_go_to_the_lowest_index(V, kind):
     _check_score(x, torch.tensor([0, V - 1, V // 2]), 1.0, k)
 
 
+@pytest.mark.parametrize("V,k", [(200000, 128), (600000, 100), (600000, 3)])
+def test_score_segments_that_share_or_lack_the_top(V, k):
+    """Long rows in which the alternatives of all segments lie across each other, in which most segments are ruled out, in
+    which one segment holds them all, and in which fewer than k tokens are left."""
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(5, V, generator=g)
+    i = torch.arange(V)
+    x[0] = -(i % 5000).float() / 512            # the same values in every segment, many of them equal
+    x[1, 20000:] = -math.inf
+    x[2, 70000:70200] += 30
+    x[3] = -math.inf
+    x[3, ::V // 40] = torch.randn(len(x[3, ::V // 40]), generator=g)
+    _check_score(x, torch.zeros(5, dtype=torch.int64), 1.0, k, grad=False)
+
+
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("V", [40, 300, 3000, 40000])
 def test_score_rows_that_are_masked_or_not_numbers(V, dtype):
@@ -398,7 +413,7 @@ def test_distill_gradient_against_differences():
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("V", [1, 2, 7, 8, 9, 12, 31, 33, 40, 63, 64])
 def test_many_short_rows(V, dtype):
-    R, tile = 52, 400
+    R, tile = 52, 1600                    # 68,800 rows and more
     x, at, g = _logits(R, V, dtype, V)
     at[1] = IGN
     if V > 6:
@@ -423,7 +438,7 @@ def test_many_short_rows(V, dtype):
 
 @pytest.mark.parametrize("tail", ["drop", "bucket"])
 def test_many_short_rows_with_odd_entries(tail):
-    V, tile = 40, 600
+    V, tile = 40, 2200
     x, _, g = _logits(31, V, "fp32", 11)
     ids = torch.randint(0, V, (31, 12), generator=g)
     t = torch.log_softmax(torch.randn(31, 20, generator=g), -1)[:, :12].contiguous()
