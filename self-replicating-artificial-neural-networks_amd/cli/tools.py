@@ -94,6 +94,9 @@ def training_main(argv=None):
     p.add_argument("--resume", default=None, help="checkpoint to resume from")
     p.add_argument("--device", default=None)
     p.add_argument("--deterministic", action="store_true", help="train the DeterministicGAE variant")
+    p.add_argument("--teacher", default=None, help="checkpoint of a trained RiboAE to learn from instead of the tokens")
+    p.add_argument("--teacher-top-k", type=int, default=8, help="best tokens of the teacher at each position")
+    p.add_argument("--distill-temperature", type=float, default=1.0)
     a = p.parse_args(argv)
     import torch
     from ..genome.tokenizer import Vocabulary
@@ -111,6 +114,11 @@ def training_main(argv=None):
     model = DeterministicGAE(**hp) if a.deterministic else ConcreteGAE(**hp,
                                                                        prior_temperature=params["prior_temperature"])
     train_set, _ = get_dataset(seqs, params["train_test_ratio"])
+    teacher = None
+    if a.teacher:
+        from ..riboae.io import load_checkpoint
+        teacher, _ = load_checkpoint(a.teacher, device)
     train(a.name, model, train_set, vocab, riboae_config["ribosomal_autoencoders_dir"], batch_size=params["batch_size"],
           min_backup_interval=params["min_backup_interval"], max_steps=a.max_steps, device=device,
-          resume_path=a.resume)
+          resume_path=a.resume, teacher=teacher, teacher_top_k=a.teacher_top_k,
+          distill_temperature=a.distill_temperature)

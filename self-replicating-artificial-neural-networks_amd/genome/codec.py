@@ -125,6 +125,17 @@ class RiboAECodec(GeneticCodec):
             outs.append(self.model.decode_tokens(g[i:i + self.batch_size], device=self.device))
         return np.concatenate(outs, 0) if outs else np.zeros((0, self.max_tokens), np.int64)
 
+    def score_sequences(self, genotypes, top_k: int = 0) -> Dict[str, np.ndarray]:
+        """The decoded ``tokens`` of each genotype with their log-probabilities (``logprob``), the ``entropy`` of each
+        position and its ``top_k`` best tokens (``top_ids``, ``top_logprobs``): how sure a phenotype is of each token and
+        which ones lie next to it."""
+        g = np.asarray(genotypes)
+        if g.ndim == 1:
+            g = g[None]
+        parts = [self.model.score_tokens(g[i:i + self.batch_size], device=self.device, top_k=top_k)
+                 for i in range(0, max(len(g), 1), self.batch_size)]
+        return {k: np.concatenate([p[k] for p in parts], 0) for k in parts[0]}
+
     def encode_sequence(self, tokens) -> np.ndarray:
         t = np.asarray(tokens)
         outs = []

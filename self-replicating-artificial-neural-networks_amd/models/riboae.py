@@ -141,8 +141,66 @@ class GeneticAutoencoder(nn.Module):
         logp = self.generative_net(z)                               # (B, L, V) log-probs
         return torch.gather(logp, -1, x.long().unsqueeze(-1)).squeeze(-1).sum(-1)
 
+    def _distill(self, z, teacher):
+        """-sum over the positions of KL(teacher's top tokens || this decoder), (B,): takes the place of log p(x|z) when the
+        decoder learns from another autoencoder.  teacher: (ids, log-probabilities, temperature), see
+        :meth:`distill_targets`."""
+        from ..ops.token_ops import topk_distill_loss
+        ids, logp, temperature = teacher
+        return -topk_distill_loss(self.generative_net.logits(z), ids, logp, temperature=temperature).sum(-1)
+
     def encode(self, x):
         return self.inference_net(x).argmax(-1)
+
+    # -- positions one by one: log-probabilities, entropies, next-best tokens ----------------------------
+    def _eval_logits(self, bits):
+        """(n, G) genotype bits -> (n, L, V) logits in eval mode, on the HIP kernels on a GPU (like ``decode_tokens``)."""
+        if bits.is_cuda:
+            from ..ops.riboae_ops import HipRiboDecoder, available
+            if available():
+                if self._hip_decoder is None or self._hip_decoder.stale(self):
+                    self._hip_decoder = HipRiboDecoder(self, bits.device)
+                return self._hip_decoder.logits(bits)
+        return self.generative_net.logits(F.one_hot(bits.long(), self.alphabet).float())
+
+    @torch.no_grad()
+    def score_tokens(self, genotypes: np.ndarray, tokens: Optional[np.ndarray] = None, device="cpu", top_k: int = 0,
+                     temperature: float = 1.0) -> Dict[str, np.ndarray]:
+        """How this decoder rates every position of the phenotypes of ``genotypes`` (n, G): ``tokens`` (the given ones, by
+        default the decoded sequence), their ``logprob``, the position's ``entropy`` and, with ``top_k``, its best tokens
+        ``top_ids`` and their ``top_logprobs`` (``ops.token_ops.token_logprobs``)."""
+        from ..ops.token_ops import token_logprobs
+        if len(genotypes) == 0:
+            shape = (0, self.max_len)
+            out = {"tokens": np.zeros(shape, np.int64), "logprob": np.zeros(shape, np.float32),
+                   "entropy": np.zeros(shape, np.float32)}
+            if top_k:
+                out.update(top_ids=np.zeros(shape + (top_k,), np.int64), top_logprobs=np.zeros(shape + (top_k,), np.float32))
+            return out
+        if tokens is None:
+            tokens = self.decode_tokens(genotypes, device=device)
+        self.eval()
+        g = torch.as_tensor((np.asarray(genotypes) > 0.5).astype(np.int64), device=device)
+        t = torch.as_tensor(np.asarray(tokens), device=device).long()
+        r = token_logprobs(self._eval_logits(g), t, temperature=temperature, top_k=top_k)
+        out = {"tokens": t, "logprob": r.logprob, "entropy": r.entropy}
+        if top_k:
+            out.update(top_ids=r.top_ids, top_logprobs=r.top_logprobs)
+        return {k: v.cpu().numpy() for k, v in out.items()}
+
+    @torch.no_grad()
+    def distill_targets(self, x, top_k: int, temperature: float = 1.0):
+        """What this autoencoder teaches about the token batch ``x`` (B, L): (ids, log-probabilities, temperature) of its
+        ``top_k`` best tokens at each position of its own reconstruction, in eval mode, for ``compute_loss(teacher=...)``."""
+        from ..ops.token_ops import token_logprobs
+        self.eval()
+        if x.is_cuda:
+            from ..ops.riboae_ops import HipRiboEncoder, available
+            if available() and (self._hip_encoder is None or self._hip_encoder.stale(self)):
+                self._hip_encoder = HipRiboEncoder(self, x.device)
+        bits = self._hip_encoder(x) if x.is_cuda and self._hip_encoder is not None else self.encode(x)
+        r = token_logprobs(self._eval_logits(bits), temperature=temperature, top_k=top_k)
+        return r.top_ids, r.top_logprobs, float(temperature)
 
     # -- numpy inference API used by the codec ----------------------------------------------------
     @torch.no_grad()
@@ -193,20 +251,24 @@ class ConcreteGAE(GeneticAutoencoder):
         logp = gumbel_log_prob(sample, ploc, 1.0 / self.prior_temperature)
         return torch.softmax(sample, -1), logq, logp
 
-    def compute_loss(self, x, temperature, kld_weight, noise=None) -> Dict[str, torch.Tensor]:
+    def compute_loss(self, x, temperature, kld_weight, noise=None, teacher=None) -> Dict[str, torch.Tensor]:
         """NELBO (model.py:88-100).  ``noise``: optional uniforms of the logits' shape (B, G, A) replacing
-        the random draw, so two runs (or the HIP and the torch path) see the same sample."""
+        the random draw, so two runs (or the HIP and the torch path) see the same sample.  ``teacher``: another
+        autoencoder's :meth:`distill_targets` of ``x``; its divergence then takes the place of the reconstruction
+        term in the loss (``nll`` stays the reconstruction's)."""
         if x.is_cuda and os.environ.get("SERANN_RIBOAE_HIP", "1") != "0":
             from ..ops.riboae_ops import available, concrete_sample
             if available():                                        # K36 fused sample + softmax + KL
                 z, kl = concrete_sample(self.inference_net(x), temperature, self.prior_temperature, noise)
                 logpx_z = self._decode(x, z)
-                nelbo = -(logpx_z - kld_weight * kl).mean()
+                fit = logpx_z if teacher is None else self._distill(z, teacher)
+                nelbo = -(fit - kld_weight * kl).mean()
                 return {"loss": nelbo, "nll": -logpx_z.mean(), "kld": kl.mean()}
         z, logq, logp = self._encode(x, temperature, noise)
         logpx_z = self._decode(x, z)
         kl = (logq - logp).flatten(1).sum(1)
-        nelbo = -(logpx_z - kld_weight * kl).mean()
+        fit = logpx_z if teacher is None else self._distill(z, teacher)
+        nelbo = -(fit - kld_weight * kl).mean()
         return {"loss": nelbo, "nll": -logpx_z.mean(), "kld": kl.mean()}
 
 
@@ -214,10 +276,10 @@ class DeterministicGAE(GeneticAutoencoder):
     def _encode(self, x):
         return torch.softmax(self.inference_net(x), -1)
 
-    def compute_loss(self, x, *args, **kw):
+    def compute_loss(self, x, *args, teacher=None, **kw):
         z = self._encode(x)
         nll = -self._decode(x, z).mean()
-        return {"loss": nll, "nll": nll, "kld": torch.zeros((), device=nll.device)}
+        return {"loss": nll if teacher is None else -self._distill(z, teacher).mean(), "nll": nll, "kld": torch.zeros((), device=nll.device)}
 
 
 def build_model(kind: str = "concrete", **hp) -> GeneticAutoencoder:

@@ -93,8 +93,7 @@ class HipRiboDecoder:
         self._plans[B] = pl
         return pl
 
-    @torch.no_grad()
-    def __call__(self, bits: torch.Tensor) -> torch.Tensor:
+    def _forward(self, bits: torch.Tensor) -> dict:
         B = bits.shape[0]
         pl = self._plan(B)
         lib, s = H.lib(), H.stream_handle()
@@ -103,6 +102,19 @@ class HipRiboDecoder:
             torch.nn.functional.one_hot(bits.to(self.device).long(), self.A).to(torch.bfloat16))
         for v, d, t in pl["launches"]:
             lib.gemm3(H.MODE_FWD, v, d.data_ptr(), t.data_ptr(), len(t), s)
+        return pl
+
+    @torch.no_grad()
+    def logits(self, bits: torch.Tensor) -> torch.Tensor:
+        """(n, G) genotype bits -> (n, L, V) fp32 logits of the MFMA decode, a view of the plan's buffer (valid until the
+        next call with n genotypes): what ``token_ops.token_logprobs`` scores positions from."""
+        return self._forward(bits)["logits"].view(bits.shape[0], self.L, self.V)
+
+    @torch.no_grad()
+    def __call__(self, bits: torch.Tensor) -> torch.Tensor:
+        B = bits.shape[0]
+        pl = self._forward(bits)
+        lib, s = H.lib(), H.stream_handle()
         lib.group_argmax(pl["logits"].data_ptr(), pl["out"].data_ptr(), B * self.L, self.V, s)
         out = pl["out"].long().clone()
         self._rescore(bits, pl, out)

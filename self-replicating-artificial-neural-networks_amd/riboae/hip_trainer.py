@@ -31,6 +31,7 @@ import numpy as np
 import torch
 
 from ..ops import hip_ops as H
+from ..ops.token_ops import topk_distill_grad
 
 SLACK = 64
 
@@ -459,8 +460,10 @@ class HipRiboTrainer:
 
     def step(self, tokens: torch.Tensor, temperature: float, kld_weight: float, lr: float,
              prior_temperature: Optional[float] = None, noise: Optional[torch.Tensor] = None,
-             seed: Optional[int] = None, update: bool = True) -> Dict[str, torch.Tensor]:
-        """One NELBO training step on a [B][L] token batch; returns device scalars (loss, nll, kld).
+             seed: Optional[int] = None, update: bool = True, teacher=None) -> Dict[str, torch.Tensor]:
+        """One NELBO training step on a [B][L] token batch; returns device scalars (loss, nll, kld).  ``teacher``: another
+        autoencoder's ``distill_targets`` of the batch, whose divergence takes the place of the reconstruction term
+        (loss and gradient in one pass over the decoder's output, ``ops.token_ops.topk_distill_grad``).
         ``update=False`` leaves the Q40 gradient arena filled and skips Adam (numerics tests)."""
         B = int(tokens.shape[0])
         L, E, G, A, V = self.L, self.E, self.G, self.A, self.V
@@ -492,12 +495,20 @@ class HipRiboTrainer:
         self._run(pl.fwd_dec)
         lib.cat_loglik_fwd(buf["yh2"].data_ptr(), buf["tok"].data_ptr(), buf["logpx"].data_ptr(), B, L, V, s, 1)
         logpx, kl = buf["logpx"][:B], buf["kl"][:B]
-        nelbo = -(logpx - kld_weight * kl).mean()
         # backward: d nelbo / d logpx = -1/B, d / d kl = w/B
-        buf["gout"][:B].fill_(-1.0 / B)
         buf["gkl"][:B].fill_(float(kld_weight) / B)
-        lib.cat_loglik_bwd(buf["yh2"].data_ptr(), buf["tok"].data_ptr(), buf["gout"].data_ptr(),
-                           buf["dh2"].data_ptr(), B, L, V, s, 1)
+        if teacher is None:
+            nelbo = -(logpx - kld_weight * kl).mean()
+            buf["gout"][:B].fill_(-1.0 / B)
+            lib.cat_loglik_bwd(buf["yh2"].data_ptr(), buf["tok"].data_ptr(), buf["gout"].data_ptr(),
+                               buf["dh2"].data_ptr(), B, L, V, s, 1)
+        else:
+            ids, logp, distill_t = teacher
+            weight = torch.full((B, L), 1.0 / B, device=self.dev)
+            out = buf["dh2"][:B * L * V].view(B, L, V)
+            div, _ = topk_distill_grad(buf["yh2"][:B * L * V].view(B, L, V), ids, logp, temperature=distill_t,
+                                       weight=weight, out=out)
+            nelbo = div.sum() + kld_weight * kl.mean()
         self._run(pl.bwd_dec)
         lib.concrete_bwd(buf["s"].data_ptr(), buf["z"].data_ptr(), buf["dzb"].data_ptr(), buf["gkl"].data_ptr(),
                          buf["dlogitsb"].data_ptr(), B, G, A, float(temperature), tp, s, 1)
@@ -560,11 +571,11 @@ class HipRiboTrainer:
                 t = 0
         self.step_i.fill_(t)
 
-    def debug_grads(self, tokens, temperature, kld_weight, noise):
+    def debug_grads(self, tokens, temperature, kld_weight, noise, teacher=None):
         """Gradients of one step without the Adam update (numerics tests): {param name: torch-layout
         array}, plus the step's (loss, nll, kld).  The BatchNorm moving statistics are restored."""
         st0 = self.stats.clone()
-        res = self.step(tokens, temperature, kld_weight, 0.0, noise=noise, update=False)
+        res = self.step(tokens, temperature, kld_weight, 0.0, noise=noise, update=False, teacher=teacher)
         g = H.from_qg(self.g)
         self.g.zero_()
         with torch.no_grad():

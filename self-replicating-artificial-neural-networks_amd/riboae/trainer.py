@@ -27,6 +27,7 @@ import torch
 
 from ..engine.torch_engine import KerasAdam
 from ..models.riboae import ConcreteGAE
+from ..ops.token_ops import MAX_TOP_K
 from .io import save_checkpoint
 
 TEMPERATURE_STEPS = int(5e6)
@@ -88,8 +89,19 @@ def get_dataset(sequences: np.ndarray, train_test_ratio: float):
 def train(experiment_name: str, model, train_tokens: np.ndarray, vocabulary, out_dir: str, batch_size: int = 512,
           min_backup_interval: int = 1000, max_steps: Optional[int] = None, device="cpu", log=print,
           resume_path: Optional[str] = None, bf16: Optional[bool] = None, demo_every: int = 50, log_every: int = 10,
-          engine: str = "auto"):
+          engine: str = "auto", teacher=None, teacher_top_k: int = 8, distill_temperature: float = 1.0):
+    """``teacher``: a trained autoencoder of the same vocabulary and sequence length; the model then learns its
+    ``teacher_top_k`` best tokens at each position (at ``distill_temperature``) instead of the batch's own tokens."""
     dev = torch.device(device)
+    if teacher is not None:
+        if (teacher.vocab, teacher.max_len) != (model.vocab, model.max_len):
+            raise ValueError(f"the teacher has {teacher.vocab} tokens x {teacher.max_len} positions, the model "
+                             f"{model.vocab} x {model.max_len}")
+        if not 1 <= teacher_top_k <= min(model.vocab, MAX_TOP_K):
+            raise ValueError(f"teacher_top_k must be in [1, {min(model.vocab, MAX_TOP_K)}], got {teacher_top_k}")
+        if teacher is model:
+            raise ValueError("a model cannot be its own teacher")
+        teacher.to(dev).eval()
     model.to(dev).train()
     is_concrete = isinstance(model, ConcreteGAE)
     if engine == "auto":
@@ -163,6 +175,7 @@ def train(experiment_name: str, model, train_tokens: np.ndarray, vocabulary, out
         if x.device != dev:
             x = x.to(dev, non_blocking=True)
         temperature, lr, kw = temperature_at(b), learning_rate_at(b), kld_weight_at(b)
+        taught = None if teacher is None else teacher.distill_targets(x, teacher_top_k, distill_temperature)
         if hip is not None:
             # a backup of step b - 1 must see step b - 1's weights: when b - 1 may be backed up (its distance to
             # the last backup allows it), its loss is settled before step b is enqueued
@@ -171,13 +184,14 @@ def train(experiment_name: str, model, train_tokens: np.ndarray, vocabulary, out
                 if loss < min_loss:
                     backup(pending[0], loss)
                 pending = None
-            metrics = hip.step(x, temperature, kw, lr)
+            metrics = hip.step(x, temperature, kw, lr, teacher=taught)
             if pending is not None:
                 settle(*pending)        # (b - 1 could not be backed up: reading its loss now costs nothing)
             pending = (b, metrics)
         else:
             with torch.autocast(device_type=dev.type, dtype=torch.bfloat16, enabled=bool(bf16)):
-                metrics = model.compute_loss(x, temperature, kw) if is_concrete else model.compute_loss(x)
+                metrics = (model.compute_loss(x, temperature, kw, teacher=taught) if is_concrete
+                           else model.compute_loss(x, teacher=taught))
             opt.zero_grad()
             metrics["loss"].float().backward()
             opt.step(lr)

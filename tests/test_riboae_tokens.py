@@ -1,0 +1,202 @@
+"""The ribosomal autoencoder's uses of the token operators: scores of decoded positions (model, codec) and learning from
+another autoencoder's best tokens (loss, trainer, command line)."""
+import copy
+import json
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from serann.genome.codec import RiboAECodec
+from serann.genome.tokenizer import Vocabulary
+from serann.models.riboae import ConcreteGAE, build_model
+from serann.riboae import trainer as T
+from serann.riboae.io import save_checkpoint
+
+from . import token_oracle as O
+
+
+def _model(seed=0, kind="concrete", V=12):
+    torch.manual_seed(seed)
+    m = build_model(kind, genotype_length=20, max_phenotype_length=32, vocabulary_size=V, embedding_dim=16)
+    with torch.no_grad():
+        for b in m.modules():
+            if isinstance(b, torch.nn.BatchNorm1d):
+                b.running_mean.normal_(0, 0.1)
+                b.running_var.uniform_(0.5, 1.5)
+    return m.eval()
+
+
+def _bits(n, seed=3):
+    return np.random.default_rng(seed).integers(0, 2, (n, 20))
+
+
+def test_score_tokens_rates_every_position():
+    m = _model()
+    bits = _bits(5)
+    r = m.score_tokens(bits, top_k=4, temperature=1.5)
+    np.testing.assert_array_equal(r["tokens"], m.decode_tokens(bits))
+    with torch.no_grad():
+        z = torch.nn.functional.one_hot(torch.as_tensor(bits), 2).float()
+        x = m.generative_net.logits(z).reshape(-1, 12)
+    ref = O.score(x, torch.as_tensor(r["tokens"]).reshape(-1), 1.5, 4, -100)
+    assert r["logprob"].shape == r["entropy"].shape == (5, 32) and r["top_ids"].shape == (5, 32, 4)
+    np.testing.assert_array_equal(r["top_ids"].reshape(-1, 4), ref["top_ids"].numpy())
+    tol = 64 * O.U * 20
+    np.testing.assert_allclose(r["logprob"].reshape(-1), ref["logprob"].numpy(), rtol=tol, atol=tol)
+    np.testing.assert_allclose(r["entropy"].reshape(-1), ref["entropy"].numpy(), rtol=tol, atol=tol)
+    np.testing.assert_array_equal(r["top_ids"][..., 0], r["tokens"])
+    given = np.zeros((5, 32), np.int64)
+    assert "top_ids" not in m.score_tokens(bits, given)
+    np.testing.assert_array_equal(m.score_tokens(bits, given)["tokens"], given)
+
+
+def test_codec_scores_in_batches():
+    m = _model()
+    vocab = Vocabulary.build([[f"t{i}" for i in range(11)]])
+    c = RiboAECodec(m, vocab, max_tokens=32, batch_size=4)
+    bits = _bits(11)
+    r = c.score_sequences(bits, top_k=3)
+    np.testing.assert_array_equal(r["tokens"], c.decode_to_sequence(bits))
+    want = m.score_tokens(bits, top_k=3)
+    for k in want:
+        np.testing.assert_array_equal(r[k], want[k])
+    assert c.score_sequences(bits[0])["logprob"].shape == (1, 32)
+    assert c.score_sequences(bits[:0], top_k=2)["top_ids"].shape == (0, 32, 2)
+
+
+@pytest.mark.parametrize("kind", ["concrete", "deterministic"])
+def test_loss_against_a_teacher(kind):
+    """The reconstruction term becomes the divergence from the teacher's tokens; the gradient is the formula's."""
+    teacher, m = _model(1), _model(2, kind).train()
+    x = torch.randint(0, 12, (6, 32), generator=torch.Generator().manual_seed(5))
+    u = torch.rand(6, 20, 2, generator=torch.Generator().manual_seed(6))
+    taught = teacher.distill_targets(x, 5, 2.0)
+    assert taught[0].shape == taught[1].shape == (6, 32, 5) and taught[2] == 2.0
+    kw = dict(noise=u) if kind == "concrete" else {}
+    plain = m.compute_loss(x, 0.3, 0.05, **kw)
+    out = m.compute_loss(x, 0.3, 0.05, teacher=taught, **kw)
+    assert torch.equal(out["nll"], plain["nll"]) and torch.equal(out["kld"], plain["kld"])
+    z = m._encode(x, 0.3, u)[0] if kind == "concrete" else m._encode(x)
+    logits = m.generative_net.logits(z).reshape(-1, 12)
+    div, dx = O.distill(logits.detach(), taught[0].reshape(-1, 5), taught[1].reshape(-1, 5), 2.0, "drop", None)
+    want = float(div.sum().detach()) / 6 + 0.05 * float(out["kld"].detach())
+    # fp32 sums of 32 positions and 6 rows, and the division: 40 roundings of the terms' size
+    assert abs(float(out["loss"].detach()) - want) <= 40 * O.U * (float(div.abs().sum()) / 6 + abs(0.05 * float(out["kld"].detach())))
+    got, = torch.autograd.grad(out["loss"], m.generative_net.bn2.bias)
+    total = dx.sum(0) / 6
+    assert torch.allclose(got.double(), total, rtol=0, atol=200 * O.U * float(dx.abs().sum()) / 6)
+
+
+def test_trainer_learns_from_a_teacher(tmp_path):
+    teacher, m = _model(1), _model(2)
+    before = copy.deepcopy(teacher.state_dict())
+    data = np.random.default_rng(0).integers(0, 12, (48, 32))
+    hist = T.train("kd", m, data, None, str(tmp_path), batch_size=16, max_steps=4, log=lambda *a: None, teacher=teacher,
+                   teacher_top_k=3, distill_temperature=2.0)
+    assert len(hist) == 4 and np.isfinite(hist).all()
+    assert all(torch.equal(a, b) for a, b in zip(before.values(), teacher.state_dict().values()))
+    for kw in (dict(teacher=_model(1, V=13)), dict(teacher=m), dict(teacher=teacher, teacher_top_k=0),
+               dict(teacher=teacher, teacher_top_k=13)):
+        with pytest.raises(ValueError):
+            T.train("kd", m, data, None, str(tmp_path), batch_size=16, max_steps=1, log=lambda *a: None, **kw)
+
+
+def test_training_command_with_a_teacher(tmp_path, monkeypatch):
+    from serann.cli import tools
+    monkeypatch.setitem(tools.riboae_config, "ribosomal_autoencoders_dir", str(tmp_path))
+    save_checkpoint(tmp_path / "t.pt", _model(1), "concrete", 1)
+    vocab = Vocabulary.build([[f"t{i}" for i in range(11)]])
+    assert len(vocab) == 12
+    vocab.save_csv(tmp_path / "v.csv")
+    np.savez(tmp_path / "d.npz", sequences=np.random.default_rng(0).integers(0, 12, (20, 32)))
+    params = {"batch_size": 8, "embedding_size": 16, "genotype_alphabet_size": 2, "genotype_size": 20,
+              "min_backup_interval": 1000, "prior_temperature": 0.1, "source_code_length": 32, "train_test_ratio": 0.9}
+    (tmp_path / "p.json").write_text(json.dumps(params))
+    tools.training_main(["-p", str(tmp_path / "p.json"), "-n", "s", "--dataset", str(tmp_path / "d.npz"), "--vocabulary",
+                         str(tmp_path / "v.csv"), "--max-steps", "2", "--device", "cpu", "--teacher", str(tmp_path / "t.pt"),
+                         "--teacher-top-k", "4", "--distill-temperature", "1.5"])
+    assert os.path.exists(tmp_path / "s_b2.pt")
+
+
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_gpu_scores_follow_the_decoder():
+    """On a GPU the positions are scored from the HIP decoder's logits.  A log-softmax moves by at most twice the largest
+    change of its logits, so the scores agree with the CPU's within twice the logits' difference (and the fp32 bound)."""
+    m = _model()
+    bits = _bits(70)
+    want = m.score_tokens(bits, top_k=3)
+    with torch.no_grad():
+        x = m.generative_net.logits(torch.nn.functional.one_hot(torch.as_tensor(bits), 2).float())
+    g = copy.deepcopy(m).cuda()
+    got = g.score_tokens(bits, want["tokens"], device="cuda", top_k=3)
+    xg = g._eval_logits(torch.as_tensor(bits).cuda()).cpu()
+    off = float((xg - x).abs().max())
+    assert off < 0.1 * float(x.abs().max())
+    assert np.abs(got["logprob"] - want["logprob"]).max() <= 2 * off + 1e-4
+    ref = O.score(xg.reshape(-1, 12), torch.as_tensor(want["tokens"]).reshape(-1), 1.0, 3, -100)
+    np.testing.assert_array_equal(got["top_ids"].reshape(-1, 3), ref["top_ids"].numpy())
+    tol = O.sum_error(xg.reshape(-1, 12), 1.0) + 6 * O.U * 40
+    np.testing.assert_allclose(got["logprob"].reshape(-1), ref["logprob"].numpy(), rtol=0, atol=tol)
+
+
+@pytest.mark.gpu
+def test_gpu_teacher_targets_match_the_cpu_where_the_codes_agree():
+    m = _model(1)
+    x = torch.randint(0, 12, (40, 32), generator=torch.Generator().manual_seed(2))
+    g = copy.deepcopy(m).cuda()
+    ids, lp, t = g.distill_targets(x.cuda(), 4, 1.5)
+    bits_c, bits_g = m.encode(x), g._hip_encoder(x.cuda()).cpu()
+    xg = g._eval_logits(bits_g.cuda()).reshape(-1, 12).cpu()
+    ref = O.score(xg, None, 1.5, 4, -100)
+    assert torch.equal(ids.reshape(-1, 4).cpu(), ref["top_ids"]) and t == 1.5
+    assert float((bits_c == bits_g).float().mean()) > 0.9
+
+
+@pytest.mark.gpu
+def test_hip_step_against_a_teacher_matches_the_fp32_oracle(monkeypatch):
+    """Every parameter gradient of a HIP step that learns from a teacher against the fp32 CPU model, with the bounds of the
+    step that learns from tokens (5 %, cosine > 0.998, an absolute floor of 0.2 % of the largest element)."""
+    from serann.riboae.hip_trainer import HipRiboTrainer
+
+    from .test_riboae_hip_train import SPEC_OF, _err
+    torch.manual_seed(0)
+    m = ConcreteGAE(genotype_length=20, max_phenotype_length=32, vocabulary_size=12, embedding_dim=16, prior_temperature=0.1)
+    g = torch.Generator().manual_seed(1)
+    x, u = torch.randint(0, 12, (48, 32), generator=g), torch.rand(48, 20, 2, generator=g)
+    taught = _model(1).distill_targets(x, 5, 2.0)
+    monkeypatch.setenv("SERANN_RIBOAE_HIP", "0")
+    c = copy.deepcopy(m).train()
+    out = c.compute_loss(x, 0.3, 0.05, noise=u, teacher=taught)
+    gr = torch.autograd.grad(out["loss"], list(c.parameters()))
+    ref = {n: t.numpy().astype(np.float64) for (n, _), t in zip(c.named_parameters(), gr)}
+    monkeypatch.delenv("SERANN_RIBOAE_HIP")
+    tr = HipRiboTrainer(m.cuda().train(), device="cuda")
+    dev = (taught[0].cuda(), taught[1].cuda(), taught[2])
+    hip, res = tr.debug_grads(x.cuda(), 0.3, 0.05, u.cuda(), teacher=dev)
+    again, res2 = tr.debug_grads(x.cuda(), 0.3, 0.05, u.cuda(), teacher=dev)
+    assert res == res2 and all(np.array_equal(hip[k], again[k]) for k in hip)
+    loss, kld = float(out["loss"].detach()), float(out["kld"].detach())
+    assert abs(res["loss"] - loss) < 1e-2 * abs(loss) and abs(res["kld"] - kld) < 1e-2 * abs(kld) + 1e-3
+    gmax = max(float(np.abs(v).max()) for v in ref.values())
+    for k, tname in SPEC_OF.items():
+        want, got = ref[tname], hip[k]
+        if np.linalg.norm(want) < 1e-4 * gmax * np.sqrt(want.size):
+            assert np.abs(got).max() < 1e-2 * gmax, k
+            continue
+        if np.linalg.norm(got - want) < 2e-3 * gmax * np.sqrt(want.size):
+            continue
+        e, cos = _err(got, want)
+        assert e < 0.05 and cos > 0.998, (k, e, cos)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("engine", ["hip", "torch"])
+def test_gpu_trainer_learns_from_a_teacher(tmp_path, engine):
+    data = np.random.default_rng(0).integers(0, 12, (96, 32))
+    torch.manual_seed(7)
+    hist = T.train("kd", _model(2), data, None, str(tmp_path), batch_size=32, max_steps=6, device="cuda", log=lambda *a: None,
+                   demo_every=0, engine=engine, teacher=_model(1), teacher_top_k=4)
+    assert len(hist) == 6 and np.isfinite(hist).all()
