@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import functools
 import math
+import operator
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -197,25 +198,28 @@ def _score_hip(logits, targets, temperature, top_k, ignore_index, want_stat):
         ids = x.new_empty(lead + (top_k,), dtype=torch.int64)
         top = x.new_empty(lead + (top_k,), dtype=torch.float32)
         idp, topp = ids.data_ptr(), top.data_ptr()
-    layout = (code, rows, n1, s0, s1, V, temperature, yp, y64, t0, t1, ignore_index)
     if want_stat:
         stat = x.new_empty((rows, 3), dtype=torch.float32)
         stp = stat.data_ptr()
-        saved = (x, y, stat, layout)
+        saved = (x, y, stat)
     nseg = _score_segments(V, code, rows)
     if nseg > 1:
         ws = x.new_empty(rows * nseg * (2 + top_k), dtype=torch.int64)
         wsp = ws.data_ptr()
-    H.lib().tok_score(x.data_ptr(), *layout, top_k, lpp, ent.data_ptr(), idp, topp, stp, wsp,
-                      _raw_stream(logits.device.index))
+    H.lib().tok_score(x.data_ptr(), code, rows, n1, s0, s1, V, temperature, yp, y64, t0, t1, ignore_index, top_k, lpp,
+                      ent.data_ptr(), idp, topp, stp, wsp, _raw_stream(logits.device.index))
     return lp, ent, ids, top, saved
 
 
 @_on_device
-def _score_grad_hip(x, layout, stat, glp, gent, shape):
+def _score_grad_hip(x, y, stat, temperature, ignore_index, glp, gent, shape):
+    # the layout again: saved tensors may come back elsewhere and with other strides (saved-tensor hooks)
+    x, rows, n1, s0, s1 = _rows(x)
+    y, t0, t1 = _same_rows(y, n1, rows) if y is not None else (None, 0, 0)
     dx = x.new_empty(shape)
-    H.lib().tok_score_grad(x.data_ptr(), *layout, H.ptr(glp), H.ptr(gent), stat.data_ptr(), dx.data_ptr(),
-                           _raw_stream(x.device.index))
+    H.lib().tok_score_grad(x.data_ptr(), _DTYPES[x.dtype], rows, n1, s0, s1, x.shape[-1], temperature, H.ptr(y),
+                           y is not None and y.dtype == torch.int64, t0, t1, ignore_index, H.ptr(glp), H.ptr(gent),
+                           stat.contiguous().data_ptr(), dx.data_ptr(), _raw_stream(x.device.index))
     return dx
 
 
@@ -226,8 +230,9 @@ def _f32(g):
 class _Score(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, temperature, top_k, ignore_index, extra):
-        lp, ent, ids, top, (x, y, stat, ctx.layout) = _score_hip(logits, targets, temperature, top_k, ignore_index, True)
-        ctx.save_for_backward(x, y, stat)
+        lp, ent, ids, top, saved = _score_hip(logits, targets, temperature, top_k, ignore_index, True)
+        ctx.save_for_backward(*saved)
+        ctx.args = (temperature, ignore_index)
         ctx.shape = logits.shape
         ctx.set_materialize_grads(False)
         extra += (ids, top)                     # no gradients: kept out of the graph
@@ -238,8 +243,9 @@ class _Score(torch.autograd.Function):
     def backward(ctx, gent, glp=None):
         if glp is None and gent is None:
             return None, None, None, None, None, None
-        x, _, stat = ctx.saved_tensors
-        return _score_grad_hip(x, ctx.layout, stat, _f32(glp), _f32(gent), ctx.shape), None, None, None, None, None
+        x, y, stat = ctx.saved_tensors
+        dx = _score_grad_hip(x, y, stat, *ctx.args, _f32(glp), _f32(gent), ctx.shape)
+        return dx, None, None, None, None, None
 
 
 def _log_softmax(logits, temperature):
@@ -290,6 +296,9 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     temperature = _check_logits(logits, temperature)
     if targets is not None:
         _check_ints(targets, "targets", logits.shape[:-1], logits.device)
+    top_k, ignore_index = operator.index(top_k), operator.index(ignore_index)
+    if not -1 << 63 <= ignore_index < 1 << 63:
+        raise ValueError("ignore_index must fit 64 bits")
     if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]):
         raise ValueError(f"top_k must be in [0, min({MAX_TOP_K}, V = {logits.shape[-1]})], got {top_k}")
     if not logits.is_cuda:
@@ -323,17 +332,21 @@ def _distill_hip(logits, ids, logprobs, temperature, bucket, weight, dx, save):
     if nseg > 1:
         ws = x.new_empty((rows * nseg, 4), dtype=torch.float32)
         wsp = ws.data_ptr()
-    layout = (code, rows, n1, s0, s1, V, temperature, ids.data_ptr(), ids.dtype == torch.int64)
-    wp = 0 if weight is None else weight.data_ptr()
-    H.lib().tok_distill(x.data_ptr(), *layout, logprobs.data_ptr(), wp, K, bucket, loss.data_ptr(),
+    H.lib().tok_distill(x.data_ptr(), code, rows, n1, s0, s1, V, temperature, ids.data_ptr(), ids.dtype == torch.int64,
+                        logprobs.data_ptr(), 0 if weight is None else weight.data_ptr(), K, bucket, loss.data_ptr(),
                         0 if dx is None else dx.data_ptr(), stp, pkp, wsp, _raw_stream(logits.device.index))
-    return loss, (x, stat, pk, layout) if dx is None else dx
+    return loss, (x, stat, pk) if dx is None else dx
 
 
 @_on_device
-def _distill_grad_hip(x, layout, ids, weight, g, stat, pk, shape):
+def _distill_grad_hip(x, ids, weight, stat, pk, g, temperature, shape):
+    # every pointer and stride anew, as in _score_grad_hip
+    x, rows, n1, s0, s1 = _rows(x)
+    ids, stat, pk = ids.contiguous(), stat.contiguous(), pk.contiguous()
+    weight = None if weight is None else weight.contiguous()
     dx = x.new_empty(shape)
-    H.lib().tok_distill_grad(x.data_ptr(), *layout, H.ptr(weight), ids.shape[-1], g.data_ptr(), stat.data_ptr(),
+    H.lib().tok_distill_grad(x.data_ptr(), _DTYPES[x.dtype], rows, n1, s0, s1, x.shape[-1], temperature, ids.data_ptr(),
+                             ids.dtype == torch.int64, H.ptr(weight), ids.shape[-1], g.data_ptr(), stat.data_ptr(),
                              pk.data_ptr(), dx.data_ptr(), _raw_stream(x.device.index))
     return dx
 
@@ -341,16 +354,15 @@ def _distill_grad_hip(x, layout, ids, weight, g, stat, pk, shape):
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, logprobs, temperature, bucket, weight):
-        loss, (x, stat, pk, ctx.layout) = _distill_hip(logits, ids, logprobs, temperature, bucket, weight, None, True)
+        loss, (x, stat, pk) = _distill_hip(logits, ids, logprobs, temperature, bucket, weight, None, True)
         ctx.save_for_backward(x, ids, weight, stat, pk)
-        ctx.shape = logits.shape
+        ctx.args = (temperature, logits.shape)
         return loss
 
     @staticmethod
     @_once
     def backward(ctx, g):
-        x, ids, weight, stat, pk = ctx.saved_tensors
-        return _distill_grad_hip(x, ctx.layout, ids, weight, _f32(g), stat, pk, ctx.shape), None, None, None, None, None
+        return _distill_grad_hip(*ctx.saved_tensors, _f32(g), *ctx.args), None, None, None, None, None
 
 
 def _distill_torch(logits, ids, logprobs, temperature, tail, weight):

@@ -515,6 +515,108 @@ def test_captured_and_replayed(V):
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def _both_backward(x, y, ids, t, w):
+    r = TO.token_logprobs(x, y)
+    a, = torch.autograd.grad([r.logprob, r.entropy], [x], [torch.ones_like(r.logprob), torch.ones_like(r.entropy)])
+    loss = TO.topk_distill_loss(x, ids, t, tail="bucket", weight=w)
+    b, = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    return a, b
+
+
+@pytest.mark.parametrize("V", [40, 3000, 70001])
+def test_saved_tensors_may_come_back_elsewhere(V):
+    """Saved-tensor hooks: what the backward pass reads lies at another address, with other strides, than in the forward."""
+    base, at, g = _logits(12, V + 4, "bf16", 25)
+    base = base.view(3, 4, V + 4)
+    ids, t = _teacher(base.view(12, -1)[:, :V], 5, 1.0, g)
+    ids, t, w = ids.view(3, 4, 5).cuda(), t.view(3, 4, 5).cuda(), torch.rand(3, 4, generator=g).cuda()
+    y = torch.randint(0, V, (3, 5), generator=g).cuda()[:, 1:]
+    leaf = base.cuda().requires_grad_(True)
+    want = _both_backward(leaf[..., 2:V + 2], y, ids, t, w)
+    with torch.autograd.graph.save_on_cpu():
+        got = _both_backward(leaf[..., 2:V + 2], y, ids, t, w)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("V", [40, 9000])
+def test_backward_passes_captured_into_a_graph(V):
+    x, at, g = _logits(8, V, "bf16", 26)
+    ids, t = _teacher(x, 5, 1.0, g)
+    w = torch.rand(8, generator=g).cuda()
+    y, ids, t = at.cuda(), ids.cuda(), t.cuda()
+    static = x.cuda()
+
+    def call():
+        return _both_backward(static.detach().requires_grad_(True), y, ids, t, w)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = call()
+    for src in (x.cuda(), torch.flip(x, [0]).cuda(), x.cuda()):
+        static.copy_(src)
+        want = [v.clone() for v in call()]
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+def test_differentiated_once():
+    x, at, _ = _logits(4, 50, "fp32", 27)
+    xd = x.cuda().requires_grad_(True)
+    r = TO.token_logprobs(xd, at.cuda())
+    d, = torch.autograd.grad(r.logprob.sum(), xd, create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
+    loss = TO.topk_distill_loss(xd, at[:, None].cuda(), torch.zeros(4, 1, device="cuda"))
+    d, = torch.autograd.grad(loss.sum(), xd, create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
+
+
+def test_only_one_of_the_outputs_is_differentiated():
+    x, at, g = _logits(6, 700, "fp32", 28)
+    gl = torch.randn(6, generator=g)
+    xd = x.cuda().requires_grad_(True)
+    r = TO.token_logprobs(xd, at.cuda(), top_k=3)
+    assert not r.top_logprobs.requires_grad and not r.top_ids.requires_grad
+    both, = torch.autograd.grad([r.logprob, r.entropy], [xd], [gl.cuda(), torch.zeros(6, device="cuda")], retain_graph=True)
+    one, = torch.autograd.grad(r.logprob, xd, gl.cuda(), retain_graph=True)
+    assert torch.equal(both, one)
+    both, = torch.autograd.grad([r.logprob, r.entropy], [xd], [torch.zeros(6, device="cuda"), gl.cuda()], retain_graph=True)
+    one, = torch.autograd.grad(r.entropy, xd, gl.cuda())
+    assert torch.equal(both, one)
+
+
+def test_two_threads_at_once():
+    import threading
+    x, at, g = _logits(40, 20000, "bf16", 29)
+    ids, t = _teacher(x, 7, 1.0, g)
+    x, at, ids, t = x.cuda(), at.cuda(), ids.cuda(), t.cuda()
+    want = tuple(TO.token_logprobs(x, at, top_k=6)) + TO.topk_distill_grad(x, ids, t)
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i] = tuple(TO.token_logprobs(x, at, top_k=6)) + TO.topk_distill_grad(x, ids, t)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+
 def test_far_offsets_in_a_large_tensor():
     """Rows behind 2^32 bytes and 2^31 elements of one tensor."""
     V = 70000

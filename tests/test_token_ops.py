@@ -106,6 +106,11 @@ def test_score_refusals():
             ok(x, y, top_k=k)
     with pytest.raises(ValueError):
         ok(torch.zeros(2, 500), top_k=129)
+    for kw in (dict(top_k=2.0), dict(top_k=None), dict(ignore_index=None), dict(ignore_index=-1.0)):
+        with pytest.raises(TypeError):
+            ok(x, y, **kw)
+    with pytest.raises(ValueError):
+        ok(x, y, ignore_index=1 << 70)
     with pytest.raises(TypeError):
         ok(x, y.float())
     with pytest.raises(TypeError):
