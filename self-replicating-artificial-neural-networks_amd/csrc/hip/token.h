@@ -367,20 +367,21 @@ __device__ __forceinline__ void tok_wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
-// n contiguous elements between global memory and LDS, 16 bytes a lane
+// n contiguous elements between global memory and LDS, 16 bytes a lane; all loads of 10 KB (64 rows of 160 bytes) under way at
+// once: a wave has no other to wait with
 template <typename T> __device__ __forceinline__ void tok_stage_in(tok_in<T> x, T* lds, int n) {
-    constexpr int VEC = TokElem<T>::VEC;
+    constexpr int VEC = TokElem<T>::VEC, N = 10;
     const int lane = threadIdx.x, nv = n / VEC;
     u32x4_t* l = reinterpret_cast<u32x4_t*>(lds);
-    int v = lane;
-    for (; v + 192 < nv; v += 256) {
-        u32x4_t r[4];
+    for (int v0 = 0; v0 < nv; v0 += 64 * N) {
+        u32x4_t r[N];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = tok_ld16<T>(x + (v + i * 64) * VEC);
+        for (int i = 0; i < N; ++i)
+            if (v0 + i * 64 + lane < nv) r[i] = tok_ld16<T>(x + (v0 + i * 64 + lane) * VEC);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) l[v + i * 64] = r[i];
+        for (int i = 0; i < N; ++i)
+            if (v0 + i * 64 + lane < nv) l[v0 + i * 64 + lane] = r[i];
     }
-    for (; v < nv; v += 64) l[v] = tok_ld16<T>(x + v * VEC);
     for (int e = nv * VEC + lane; e < n; e += 64) lds[e] = x[e];
 }
 template <typename T> __device__ __forceinline__ void tok_stage_out(const T* lds, tok_out<T> o, int n) {

@@ -477,10 +477,21 @@ template <typename T, bool GRAD> __global__ __launch_bounds__(64) void tok_disti
     const bool there = lane < nrow;
     const float w = there ? (a.w ? a.w[row] : 1.f) : 0.f;
     const bool live = w != 0.f;
-    for (int i = lane; i < nrow * K; i += 64) {
-        const int64_t id = tok_int(a.ids, a.id64, row0 * K + i);
-        is[i] = (uint64_t)id < (uint64_t)V ? (signed char)id : (signed char)-1;
-        ts[i] = a.t[row0 * K + i];
+    for (int i0 = lane; i0 < nrow * K; i0 += 64 * 8) {       // 8 entries a lane under way at once
+        int64_t id[8];
+        float t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i0 + i * 64 < nrow * K) {
+                id[i] = tok_int(a.ids, a.id64, row0 * K + i0 + i * 64);
+                t[i] = a.t[row0 * K + i0 + i * 64];
+            }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i0 + i * 64 < nrow * K) {
+                is[i0 + i * 64] = (uint64_t)id[i] < (uint64_t)V ? (signed char)id[i] : (signed char)-1;
+                ts[i0 + i * 64] = t[i];
+            }
     }
     tok_stage_rows<T>(a.r, row0, nrow, rows);
     T* x = rows + lane * V;
