@@ -185,14 +185,14 @@ struct LossDesc {
 
 // Token operators (token_score.hip, token_distill.hip).  Logits: rows of V elements (dtype 0 fp32, 1 bf16, 2 fp16), row r at
 // (r / n1) * s0 + (r % n1) * s1 elements; loss, log-probabilities, statistics: fp32, one a row.
-int64_t tok_score_segments(int64_t V, int dtype, int64_t rows);
+int64_t tok_score_segments(int64_t V, int dtype);
 void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s0, int64_t s1, int64_t V, double temperature,
                       uint64_t y, int y64, int64_t t0, int64_t t1, int64_t ignore, int k, uint64_t lp, uint64_t ent,
                       uint64_t ids, uint64_t top, uint64_t stat, uint64_t ws, uint64_t stream);
 void launch_tok_score_grad(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s0, int64_t s1, int64_t V,
                            double temperature, uint64_t y, int y64, int64_t t0, int64_t t1, int64_t ignore, uint64_t glp,
                            uint64_t gent, uint64_t stat, uint64_t dx, uint64_t stream);
-int64_t tok_distill_segments(int64_t V, int dtype, int64_t rows, int grad);
+int64_t tok_distill_segments(int64_t V, int dtype, int grad);
 void launch_tok_distill(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s0, int64_t s1, int64_t V, double temperature,
                         uint64_t ids, int id64, uint64_t t, uint64_t w, int K, int bucket, uint64_t loss, uint64_t dx,
                         uint64_t stat, uint64_t pk, uint64_t ws, uint64_t stream);

@@ -193,7 +193,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void to
     constexpr int WORDS = NT * NV * VEC / 32 + 1;
     __shared__ DistEntries E;
     __shared__ uint32_t bits[WORDS];                         // listed tokens of the segment
-    constexpr int SPECIAL = NT == 64 ? 192 : NT == 256 ? 128 : 96;     // a wave
+    constexpr int SPECIAL = NT == 64 ? 192 : NT == 256 ? 128 : NT == 512 ? 96 : 48;     // a wave
     __shared__ TokSpecial<SPECIAL> lists[NW];
     __shared__ float red[NW][3];
     __shared__ int dup, over;                                // an id occurs twice; some wave's list did not fit
@@ -664,18 +664,19 @@ template <typename T, int G> __global__ __launch_bounds__(256) void tok_distill_
 }
 
 // ---- launchers -------------------------------------------------------------------------------------------------------------
-// One pass (loss and gradient from one read) for rows of up to 8192 vectors (512 threads x 16)
-constexpr int DIST_ONE_PASS_VEC = 8192;
+// One pass (loss and gradient from one read) for rows of up to 16384 vectors (1024 threads x 16): 2,000 rows of 50,001 fp32
+// logits 182 us, by two launches 243; statistics alone whole up to 8192
+constexpr int DIST_ONE_PASS_VEC = 16384;
 
-static TokPlan dist_plan(int64_t V, int dtype, int64_t rows) { return tok_plan(V, tok_esize(dtype), rows, 4096, true); }
+static TokPlan dist_plan(int64_t V, int dtype) { return tok_plan(V, tok_esize(dtype), 8192); }
 static bool dist_one_pass(int64_t V, int dtype) { return V / (16 / tok_esize(dtype)) <= DIST_ONE_PASS_VEC; }
 
 // Workspace of a call: segments a row is cut into (16 bytes each when more than one); 0: the one-pass form (with a gradient),
 // which needs no workspace, stat or pk
-int64_t tok_distill_segments(int64_t V, int dtype, int64_t rows, int grad) {
-    if (V <= TOK_NARROW_V || rows <= 0) return grad ? 0 : 1;
+int64_t tok_distill_segments(int64_t V, int dtype, int grad) {
+    if (V <= TOK_NARROW_V) return grad ? 0 : 1;
     if (grad && dist_one_pass(V, dtype)) return 0;
-    return dist_plan(V, dtype, rows).nseg;
+    return dist_plan(V, dtype).nseg;
 }
 
 template <typename T, bool GRAD> static void distill_wide(const DistArgs& a, const TokPlan& p, hipStream_t s) {
@@ -687,7 +688,8 @@ template <typename T, bool GRAD> static void distill_wide(const DistArgs& a, con
     else if (p.nv == 4) tok_launch(tok_distill_kernel<T, 256, 4, GRAD>, units, nt, 0, s, a);
     else if (p.nv == 8) tok_launch(tok_distill_kernel<T, 256, 8, GRAD>, units, nt, 0, s, a);
     else if (p.nt == 256) tok_launch(tok_distill_kernel<T, 256, 16, GRAD>, units, nt, 0, s, a);
-    else if constexpr (GRAD) tok_launch(tok_distill_kernel<T, 512, 16, GRAD>, units, nt, 0, s, a);
+    else if (p.nt == 512) tok_launch(tok_distill_kernel<T, 512, 16, GRAD>, units, nt, 0, s, a);
+    else if constexpr (GRAD) tok_launch(tok_distill_kernel<T, 1024, 16, GRAD>, units, nt, 0, s, a);
 }
 template <typename T, bool GRAD> static void distill_narrow(const DistArgs& a, hipStream_t s) {
     if (tok_lane_rows(a.r.V, sizeof(T), a.r.rows) && a.K <= DIST_LANE_K) {
@@ -751,7 +753,7 @@ void launch_tok_distill(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t
     const bool narrow = V <= TOK_NARROW_V, one = narrow || dist_one_pass(V, dtype), grad = dx && one;
     TokPlan p{};
     if (!narrow) {
-        p = grad ? tok_plan(V, tok_esize(dtype), rows, DIST_ONE_PASS_VEC, false) : dist_plan(V, dtype, rows);
+        p = grad ? tok_plan(V, tok_esize(dtype), DIST_ONE_PASS_VEC) : dist_plan(V, dtype);
         a.nseg = p.nseg;
         a.segvec = p.segvec;
         if (p.nseg > 1 && !ws) throw std::runtime_error("tok_distill: this shape needs a workspace");

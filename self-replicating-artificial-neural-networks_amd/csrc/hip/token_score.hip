@@ -83,7 +83,7 @@ template <typename T, int NT, int NV>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4 : 5))) void tok_score_kernel(ScoreArgs a) {
     constexpr int VEC = TokElem<T>::VEC, NW = NT / 64;
     // one-wave rows: 8 KB of lists a block, or LDS would keep waves away
-    constexpr int SPECIAL = NT == 64 ? 192 : 128;     // vectors a wave
+    constexpr int SPECIAL = NT == 64 ? 192 : NT == 256 ? 128 : 64;     // vectors a wave
     constexpr int CAND = NT == 64 ? 512 : 1024;
     __shared__ float red[NW][3];
     __shared__ uint64_t best[NW];
@@ -305,7 +305,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
 // Joins the segments of a row.  The sums are rescaled to the row's maximum, a segment a lane, and added by a fixed tree.  Of
 // the sorted lists of keys: with j = ceil(k / lists), the smallest of the j-th keys has at least k keys at or above it, and so
 // has the largest of the k-th keys; what lies below both is dropped, the rest (about 1.5 k) ranked by counting.  One wave for
-// up to 512 keys a row (2,000 rows of 4 lists of 32: 9.4 us, with four waves and their barriers 12.4), four for more.
+// up to 32 alternatives and 512 keys a row (2,000 rows of 4 lists of 32: 9.4 us, with four waves and their barriers 12.4), four
+// for more (48 rows of 4 lists of 64: 7.9 us, with one wave 11.0).
 constexpr int JOIN_CAND = 1024;
 template <int NT> __global__ __launch_bounds__(NT) void tok_score_join_kernel(ScoreArgs a, int dtype) {
     __shared__ __attribute__((aligned(16))) uint64_t cand[JOIN_CAND];
@@ -698,11 +699,12 @@ __global__ __launch_bounds__(256) void tok_score_grad_narrow_kernel(ScoreGradArg
 }
 
 // ---- launchers ---------------------------------------------------------------------------------------------------------
-static TokPlan score_plan(int64_t V, int dtype, int64_t rows) { return tok_plan(V, tok_esize(dtype), rows, 4096, true); }
+// whole up to 8192 vectors (512 threads x 16): 2,000 rows of 32,000 fp32 logits 40 us, in two pieces 42; one row 5.4 and 8.7
+static TokPlan score_plan(int64_t V, int dtype) { return tok_plan(V, tok_esize(dtype), 8192); }
 
 // segments a row is cut into (the workspace holds 16 + 8 k bytes for each when more than one)
-int64_t tok_score_segments(int64_t V, int dtype, int64_t rows) {
-    return V <= TOK_NARROW_V || rows <= 0 ? 1 : score_plan(V, dtype, rows).nseg;
+int64_t tok_score_segments(int64_t V, int dtype) {
+    return V <= TOK_NARROW_V ? 1 : score_plan(V, dtype).nseg;
 }
 
 template <typename T> static void score_wide(const ScoreArgs& a, const TokPlan& p, hipStream_t s) {
@@ -713,7 +715,8 @@ template <typename T> static void score_wide(const ScoreArgs& a, const TokPlan& 
     else if (p.nt == 64) tok_launch(tok_score_kernel<T, 64, 8>, units, nt, 0, s, a);
     else if (p.nv == 4) tok_launch(tok_score_kernel<T, 256, 4>, units, nt, 0, s, a);
     else if (p.nv == 8) tok_launch(tok_score_kernel<T, 256, 8>, units, nt, 0, s, a);
-    else tok_launch(tok_score_kernel<T, 256, 16>, units, nt, 0, s, a);
+    else if (p.nt == 256) tok_launch(tok_score_kernel<T, 256, 16>, units, nt, 0, s, a);
+    else tok_launch(tok_score_kernel<T, 512, 16>, units, nt, 0, s, a);
 }
 template <typename T> static void score_narrow(const ScoreArgs& a, hipStream_t s) {
     if (tok_lane_rows(a.r.V, sizeof(T), a.r.rows) && a.k <= 8) {        // more alternatives: rounds on 8 lanes cost less
@@ -770,7 +773,7 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
         else score_narrow<f16_t>(a, s);
             return;
     }
-    const TokPlan p = score_plan(V, dtype, rows);
+    const TokPlan p = score_plan(V, dtype);
     a.nseg = p.nseg;
     a.segvec = p.segvec;
     if (p.nseg > 1) {
@@ -782,7 +785,7 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
     else if (dtype == 1) score_wide<bf16_t>(a, p, s);
     else score_wide<f16_t>(a, p, s);
     if (p.nseg > 1) {
-        if (p.nseg * k <= 512) tok_launch(tok_score_join_kernel<64>, rows, 64, 0, s, a, dtype);
+        if (k <= 32 && p.nseg * k <= 512) tok_launch(tok_score_join_kernel<64>, rows, 64, 0, s, a, dtype);
         else tok_launch(tok_score_join_kernel<256>, rows, 256, 0, s, a, dtype);
     }
 }

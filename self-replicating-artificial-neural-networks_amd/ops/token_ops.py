@@ -140,13 +140,13 @@ def _same_rows(y, n1, rows):
 
 
 @functools.lru_cache(maxsize=1024)
-def _score_segments(V, code, rows):
-    return H.lib().tok_score_segments(V, code, rows)
+def _score_segments(V, code):
+    return H.lib().tok_score_segments(V, code)
 
 
 @functools.lru_cache(maxsize=1024)
-def _distill_segments(V, code, rows, grad):
-    return H.lib().tok_distill_segments(V, code, rows, grad)
+def _distill_segments(V, code, grad):
+    return H.lib().tok_distill_segments(V, code, grad)
 
 
 # the current stream of a device as the launchers take it; torch.cuda.current_stream() builds a Stream object first (2 of the
@@ -202,7 +202,7 @@ def _score_hip(logits, targets, temperature, top_k, ignore_index, want_stat):
         stat = x.new_empty((rows, 3), dtype=torch.float32)
         stp = stat.data_ptr()
         saved = (x, y, stat)
-    nseg = _score_segments(V, code, rows)
+    nseg = _score_segments(V, code)
     if nseg > 1:
         ws = x.new_empty(rows * nseg * (2 + top_k), dtype=torch.int64)
         wsp = ws.data_ptr()
@@ -323,7 +323,7 @@ def _distill_hip(logits, ids, logprobs, temperature, bucket, weight, dx, save):
     if dx is True:
         dx = x.new_empty(logits.shape)
     stp = pkp = wsp = 0
-    nseg = _distill_segments(V, code, rows, dx is not None)
+    nseg = _distill_segments(V, code, dx is not None)
     stat = pk = None
     if save or dx is not None and nseg > 0:
         stat = x.new_empty((rows, 4), dtype=torch.float32)

@@ -101,7 +101,7 @@ def _check_score(x, y, T, k, grad=True, seed=0, tile=1):
 
 # every launch shape: lane groups (V <= 512), one-wave rows, 256-thread rows, rows cut into segments; odd sizes around each
 SIZES = [1, 2, 3, 7, 8, 9, 40, 63, 64, 65, 127, 129, 255, 257, 511, 512, 513, 1000, 1025, 2047, 2049, 4095, 4097, 8193, 16385,
-         32000, 32769, 50001]
+         32000, 32769, 50001, 65537]
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
@@ -324,7 +324,7 @@ def _check_distill(x, ids, t, T, tail, w, tile=1):
 
 @pytest.mark.parametrize("tail", ["drop", "bucket"])
 @pytest.mark.parametrize("dtype", list(DTYPES))
-@pytest.mark.parametrize("V", [1, 2, 7, 8, 9, 40, 64, 65, 129, 257, 512, 513, 1025, 2049, 4097, 8193, 32000, 65537, 70001])
+@pytest.mark.parametrize("V", [1, 2, 7, 8, 9, 40, 64, 65, 129, 257, 512, 513, 1025, 2049, 4097, 8193, 32000, 65537, 70001, 131080])
 def test_distill_sizes(V, dtype, tail):
     R = 5 if V > 600 else 37
     x, _, g = _logits(R, V, dtype, V)
