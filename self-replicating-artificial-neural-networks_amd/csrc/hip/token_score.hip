@@ -203,6 +203,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
     __syncthreads();                                         // the sums and the candidates are complete
     const int nc = ncand;
     const bool slow = !(B > -INFINITY) || nc > CAND;
+    if (a.k == 0 && !slow && wave) return;                   // the rest is one wave's work
     if (slow) {
         // thousands of vectors at the bound (equal values), or fewer than k elements left: element by element, read again
         sum = ScoreSums{0.f, 0.f, 0.f};
