@@ -70,7 +70,7 @@ __device__ __forceinline__ gc_f32x4_t gc_mma(const GcFrag& a, const GcFrag& b, g
 // 2s and 2s + 1
 __device__ __forceinline__ int gc_perm(int s, int q, int j) { return 32 * s + 16 * (j >> 2) + 4 * q + (j & 3); }
 
-typedef float gc_f2 __attribute__((ext_vector_type(2)));    // packed fp32 (v_pk_* VALU)
+typedef float gc_f2 __attribute__((ext_vector_type(2)));    // pairs of fp32 (the build keeps them off v_pk_*)
 
 // Activations resolved at compile time: A = ACT_LINEAR / ACT_RELU / ACT_SIGMOID, or GC_ACT_RT (-1) for
 // a runtime code (activated Conv1D layers, which the generator's template never emits).

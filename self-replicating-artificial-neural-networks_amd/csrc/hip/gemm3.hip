@@ -2709,7 +2709,7 @@ __global__ __launch_bounds__(256) void g3_tiled_kernel(const GemmDesc* __restric
         const int sc = t & 31, sg = t >> 5;              // column of the slice, 16-row group
         // rows past M: their dY is 0 (the A loads returned zeros) and their act' is masked below, so every
         // sum gets exact zeros from them.  Activation and the full-rows case are compile-time in the row
-        // loop; the rows are taken in pairs so the sums issue as packed fp32 (v_pk_fma_f32)
+        // loop; the rows are taken in pairs (float2 arithmetic; the build keeps it off v_pk_*)
         const int nrow = M - m0 - sg * 16;
         auto col_sums = [&](auto act_tag, auto full_tag, const float* xc, const float* gc, float w, float bv,
                             float mu, float is, float* sm) {
