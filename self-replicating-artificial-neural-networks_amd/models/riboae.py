@@ -133,21 +133,29 @@ class GeneticAutoencoder(nn.Module):
         return logits.argmax(-1)
 
     def _decode(self, x, z):
-        if z.is_cuda and os.environ.get("SERANN_RIBOAE_HIP", "1") != "0":
-            from ..ops.riboae_ops import available, categorical_loglik
-            if available():
-                # fused log-softmax + gather + sum over the sequence (HIP, SURVEY K37)
-                return categorical_loglik(self.generative_net.logits(z), x)
-        logp = self.generative_net(z)                               # (B, L, V) log-probs
-        return torch.gather(logp, -1, x.long().unsqueeze(-1)).squeeze(-1).sum(-1)
+        return self._fit(x, z)[0]
 
-    def _distill(self, z, teacher):
-        """-sum over the positions of KL(teacher's top tokens || this decoder), (B,): takes the place of log p(x|z) when the
-        decoder learns from another autoencoder.  teacher: (ids, log-probabilities, temperature), see
-        :meth:`distill_targets`."""
+    def _fit(self, x, z, teacher=None):
+        """(log p(x|z), the term of the loss), (B,) each.  Without a teacher they are the same; with one, the term is -sum over
+        the positions of KL(teacher's top tokens || this decoder).  teacher: (ids, log-probabilities, temperature), see
+        :meth:`distill_targets`.  The decoder runs once (its BatchNorm layers take every pass of a training step in)."""
+        logits = self.generative_net.logits(z)
+        logpx_z = self._loglik(logits, x)
+        if teacher is None:
+            return logpx_z, logpx_z
         from ..ops.token_ops import topk_distill_loss
         ids, logp, temperature = teacher
-        return -topk_distill_loss(self.generative_net.logits(z), ids, logp, temperature=temperature).sum(-1)
+        return logpx_z, -topk_distill_loss(logits, ids, logp, temperature=temperature).sum(-1)
+
+    @staticmethod
+    def _loglik(logits, x):
+        if logits.is_cuda and os.environ.get("SERANN_RIBOAE_HIP", "1") != "0":
+            from ..ops.riboae_ops import available, categorical_loglik
+            if available():
+                # fused log-softmax + gather + sum over the sequence (HIP)
+                return categorical_loglik(logits, x)
+        logp = F.log_softmax(logits, dim=-1)                        # (B, L, V) log-probs
+        return torch.gather(logp, -1, x.long().unsqueeze(-1)).squeeze(-1).sum(-1)
 
     def encode(self, x):
         return self.inference_net(x).argmax(-1)
@@ -260,14 +268,12 @@ class ConcreteGAE(GeneticAutoencoder):
             from ..ops.riboae_ops import available, concrete_sample
             if available():                                        # K36 fused sample + softmax + KL
                 z, kl = concrete_sample(self.inference_net(x), temperature, self.prior_temperature, noise)
-                logpx_z = self._decode(x, z)
-                fit = logpx_z if teacher is None else self._distill(z, teacher)
+                logpx_z, fit = self._fit(x, z, teacher)
                 nelbo = -(fit - kld_weight * kl).mean()
                 return {"loss": nelbo, "nll": -logpx_z.mean(), "kld": kl.mean()}
         z, logq, logp = self._encode(x, temperature, noise)
-        logpx_z = self._decode(x, z)
+        logpx_z, fit = self._fit(x, z, teacher)
         kl = (logq - logp).flatten(1).sum(1)
-        fit = logpx_z if teacher is None else self._distill(z, teacher)
         nelbo = -(fit - kld_weight * kl).mean()
         return {"loss": nelbo, "nll": -logpx_z.mean(), "kld": kl.mean()}
 
@@ -278,8 +284,9 @@ class DeterministicGAE(GeneticAutoencoder):
 
     def compute_loss(self, x, *args, teacher=None, **kw):
         z = self._encode(x)
-        nll = -self._decode(x, z).mean()
-        return {"loss": nll if teacher is None else -self._distill(z, teacher).mean(), "nll": nll, "kld": torch.zeros((), device=nll.device)}
+        logpx_z, fit = self._fit(x, z, teacher)
+        nll = -logpx_z.mean()
+        return {"loss": nll if teacher is None else -fit.mean(), "nll": nll, "kld": torch.zeros((), device=nll.device)}
 
 
 def build_model(kind: str = "concrete", **hp) -> GeneticAutoencoder:

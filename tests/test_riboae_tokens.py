@@ -89,6 +89,19 @@ def test_loss_against_a_teacher(kind):
     assert torch.allclose(got.double(), total, rtol=0, atol=200 * O.U * float(dx.abs().sum()) / 6)
 
 
+@pytest.mark.parametrize("kind", ["concrete", "deterministic"])
+def test_a_teacher_leaves_the_moving_statistics_of_a_step(kind):
+    """The decoder runs once a step, with and without a teacher: its BatchNorm layers take the batch's statistics in once."""
+    x = torch.randint(0, 12, (6, 32), generator=torch.Generator().manual_seed(5))
+    kw = dict(noise=torch.rand(6, 20, 2, generator=torch.Generator().manual_seed(6))) if kind == "concrete" else {}
+    taught = _model(1).distill_targets(x, 5, 2.0)
+    plain, learner = _model(2, kind).train(), _model(2, kind).train()
+    plain.compute_loss(x, 0.3, 0.05, **kw)
+    learner.compute_loss(x, 0.3, 0.05, teacher=taught, **kw)
+    for (name, a), (_, b) in zip(plain.named_buffers(), learner.named_buffers()):
+        assert torch.equal(a, b), name
+
+
 def test_trainer_learns_from_a_teacher(tmp_path):
     teacher, m = _model(1), _model(2)
     before = copy.deepcopy(teacher.state_dict())
