@@ -149,6 +149,29 @@ def _distill_segments(V, code, grad):
     return H.lib().tok_distill_segments(V, code, grad)
 
 
+def _span(t):
+    """[first, last) byte of what a tensor's elements cover."""
+    if t.numel() == 0:
+        return 0, 0
+    n = 1 + sum((k - 1) * s for k, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _check_out(out, logits, *inputs):
+    if not isinstance(out, torch.Tensor):
+        raise TypeError("out must be a tensor")
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of the logits' shape, type and device")
+    if out.requires_grad:
+        raise ValueError("out must not require a gradient")
+    lo, hi = _span(out)
+    for t in (logits,) + inputs:
+        if t is not None:
+            a, b = _span(t)
+            if a < hi and lo < b:
+                raise ValueError("out must not share memory with the logits or another argument")
+
+
 # the current stream of a device as the launchers take it; torch.cuda.current_stream() builds a Stream object first (2 of the
 # 16 us that a small call took)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
@@ -423,14 +446,13 @@ def topk_distill_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
                       out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The losses of :func:`topk_distill_loss` and the gradient of their sum with respect to ``logits``, in one pass over the
     logits where a row fits a block's registers.  The gradient has the logits' shape and type, is contiguous, and goes to
-    ``out`` when given (which must not share memory with the logits).  Nothing is recorded for autograd."""
+    ``out`` when given (which must not share memory with any argument).  Nothing is recorded for autograd."""
     temperature = _check_logits(logits, temperature)
     _check_teacher(logits, teacher_ids, teacher_logprobs, tail, weight)
     if out is not None:
-        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or not out.is_contiguous():
-            raise ValueError("out must be a contiguous tensor of the logits' shape, type and device")
-        if out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr() and logits.numel():
-            raise ValueError("out must not share memory with the logits")
+        _check_out(out, logits, teacher_ids, teacher_logprobs, weight)
+        if not out.is_inference():
+            torch.autograd.graph.increment_version(out)      # autograd notices if it had been saved for a backward pass
     logits = logits.detach()
     if not logits.is_cuda:
         with torch.enable_grad():

@@ -150,6 +150,31 @@ def test_distill_refusals():
             TO.topk_distill_grad(x, ids, t, out=out)
 
 
+def test_gradient_into_a_given_tensor():
+    """``out`` may lie beside the arguments in one allocation, but overlap none of them; autograd sees that it was written."""
+    g = torch.Generator().manual_seed(11)
+    ids = torch.randint(0, 10, (4, 3), generator=g)
+    flat = torch.randn(140, generator=g)
+    x, t, w = flat[:40].view(4, 10), flat[40:52].view(4, 3), flat[52:56]
+    want_loss, want = TO.topk_distill_grad(x, ids, t, weight=w)
+    for start in (1, 13, 39, 40, 51, 55):                  # over the logits, the teacher, the weights
+        with pytest.raises(ValueError):
+            TO.topk_distill_grad(x, ids, t, weight=w, out=flat[start:start + 40].view(4, 10))
+    with pytest.raises(ValueError):
+        TO.topk_distill_grad(x, ids, t, out=torch.zeros(4, 10, requires_grad=True))
+    with pytest.raises(TypeError):
+        TO.topk_distill_grad(x, ids, t, out=[0.0])
+    out = flat[56:96].view(4, 10)
+    loss, dx = TO.topk_distill_grad(x, ids, t, weight=w, out=out)
+    assert dx is out and torch.equal(dx, want) and torch.equal(loss, want_loss)
+    a = torch.ones(4, 10, requires_grad=True)
+    out = torch.zeros(4, 10)
+    y = (a * out).sum()
+    TO.topk_distill_grad(x, ids, t, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_row_layouts():
     """Strided rows are described, not copied, where two strides do."""
     x = torch.zeros(3, 6, 10)
