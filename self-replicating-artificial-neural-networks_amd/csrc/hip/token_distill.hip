@@ -769,7 +769,7 @@ void launch_tok_distill(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t
         if (dtype == 0) tok_launch(tok_distill_join_kernel<float>, units, nt, 0, s, a);
         else if (dtype == 1) tok_launch(tok_distill_join_kernel<bf16_t>, units, nt, 0, s, a);
         else tok_launch(tok_distill_join_kernel<f16_t>, units, nt, 0, s, a);
-        }
+    }
     if (dx && !grad)
         launch_tok_distill_grad(x, dtype, rows, n1, s0, s1, V, temperature, ids, id64, w, K, 0, stat, pk, dx, stream);
 }

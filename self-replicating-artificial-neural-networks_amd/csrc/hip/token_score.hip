@@ -305,9 +305,10 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
 
 // Joins the segments of a row.  The sums are rescaled to the row's maximum, a segment a lane, and added by a fixed tree.  Of
 // the sorted lists of keys: with j = ceil(k / lists), the smallest of the j-th keys has at least k keys at or above it, and so
-// has the largest of the k-th keys; what lies below both is dropped, the rest (about 1.5 k) ranked by counting.  One wave for
-// up to 32 alternatives and 512 keys a row (2,000 rows of 4 lists of 32: 9.4 us, with four waves and their barriers 12.4), four
-// for more (48 rows of 4 lists of 64: 7.9 us, with one wave 11.0).
+// has the largest of the k-th keys; what lies below both is dropped, the rest (about 1.5 k) ranked by counting.  Four waves a row
+// share the keys (fp32, rows of 4 lists: 48 rows of lists of 16 4.0 us, with one wave 5.0; of 32 4.4 and 8.0; 2,000 rows of 64
+// 12.0 and 16.8); one wave where the barriers would cost more: up to 32 keys (2,000 rows of lists of 8: 6.2 us, with four waves
+// 8.8; 8 rows: 3.7 and 3.8), and up to 96 where the rows fill the chip (2,000 rows of lists of 16: 7.1 and 9.0).
 constexpr int JOIN_CAND = 1024;
 template <int NT> __global__ __launch_bounds__(NT) void tok_score_join_kernel(ScoreArgs a, int dtype) {
     __shared__ __attribute__((aligned(16))) uint64_t cand[JOIN_CAND];
@@ -772,7 +773,7 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
         if (dtype == 0) score_narrow<float>(a, s);
         else if (dtype == 1) score_narrow<bf16_t>(a, s);
         else score_narrow<f16_t>(a, s);
-            return;
+        return;
     }
     const TokPlan p = score_plan(V, dtype);
     a.nseg = p.nseg;
@@ -786,7 +787,8 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
     else if (dtype == 1) score_wide<bf16_t>(a, p, s);
     else score_wide<f16_t>(a, p, s);
     if (p.nseg > 1) {
-        if (k <= 32 && p.nseg * k <= 512) tok_launch(tok_score_join_kernel<64>, rows, 64, 0, s, a, dtype);
+        const int nk = p.nseg * k;
+        if (nk <= 32 || (nk <= 96 && rows > 1024)) tok_launch(tok_score_join_kernel<64>, rows, 64, 0, s, a, dtype);
         else tok_launch(tok_score_join_kernel<256>, rows, 256, 0, s, a, dtype);
     }
 }
