@@ -20,7 +20,7 @@
 struct ScoreArgs {
     TokRows r;
     int64_t y, t0, t1, ignore;   // targets (0: none), their strides
-    int y64, k;
+    int y64, k, kj;              // kj: see tok_counted_bound; 0 where k lanes' maxima do
     int nseg, segvec;
     float *lp, *ent;
     int64_t* ids;
@@ -79,6 +79,33 @@ struct ScoreSums {
     }
 };
 
+// One wave, many alternatives: k lanes' maxima would be a poor bound (of 64 lanes the lowest one).  A value that some 1.25 k elements
+// should reach, were they spread evenly -- the kj-th largest of the lanes' maxima -- is put right by counting the row's elements
+// at or above it: k to `cap` of them are looked for, by steps and bisection.  -inf, or more than cap, where 16 counts do not find
+// such a value.
+template <typename SEG> __device__ __forceinline__ float tok_counted_bound(const SEG& s, float tm, float m, int k, int kj, int cap) {
+    float B = tok_kth_bound(tm, kj), lo = -INFINITY, hi = m;
+    if (!(m < INFINITY)) return -INFINITY;
+    if (B == -INFINITY) B = tok_group<64, TokMin>(tm > -INFINITY ? tm : m);
+    float step = m > B ? m - B : fabsf(m) * 0.0078125f + 1e-6f;
+    for (int it = 0; it < 16 && B > -INFINITY; ++it) {
+        const int c = s.count(B);
+        if (c >= k) {
+            lo = B;
+            if (c <= cap) break;
+        } else {
+            hi = B;
+        }
+        if (lo == -INFINITY) {
+            B -= step;
+            step *= 2.f;
+        } else {
+            B = 0.5f * lo + 0.5f * hi;
+        }
+    }
+    return lo;
+}
+
 template <typename T, int NT, int NV>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4 : 5))) void tok_score_kernel(ScoreArgs a) {
     constexpr int VEC = TokElem<T>::VEC, NW = NT / 64;
@@ -120,19 +147,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
     float wb = wm0;
     if (a.k > 1) {
         // this wave's share of the bound
-        const int kk = NW == 1 ? a.k : (a.k + NW - 1) / NW;
-        if (kk <= 64) {
-            wb = tok_kth_bound(tm, kk);
-        } else {
-            // one wave, k > 64: two elements a lane (the two best vectors' maxima) at or above the smallest second one
-            float b1 = s.xt, b2 = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                b2 = tok_max(b2, fminf(b1, s.vm[i]));
-                b1 = tok_max(b1, s.vm[i]);
-            }
-            wb = tok_group<64, TokMin>(b2);
-        }
+        if constexpr (NW > 1) wb = tok_kth_bound(tm, (a.k + NW - 1) / NW);
+        else wb = a.kj == 0 ? tok_kth_bound(tm, a.k) : tok_counted_bound(s, tm, wm0, a.k, a.kj, min(a.k + (a.k >> 1) + 16, SPECIAL));
     }
     if (lane == 0) {
         red[wave][0] = wm0;
@@ -177,13 +193,18 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
             if (lane == 0) atomicAdd(&ncand, CAND + 1);
         } else if (a.k) {
             // the wave's candidates, one atomic for all that a step finds; their order does not matter
+            int have = 0;
             const auto put = [&](bool hit, uint64_t key) {
                 const uint64_t mask = __ballot(hit);
                 if (mask == 0) return;
-                int base = 0;
-                if (lane == 0) base = atomicAdd(&ncand, (int)__popcll(mask));
-                const int at = __builtin_amdgcn_readfirstlane(base) + tok_below(mask);
+                int base = have;
+                if constexpr (NW > 1) {
+                    if (lane == 0) base = atomicAdd(&ncand, (int)__popcll(mask));
+                    base = __builtin_amdgcn_readfirstlane(base);
+                }
+                const int at = base + tok_below(mask);
                 if (hit && at < CAND) cand[at] = key;
+                have += (int)__popcll(mask);
             };
             for (int b = 0; b < nl * VEC; b += 64) {
                 const int i = b + lane, slot = min(i / VEC, nl - 1), e = i & (VEC - 1);
@@ -191,6 +212,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
                 put(i < nl * VEC && xv >= B, tok_key(xv, e0 + list.vec(slot) * VEC + e));
             }
             if (ntail && wave == 0) put(tid < ntail && s.xt >= B, tok_key(s.xt, e0 + nv * VEC + tid));
+            if (NW == 1 && lane == 0) ncand = have;
         }
     }
     float S = tok_group<64, TokSum>(sum.S), W = tok_group<64, TokSum>(sum.W), n = tok_group<64, TokSum>(sum.n);
@@ -440,11 +462,10 @@ template <> struct NarrowKey<float> {
     static __device__ __forceinline__ int index(uint64_t k) { return tok_key_index(k); }
     static __device__ __forceinline__ float value(uint64_t k) { return tok_key_value(k); }
 };
-template <typename K> __device__ __forceinline__ void order2(K& a, K& b) {
-    const K hi = a > b ? a : b, lo = a > b ? b : a;
-    a = hi;
-    b = lo;
-}
+// Up to this many alternatives of a narrow row by rounds of the group's best head, more by sorting the row (120,000 rows of 40 fp32
+// logits: k = 12 27 us, sorted 29; k = 20 36 and 30; k = 40 56 and 30.  Of 200: k = 20 136 and 148, k = 40 232 and 144).  Groups of 64
+// lanes get no more than score_narrow_takes lets through.
+template <int G> constexpr int NARROW_ROUNDS = G == 8 ? 16 : G == 16 ? 20 : 24;
 
 template <typename T, int G>
 __global__ __launch_bounds__(256) void tok_score_narrow_kernel(ScoreArgs a) {
@@ -488,13 +509,39 @@ __global__ __launch_bounds__(256) void tok_score_narrow_kernel(ScoreArgs a) {
             const bool in = gl * 8 + e < V && f[e] == f[e];
             h[e] = in ? NK::make(f[e], gl * 8 + e) : (K)0;
         }
-        // Batcher's odd-even merge sort of 8, largest first
-        order2(h[0], h[1]); order2(h[2], h[3]); order2(h[4], h[5]); order2(h[6], h[7]);
-        order2(h[0], h[2]); order2(h[1], h[3]); order2(h[4], h[6]); order2(h[5], h[7]);
-        order2(h[1], h[2]); order2(h[5], h[6]);
-        order2(h[0], h[4]); order2(h[1], h[5]); order2(h[2], h[6]); order2(h[3], h[7]);
-        order2(h[2], h[4]); order2(h[3], h[5]);
-        order2(h[1], h[2]); order2(h[3], h[4]); order2(h[5], h[6]);
+        tok_sort_lane<8>(h);
+        if (G < 64 && a.k > NARROW_ROUNDS<G>) {
+            tok_sort_group<G, 8>(h, gl);
+            const int at = gl * 8;
+            if (live && at < a.k) {
+                int64_t id[8];
+                float lp[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const K key = S == S ? h[e] : (K)0;
+                    id[e] = key ? NK::index(key) : -1;
+                    lp[e] = key ? score_toplp(a, NK::value(key), m, lnS) : NAN;
+                }
+                tok_out<int64_t> ids = (tok_out<int64_t>)a.ids + row * a.k + at;
+                tok_out<float> top = (tok_out<float>)a.top + row * a.k + at;
+                if (at + 8 <= a.k) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2)
+                        tok_st16<int64_t>(ids + e, u32x4_t{(uint32_t)id[e], (uint32_t)(id[e] >> 32), (uint32_t)id[e + 1],
+                                                           (uint32_t)(id[e + 1] >> 32)});
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4) tok_st16<float>(top + e, TokElem<float>::pack(lp + e));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (at + e < a.k) {
+                            ids[e] = id[e];
+                            top[e] = lp[e];
+                        }
+                }
+            }
+            return;
+        }
         K keep = 0;
         for (int j = 0; j < a.k; ++j) {
             const K top = tok_group<G, TokTop>(h[0]);
@@ -704,6 +751,17 @@ __global__ __launch_bounds__(256) void tok_score_grad_narrow_kernel(ScoreGradArg
 // whole up to 8192 vectors (512 threads x 16): 2,000 rows of 32,000 fp32 logits 40 us, in two pieces 42; one row 5.4 and 8.7
 static TokPlan score_plan(int64_t V, int dtype) { return tok_plan(V, tok_esize(dtype), 8192); }
 
+// Up to this many alternatives of a row on one wave by the lanes' maxima, more by a counted bound (120,000 rows of 1,000 fp32
+// logits: k = 20 182 us, counted 198; k = 32 250 and 247; k = 64 1,390 and 337; k = 100 4,540 and 482, before the candidates were sorted)
+constexpr int ONE_WAVE_LANES = 24;
+
+// Rows of 257 to 512 elements with alternatives: a row a wave by the long rows' kernel where listing candidates costs less than
+// rounds over 64 lanes (120,000 rows of 500: fp32 with k = 1 104 us, narrow 108, k = 20 139 and 300; bf16 with k = 8 136 and
+// 120, k = 20 152 and 169)
+static bool score_narrow_takes(int64_t V, int dtype, int k) {
+    return V <= 256 || (V <= TOK_NARROW_V && k <= (dtype == 0 ? 0 : 12));
+}
+
 // segments a row is cut into (the workspace holds 16 + 8 k bytes for each when more than one)
 int64_t tok_score_segments(int64_t V, int dtype) {
     return V <= TOK_NARROW_V ? 1 : score_plan(V, dtype).nseg;
@@ -769,7 +827,7 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
     a.stat = as_ptr<float>(stat);
     a.nseg = 1;
     const hipStream_t s = as_stream(stream);
-    if (V <= TOK_NARROW_V) {
+    if (score_narrow_takes(V, dtype, k)) {
         if (dtype == 0) score_narrow<float>(a, s);
         else if (dtype == 1) score_narrow<bf16_t>(a, s);
         else score_narrow<f16_t>(a, s);
@@ -778,6 +836,11 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
     const TokPlan p = score_plan(V, dtype);
     a.nseg = p.nseg;
     a.segvec = p.segvec;
+    if (p.nt == 64 && k > ONE_WAVE_LANES) {
+        const int64_t nvec = V / (16 / tok_esize(dtype)), lanes = nvec < 64 ? nvec : 64;
+        const double q = 1.25 * k / V, n = (double)V / lanes;
+        a.kj = q < 1 ? (int)ceil(lanes * (1 - pow(1 - q, n))) : (int)lanes;
+    }
     if (p.nseg > 1) {
         if (!ws) throw std::runtime_error("tok_score: this shape needs a workspace");
         a.part = as_ptr<float4>(ws);

@@ -122,6 +122,35 @@ def test_score_top_k(V, k, dtype):
     _check_score(x, at, 2.0, k, grad=False)
 
 
+MANY_KINDS = {
+    "normal": lambda V, g: torch.randn(6, V, generator=g) * 2.5,
+    "ascending": lambda V, g: (torch.arange(V) / V * 8).expand(6, V).clone(),
+    "one_block": lambda V, g: torch.where((torch.arange(V) // 16) % 9 == 0, torch.randn(6, V, generator=g) + 9, torch.randn(6, V, generator=g)),
+    "few_values": lambda V, g: torch.randint(0, 5, (6, V), generator=g).float(),
+    "heavy_tail": lambda V, g: torch.randn(6, V, generator=g) / torch.rand(6, V, generator=g).clamp_min(1e-3) - 20,
+    "few_left": lambda V, g: torch.where(torch.rand(6, V, generator=g) < 0.05, torch.randn(6, V, generator=g), -math.inf),
+    "half_left": lambda V, g: torch.where(torch.arange(V) < V // 2, torch.randn(6, V, generator=g), -math.inf),
+    "lowest": lambda V, g: torch.where(torch.rand(6, V, generator=g) < 0.5, torch.randn(6, V, generator=g), torch.finfo(torch.float16).min),
+}
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("kind", list(MANY_KINDS))
+def test_score_many_alternatives(kind, dtype):
+    """Sorted short rows, counted bounds of rows on one wave, lists longer than a wave: the same ranking, whatever the values."""
+    for V, ks in ((33, (17, 33)), (64, (16, 64)), (100, (20, 21, 100)), (129, (24, 25, 128)), (256, (25, 128)), (257, (1, 13, 128)),
+                  (300, (12, 24, 64)), (512, (13, 25, 128)), (700, (24, 25, 90)), (1030, (48, 128)), (2500, (31, 128)),
+                  (4091, (64, 128)), (6000, (100,))):
+        g = torch.Generator().manual_seed(V)
+        x = MANY_KINDS[kind](V, g).to(DTYPES[dtype])
+        if kind == "normal":
+            x[2, V // 3] = math.nan
+        y = x.float().nan_to_num(0.0).argmax(-1)
+        for k in ks:
+            print(kind, dtype, V, k, flush=True)
+            _check_score(x, y, 1.3, k, grad=False)
+
+
 @pytest.mark.parametrize("V", [40, 700, 5000, 40000])
 @pytest.mark.parametrize("kind", ["constant", "two_values", "ascending", "zeros_signed", "mostly_masked"])
 def test_score_ties_go_to_the_lowest_index(V, kind):
