@@ -11,8 +11,8 @@
 // 256 CUs have at 5 TB/s of bf16, so every operation an element counts (one fma to the exponent, v_max3, no canonicalisation).
 // Top k: k threads' maxima are k different elements, so the smallest of the per-wave ceil(k / waves)-th largest thread
 // maxima is a lower bound of the k-th largest element.  The vectors that reach it go to an LDS list (about 1.5 k of them);
-// their elements at or above it are ranked by counting: no data-dependent loop.  If the lists overflow (thousands of equal
-// values), k exact argmax rounds over the row replace them: slower, never wrong.
+// their elements at or above it are ranked: no data-dependent loop.  Where the lists overflow (thousands of equal values) or fewer
+// than k elements are left (masks), the k-th value is found by counting instead (score_select), the row read again from L2.
 // Narrow rows (V <= 512, the autoencoder's vocabulary): 8 to 64 lanes a row with 8 elements each; the lane's 8 keys are
 // sorted by a network and k rounds take the best head of the group.
 #include "token.h"
@@ -106,14 +106,131 @@ template <typename SEG> __device__ __forceinline__ float tok_counted_bound(const
     return lo;
 }
 
+// The k best of a block's elements (nv vectors at x, then the ntail elements xt; none is NaN or +inf; the row's element e0 is the
+// first) whatever their values: all elements above some t, ranked, and where they are fewer than k the first of those equal to t
+// in the order of their index.  t is the maximum m where n >= k have it, -inf where up to CAND are above that, else found bit by
+// bit in the order of floats, a count of the block a bit, until k to CAND are at or above it or all bits are known.  A row of
+// 32,000 bf16 logits of which 10 are not masked, k = 64: 25 us; k rounds of a block-wide maximum, the next smaller key each, took
+// 320; 20,000 equal rows of 1,000 fp32, k = 20: 37 and 190.  Returns how many there are.
+template <typename T, int NT, int CAND, typename F>
+__device__ __forceinline__ int score_select(tok_in<T> x, int nv, int ntail, float xt, int e0, int k, float m, float n, uint64_t* cand,
+                                         int* ncand, int* tally, const F& emit) {
+    constexpr int VEC = TokElem<T>::VEC, NW = NT / 64;
+    constexpr int LOW = sizeof(T) == 4 ? 0 : __is_same(T, bf16_t) ? 16 : 13;       // bits that the type's values do not use
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // sum over the waves of a number each has; f(waves before this one)
+    const auto total = [&](int mine, int& before) {
+        before = 0;
+        if constexpr (NW == 1) return mine;
+        __syncthreads();
+        if (lane == 0) tally[wave] = mine;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            before += w < wave ? tally[w] : 0;
+            all += tally[w];
+        }
+        return all;
+    };
+    const auto above = [&](float t) {                        // elements >= t
+        int c = (int)__popcll(__ballot(tid < ntail && xt >= t)), before;
+        for (int v0 = 0; v0 < nv; v0 += NT) {
+            const bool in = v0 + tid < nv;
+            u32x4_t r{};
+            if (in) r = tok_ld16<T>(x + (int64_t)(v0 + tid) * VEC);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) c += (int)__popcll(__ballot(in && TokElem<T>::get(r, e) >= t));
+        }
+        return total(c, before);
+    };
+    constexpr uint32_t NONE = 0x007fffffu;                   // -inf in the order of floats
+    float ge, gt;                                            // equal: >= ge and not >= gt; larger: >= gt
+    int larger;
+    if (n >= (float)k) {
+        ge = m;
+        gt = INFINITY;
+        larger = 0;
+    } else {
+        ge = -INFINITY;
+        gt = tok_unorder(NONE + 1);
+        larger = above(gt);
+        if (larger > CAND) {
+            uint32_t t = 0;
+            for (int bit = 31; bit >= LOW && larger > CAND; --bit) {
+                const uint32_t c = t | 1u << bit;
+                const int have = c <= NONE ? larger : above(tok_unorder(c));
+                if (have >= k) {
+                    t = c;
+                    larger = have;
+                }
+            }
+            ge = gt = tok_unorder(t);
+            if (larger > CAND) {                             // equal ones at t: as many as there are
+                gt = tok_unorder(t + (1u << LOW));
+                larger = above(gt);
+            }
+        }
+    }
+    __syncthreads();
+    if (tid == 0) *ncand = 0;
+    __syncthreads();
+    const int need = k - larger;                             // of the equal ones
+    int ties = 0;
+    const auto chunk = [&](const float* f, int have, int at) {
+        uint32_t eq = 0;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const bool in = e < have, big = in && f[e] >= gt;
+            if (in && !big && f[e] >= ge) eq |= 1u << e;
+            if (larger && __ballot(big)) {
+                if (big) cand[atomicAdd(ncand, 1)] = tok_key(f[e], at + e);        // up to CAND
+            }
+        }
+        if (ties < need) {
+            const int mine = __popc(eq);
+            int below = 0, all = 0, before;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint64_t mask = __ballot((mine >> b) & 1);
+                below += tok_below(mask) << b;
+                all += (int)__popcll(mask) << b;
+            }
+            all = total(all, before);
+            int rank = ties + before + below;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if ((eq >> e) & 1) {
+                    if (rank < need) emit(larger + rank, tok_key(f[e], at + e));
+                    ++rank;
+                }
+            ties += all;
+        }
+    };
+    float f[VEC];
+    for (int v0 = 0; v0 < nv && (larger || ties < need); v0 += NT) {
+        const int v = v0 + tid;
+        u32x4_t r{};
+        if (v < nv) r = tok_ld16<T>(x + (int64_t)v * VEC);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = TokElem<T>::get(r, e);
+        chunk(f, v < nv ? VEC : 0, e0 + v * VEC);
+    }
+    f[0] = xt;
+    chunk(f, tid < ntail ? 1 : 0, e0 + nv * VEC + tid);
+    __syncthreads();
+    tok_rank<NT>(cand, larger, k, emit);
+    return need > 0 ? larger + min(ties, need) : k;
+}
+
 template <typename T, int NT, int NV>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4 : 5))) void tok_score_kernel(ScoreArgs a) {
     constexpr int VEC = TokElem<T>::VEC, NW = NT / 64;
-    // one-wave rows: 8 KB of lists a block, or LDS would keep waves away
+    // one-wave rows: 6 KB of lists a block, or LDS would keep waves away
     constexpr int SPECIAL = NT == 64 ? 192 : NT == 256 ? 128 : 64;     // vectors a wave
-    constexpr int CAND = NT == 64 ? 512 : 1024;
+    constexpr int CAND = NT == 64 ? 256 : 1024;       // one wave: what it can sort
     __shared__ float red[NW][3];
-    __shared__ uint64_t best[NW];
+    __shared__ int tally[NW];
     __shared__ TokSpecial<SPECIAL> lists[NW];
     __shared__ __attribute__((aligned(16))) uint64_t cand[CAND];
     __shared__ int ncand;                                    // over CAND: some list did not fit
@@ -266,55 +383,23 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
         a.part[u] = make_float4(m, n, S, W);
     if (a.k) {
         int done = 0;
-        if (!(S == S)) {
-            // a row (or segment) with a NaN or +inf logit has no ranking
-        } else if (!slow) {
-            done = nc < a.k ? nc : a.k;
-            tok_rank<NT>(cand, nc, a.k, [&](int rank, uint64_t key) {
-                if (a.nseg == 1) {
-                    a.ids[row * a.k + rank] = tok_key_index(key);
-                    a.top[row * a.k + rank] = score_toplp(a, tok_key_value(key), m, lnS);
-                } else {
-                    a.keys[u * a.k + rank] = key;
-                }
-            });
-        } else {
-            // k rounds of the largest key below the last one, read again (L2); an exhausted segment yields key 0
-            uint64_t last = ~0ull;
-            for (done = 0; done < a.k; ++done) {
-                uint64_t bk = 0;
-                for (int v = tid; v < nv; v += NT) {
-                    const u32x4_t r = tok_ld16<T>(x + (int64_t)v * VEC);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const uint64_t key = tok_key(TokElem<T>::get(r, e), e0 + v * VEC + e);
-                        if (key < last && key > bk) bk = key;
-                    }
-                }
-                if (tid < ntail) {
-                    const uint64_t key = tok_key(s.xt, e0 + nv * VEC + tid);
-                    if (key < last && key > bk) bk = key;
-                }
-                bk = tok_group<64, TokTop>(bk);
-                if (lane == 0) best[wave] = bk;
-                __syncthreads();
-                bk = best[0];
-#pragma unroll
-                for (int w = 1; w < NW; ++w) bk = best[w] > bk ? best[w] : bk;
-                __syncthreads();
-                if (bk == 0) break;
-                last = bk;
-                if (tid == 0) {
-                    if (a.nseg == 1) {
-                        a.ids[row * a.k + done] = tok_key_index(bk);
-                        a.top[row * a.k + done] = score_toplp(a, tok_key_value(bk), m, lnS);
-                    } else {
-                        a.keys[u * a.k + done] = bk;
-                    }
-                }
+        const auto emit = [&](int rank, uint64_t key) {
+            if (a.nseg == 1) {
+                a.ids[row * a.k + rank] = tok_key_index(key);
+                a.top[row * a.k + rank] = score_toplp(a, tok_key_value(key), m, lnS);
+            } else {
+                a.keys[u * a.k + rank] = key;
+            }
+        };
+        if (S == S) {                                        // a row (or segment) with a NaN or +inf logit has no ranking
+            if (slow) {
+                done = score_select<T, NT, CAND>(x, nv, ntail, s.xt, e0, a.k, m, n, cand, &ncand, tally, emit);
+            } else {
+                done = nc < a.k ? nc : a.k;
+                tok_rank<NT>(cand, nc, a.k, emit);
             }
         }
-        for (int j = done + tid; j < a.k; j += NT) {     // fewer than k elements
+        for (int j = done + tid; j < a.k; j += NT) {         // fewer than k elements
             if (a.nseg == 1) {
                 a.ids[row * a.k + j] = -1;
                 a.top[row * a.k + j] = NAN;

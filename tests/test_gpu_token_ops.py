@@ -163,6 +163,23 @@ def test_score_ties_go_to_the_lowest_index(V, kind):
     _check_score(x, torch.tensor([0, V - 1, V // 2]), 1.0, k)
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("second", [1.5, 0.0, -0.0, -2.0, -1000.0])
+def test_score_ties_below_the_maximum(second, dtype):
+    """A few elements at the top, very many or some hundreds equal ones next: what the lists do not hold is found by counting."""
+    for V in (300, 700, 1030, 4091, 5000, 33333, 140001):
+        for tied in (V // 2, min(V // 2, 650)):
+            g = torch.Generator().manual_seed(V + tied)
+            x = torch.randn(3, V, generator=g).abs().neg() * 8 + second - 4
+            at = torch.rand(3, V, generator=g).argsort(-1)
+            x.scatter_(1, at[:, :tied], second)
+            x.scatter_(1, at[:, tied:tied + 5], torch.arange(5.0).expand(3, 5) + 4)
+            x[2, at[2, -9:]] = -math.inf
+            print(V, tied, second, dtype, flush=True)
+            _check_score(x.to(DTYPES[dtype]), at[:, 0], 1.0, 20, grad=False)
+            _check_score(x.to(DTYPES[dtype]), at[:, 0], 1.0, 100, grad=False)
+
+
 @pytest.mark.parametrize("V,k", [(200000, 128), (600000, 100), (600000, 3)])
 def test_score_segments_that_share_or_lack_the_top(V, k):
     """Long rows in which the alternatives of all segments lie across each other, in which most segments are ruled out, in
