@@ -14,7 +14,7 @@
 // their elements at or above it are ranked: no data-dependent loop.  Where the lists overflow (thousands of equal values) or fewer
 // than k elements are left (masks), the k-th value is found by counting instead (score_select), the row read again from L2.
 // Narrow rows (V <= 512, the autoencoder's vocabulary): 8 to 64 lanes a row with 8 elements each; the lane's 8 keys are
-// sorted by a network and k rounds take the best head of the group.
+// sorted by a network, and k rounds take the best head of the group or, for many alternatives, merges sort the row.
 #include "token.h"
 
 struct ScoreArgs {
@@ -79,11 +79,12 @@ struct ScoreSums {
     }
 };
 
-// One wave, many alternatives: k lanes' maxima would be a poor bound (of 64 lanes the lowest one).  A value that some 1.25 k elements
-// should reach, were they spread evenly -- the kj-th largest of the lanes' maxima -- is put right by counting the row's elements
-// at or above it: k to `cap` of them are looked for, by steps and bisection.  -inf, or more than cap, where 16 counts do not find
-// such a value.
-template <typename SEG> __device__ __forceinline__ float tok_counted_bound(const SEG& s, float tm, float m, int k, int kj, int cap) {
+// One wave, many alternatives: k lanes' maxima would be a poor bound (of 64 lanes the lowest one).  A value that some 1.25 k
+// elements should reach, were they spread evenly -- the kj-th largest of the lanes' maxima -- is put right by counting the row's
+// elements at or above it: k to `cap` of them are looked for, by steps and bisection.  -inf, or more than cap, where 16 counts
+// do not find such a value.
+template <typename SEG>
+__device__ __forceinline__ float tok_counted_bound(const SEG& s, float tm, float m, int k, int kj, int cap) {
     float B = tok_kth_bound(tm, kj), lo = -INFINITY, hi = m;
     if (!(m < INFINITY)) return -INFINITY;
     if (B == -INFINITY) B = tok_group<64, TokMin>(tm > -INFINITY ? tm : m);
@@ -113,12 +114,12 @@ template <typename SEG> __device__ __forceinline__ float tok_counted_bound(const
 // 32,000 bf16 logits of which 10 are not masked, k = 64: 25 us; k rounds of a block-wide maximum, the next smaller key each, took
 // 320; 20,000 equal rows of 1,000 fp32, k = 20: 37 and 190.  Returns how many there are.
 template <typename T, int NT, int CAND, typename F>
-__device__ __forceinline__ int score_select(tok_in<T> x, int nv, int ntail, float xt, int e0, int k, float m, float n, uint64_t* cand,
-                                         int* ncand, int* tally, const F& emit) {
+__device__ __forceinline__ int score_select(tok_in<T> x, int nv, int ntail, float xt, int e0, int k, float m, float n,
+                                            uint64_t* cand, int* ncand, int* tally, const F& emit) {
     constexpr int VEC = TokElem<T>::VEC, NW = NT / 64;
     constexpr int LOW = sizeof(T) == 4 ? 0 : __is_same(T, bf16_t) ? 16 : 13;       // bits that the type's values do not use
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // sum over the waves of a number each has; f(waves before this one)
+    // the sum of a number that each wave has; before: of the waves below this one
     const auto total = [&](int mine, int& before) {
         before = 0;
         if constexpr (NW == 1) return mine;
@@ -265,7 +266,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NV == 16 ? 4
     if (a.k > 1) {
         // this wave's share of the bound
         if constexpr (NW > 1) wb = tok_kth_bound(tm, (a.k + NW - 1) / NW);
-        else wb = a.kj == 0 ? tok_kth_bound(tm, a.k) : tok_counted_bound(s, tm, wm0, a.k, a.kj, min(a.k + (a.k >> 1) + 16, SPECIAL));
+        else if (a.kj == 0) wb = tok_kth_bound(tm, a.k);
+        else wb = tok_counted_bound(s, tm, wm0, a.k, a.kj, min(a.k + (a.k >> 1) + 16, SPECIAL));
     }
     if (lane == 0) {
         red[wave][0] = wm0;
@@ -547,9 +549,9 @@ template <> struct NarrowKey<float> {
     static __device__ __forceinline__ int index(uint64_t k) { return tok_key_index(k); }
     static __device__ __forceinline__ float value(uint64_t k) { return tok_key_value(k); }
 };
-// Up to this many alternatives of a narrow row by rounds of the group's best head, more by sorting the row (120,000 rows of 40 fp32
-// logits: k = 12 27 us, sorted 29; k = 20 36 and 30; k = 40 56 and 30.  Of 200: k = 20 136 and 148, k = 40 232 and 144).  Groups of 64
-// lanes get no more than score_narrow_takes lets through.
+// Up to this many alternatives of a narrow row by rounds of the group's best head, more by sorting the row (120,000 rows of 40
+// fp32 logits: k = 12 27 us, sorted 29; k = 20 36 and 30; k = 40 56 and 30.  Of 200: k = 20 136 and 148, k = 40 232 and 144).
+// Groups of 64 lanes get no more than score_narrow_takes lets through.
 template <int G> constexpr int NARROW_ROUNDS = G == 8 ? 16 : G == 16 ? 20 : 24;
 
 template <typename T, int G>
@@ -837,7 +839,8 @@ __global__ __launch_bounds__(256) void tok_score_grad_narrow_kernel(ScoreGradArg
 static TokPlan score_plan(int64_t V, int dtype) { return tok_plan(V, tok_esize(dtype), 8192); }
 
 // Up to this many alternatives of a row on one wave by the lanes' maxima, more by a counted bound (120,000 rows of 1,000 fp32
-// logits: k = 20 182 us, counted 198; k = 32 250 and 247; k = 64 1,390 and 337; k = 100 4,540 and 482, before the candidates were sorted)
+// logits, before the candidates were sorted: k = 20 182 us, counted 198; k = 32 250 and 247; k = 64 1,390 and 337; k = 100 4,540
+// and 482)
 constexpr int ONE_WAVE_LANES = 24;
 
 // Rows of 257 to 512 elements with alternatives: a row a wave by the long rows' kernel where listing candidates costs less than

@@ -125,12 +125,12 @@ def test_score_top_k(V, k, dtype):
 MANY_KINDS = {
     "normal": lambda V, g: torch.randn(6, V, generator=g) * 2.5,
     "ascending": lambda V, g: (torch.arange(V) / V * 8).expand(6, V).clone(),
-    "one_block": lambda V, g: torch.where((torch.arange(V) // 16) % 9 == 0, torch.randn(6, V, generator=g) + 9, torch.randn(6, V, generator=g)),
+    "one_block": lambda V, g: torch.randn(6, V, generator=g) + torch.where((torch.arange(V) // 16) % 9 == 0, 9.0, 0.0),
     "few_values": lambda V, g: torch.randint(0, 5, (6, V), generator=g).float(),
     "heavy_tail": lambda V, g: torch.randn(6, V, generator=g) / torch.rand(6, V, generator=g).clamp_min(1e-3) - 20,
     "few_left": lambda V, g: torch.where(torch.rand(6, V, generator=g) < 0.05, torch.randn(6, V, generator=g), -math.inf),
     "half_left": lambda V, g: torch.where(torch.arange(V) < V // 2, torch.randn(6, V, generator=g), -math.inf),
-    "lowest": lambda V, g: torch.where(torch.rand(6, V, generator=g) < 0.5, torch.randn(6, V, generator=g), torch.finfo(torch.float16).min),
+    "lowest": lambda V, g: torch.where(torch.rand(6, V, generator=g) < 0.5, torch.randn(6, V, generator=g), -65504.0),
 }
 
 
