@@ -293,13 +293,14 @@ template <int E, typename F> __device__ __forceinline__ void tok_sort_list(const
 
 // The k largest of a list by counting or, where it is long, by the first wave's sort: one wave a row sorts from 17 keys on (120,000
 // rows of 1,000 fp32 logits, k = 64: 234 us, counting 337; k = 4: 160 and 146), blocks of more waves from 97 on (5,000 rows of
-// 6,000 fp32 logits, k = 100: 41 us, counting 50; k = 20: no difference).
+// 6,000 fp32 logits, k = 100: 41 us, counting 50; k = 20: no difference; 48 of 128,001 bf16, k = 128, some 300 keys: 18 and 24).
 template <int NT, typename F> __device__ __forceinline__ void tok_rank(const uint64_t* keys, int n, int k, const F& f) {
-    if (n > (NT == 64 ? 16 : 96) && n <= 256) {
+    if (n > (NT == 64 ? 16 : 96) && n <= (NT == 64 ? 256 : 512)) {
         if (NT > 64 && threadIdx.x >= 64) return;
         if (NT == 64 && n <= 64) tok_sort_list<1>(keys, n, k, f);
         else if (n <= 128) tok_sort_list<2>(keys, n, k, f);
-        else tok_sort_list<4>(keys, n, k, f);
+        else if (n <= 256) tok_sort_list<4>(keys, n, k, f);
+        else if constexpr (NT > 64) tok_sort_list<8>(keys, n, k, f);
     } else {
         tok_count_ranks<NT>(keys, n, k, f);
     }
