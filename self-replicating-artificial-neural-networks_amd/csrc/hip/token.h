@@ -314,13 +314,14 @@ __device__ __forceinline__ int64_t tok_int(int64_t base, int is64, int64_t i) {
     return is64 ? ((tok_in<int64_t>)base)[i] : (int64_t)((tok_in<int32_t>)base)[i];
 }
 
-// A row's exponents, d = fma(x, c, -mc).  Where |m| c is near overflow (a row of the type's lowest values), two different
-// logits lie so far apart that only those equal to m count: everything else gets -inf.
+// A row's exponents, d = fma(x, c, -mc).  dmax is up to half a step of mc: 2^6 below |m| c = 2^31, so that 2^-dmax stays finite,
+// and any number of octaves above it.  But from 2^31 on two different fp32 logits lie at least 2^31 2^-24 = 128 octaves apart, so
+// only those equal to m count there: everything else gets -inf, and dmax is 0.
 struct TokRef {
     float c, mc, dmax, meq;      // meq: the value of the elements to count (a NaN, equal to nothing, in a row of -inf)
 };
 __device__ __forceinline__ TokRef tok_ref(float m, float c) {
-    const bool none = m == -INFINITY, big = !none && fabsf(m) * c >= 1e37f;
+    const bool none = m == -INFINITY, big = !none && fabsf(m) * c >= 2147483648.f;
     TokRef r;
     r.c = big ? 1e-30f : c;
     r.mc = none ? 0.f : big ? INFINITY : m * c;

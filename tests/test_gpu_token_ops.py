@@ -687,3 +687,31 @@ def test_far_offsets_in_a_large_tensor():
     assert float((loss[-4:] - l4).abs().max()) <= 2 * O.sum_error(x, 1.0) + 4 * O.U * float(l4.max())
     assert float(dx[:-4].abs().amax()) == 0
     assert float((dx[-4:].float() - d4.float()).abs().max()) <= 2 ** -7
+
+
+# ---- rows of large finite values --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,values,T", [
+    ("fp32", (1e10, -1e10, 1e12, -1e12, 1e20, -1e20, 1e30, -1e30), 1.0),
+    ("fp32", (1e10, -1e10, 1e12, -1e12, 1e20, -1e20, 1e30, -1e30), 0.7),
+    ("fp32", (3e9, -3e9, 1e9, -1e9, 2.1e9, -2.1e9, 1e20, -1e20), 0.8),
+    ("bf16", (1e10, -1e10, 1e12, -1e12, 1e20, -1e20, 1e30, -1e30), 1.0),
+    ("bf16", (1e9, -1e9, 1.4e9, -1.4e9, 1e20, -1e20, 1e30, -1e30), 0.8),
+    ("fp16", (65504.0, -65504.0, 60000.0, -60000.0, 30000.0, -30000.0, 777.0, -777.0), 1e-4)])
+@pytest.mark.parametrize("V,tile", [(40, 1), (40, 4100), (100, 1), (300, 1), (700, 1), (5000, 1), (70001, 1), (140001, 1)])
+def test_rows_of_large_finite_values(V, tile, dtype, values, T):
+    """A row filled with one large value is uniform, one with a larger element is sure of it, whatever rounding m c takes."""
+    x = torch.tensor(values).to(DTYPES[dtype])[:, None].repeat(2, V)
+    n = len(values)
+    at = torch.arange(2 * n) % V
+    step = x[n:, 0].double() * (1 + 2.0 ** (-7 if dtype == "bf16" else -10 if dtype == "fp16" else -20))
+    up = torch.maximum(step, (2 - step / x[n:, 0].double()) * x[n:, 0].double()).to(x.dtype)      # towards plus infinity
+    if dtype == "fp16":
+        x[n], up[0] = 60000.0, 65504.0
+    assert (up > x[n:, 0]).all() and up.isfinite().all()
+    x[n:, V // 2] = up
+    _check_score(x, at, T, min(V, 6), tile=tile)
+    ids = torch.stack([at, (at + 1) % V, torch.full_like(at, V // 2)], 1)
+    t = torch.log_softmax(torch.randn(2 * n, 5, generator=torch.Generator().manual_seed(V)), -1)[:, :3].contiguous()
+    ids[:, 2] = torch.where(ids[:, :2].eq(V // 2).any(-1), -1, ids[:, 2])
+    for tail in ("drop", "bucket"):
+        _check_distill(x, ids, t, T, tail, None, tile=tile)
