@@ -4,10 +4,16 @@
 // same id add up.  With z = x / T, q = softmax(z):
 //   drop  : p_k = exp(t_k) / sum_k exp(t_k)                                   loss = w T^2 sum_k p_k (ln p_k - ln q_ik)
 //   bucket: p_k = exp(t_k), p_0 = max(0, 1 - sum p_k), q_0 = sum_{v not listed} q_v,
-//           loss = w T^2 ( sum_k p_k (ln p_k - ln q_ik) + p_0 (ln p_0 - ln q_0) )       (no bucket where q_0 = 0)
-//   gradient, with P = sum p_k, A = P + p_0, B = A - p_0 / q_0 (drop: A = B = P):
-//           dx_v = w T ( A q_v - p_v ) for listed v,   w T B q_v for the others
+//           loss = w T^2 ( sum_k p_k (ln p_k - ln q_ik) + p_0 (ln p_0 - ln q_0) )       (no bucket where ln q_0 < -745)
+//   gradient, with P = sum p_k, A = P + p_0 (drop: A = P):
+//           dx_v = w T ( A q_v - p_v ) for listed v,   w T (A q_0 - p_0) (q_v / q_0) for the others (drop: w T P q_v)
 // A row of weight 0 is not read: loss and gradient 0.
+//
+// A student may be so sure of its list that q_0 is nothing in fp32 (88 T below the row's maximum), and that is where the bucket
+// has most to say.  So q_0 has a reference of its own, mu: the row's maximum m while the sum relative to it is 2^-64 or more (what
+// underflows then, 2^-126 an element, does not count), else the largest unlisted element, in a second look that only such rows
+// take.  ln q_0 = (mu - m) / T + ln rest - ln sum, and q_v / q_0 = exp((x_v - mu) / T) / rest.  Below exp(-745), where 64 bits end,
+// the rest counts as ruled out (a finite mask value), as -inf does.
 //
 // The loss of a good student is a small difference of large terms (its digits go with the rounding of ln sum alone), so a
 // row's sums are fp32 but its logarithms and K terms fp64: K + 3 transcendentals a row, next to V fp32 ones.
@@ -30,9 +36,9 @@ struct DistArgs {
     float T;
     float* loss;
     int64_t dx;           // [rows][V], one-pass form
-    float4* stat;         // (m, log2 sum, A, B) for the gradient launch
-    float* pk;            // [rows][K]: the entry's p (its first occurrence carries the sum), -1: skip
-    float4* part;         // nseg > 1: (m, n, S, -) of each segment; bucket: over unlisted elements, m over all
+    float4* stat;         // for the gradient launch, two a row: (m, l2S, A, -) and (mu, l2u, B, -) of DistRow
+    float* pk;            // [rows][K]: p of the entry's token
+    float4* part;         // nseg > 1: (mu, n, S, m) of each segment: its sums relative to mu (bucket: of the unlisted), its maximum
 };
 
 // The K entries of a row in LDS: id (-1: absent), the student's logit there, p
@@ -41,8 +47,10 @@ struct DistEntries {
     float x[DIST_MAX_K], t[DIST_MAX_K], p[DIST_MAX_K];
 };
 struct DistRow {
-    float m, l2S, A, B;
+    float m, l2S, A;      // listed: A q - p, log2 q = (x - m) c - l2S
+    float mu, l2u, B;     // others: B exp2((x - mu) c - l2u)
 };
+constexpr float DIST_FAR = 0x1p-64f;      // a rest below this, relative to the row's maximum, takes a reference of its own
 
 __device__ __forceinline__ double group_sum64(double v) { return tok_group<64, TokSum>(v); }
 
@@ -57,54 +65,77 @@ struct DistTeach {
         if (e != 0.0) acc += e * (l - (x == -INFINITY ? -(double)INFINITY : ((double)x - (double)m) * inv_t));
     }
 };
-// A row's loss and the gradient's factors.  rest / listed: the student's sums relative to m over the elements outside / inside
-// the list (drop mode: their sum counts).  shift: ln p_k = t_k - shift.
+// A row's loss and the gradient's factors.  rest: the student's sum over the elements outside the list relative to mu (mu = m where
+// there is nothing), listed: inside it, relative to m (drop mode: their sum counts, mu = m).  shift: ln p_k = t_k - shift.
 struct DistDone {
     DistRow d;
     double kl, shift;
     bool none;
 };
-__device__ __forceinline__ DistDone dist_finish(const DistArgs& a, float m, double rest, double listed, double tot, double acc,
-                                                float s) {
+__device__ __forceinline__ DistDone dist_finish(const DistArgs& a, float m, float mu, double rest, double listed, double tot,
+                                                double acc, float s) {
     DistDone r;
-    double sum = rest + listed;
+    double far = 0.0, rm = rest;                             // (mu - m) / T, the rest relative to m
+    if (__builtin_expect(__ballot(mu != m) != 0, 0)) {
+        far = mu == m ? 0.0 : ((double)mu - (double)m) * a.r.dinv_t;
+        rm = rest * exp(far);
+    }
+    double sum = rm + listed;
     if (m == INFINITY) sum = (double)NAN;
     r.none = sum == 0.0;                                     // nothing left of the student: infinite loss, no gradient
     const double lnS = r.none ? 0.0 : log(sum);
-    double P, A, B;
+    r.d.m = r.d.mu = r.none ? 0.f : m;
+    r.d.l2S = r.d.l2u = r.none ? INFINITY : (float)(lnS * 1.4426950408889634);
     if (a.bucket) {
         r.shift = 0.0;
-        P = tot;
         r.kl = acc + (tot != 0.0 ? tot * lnS : 0.0);
-        A = B = P;
-        const double p0 = rest == 0.0 ? 0.0 : 1.0 - P;
-        if (p0 > 0.0) {
-            const double lq0 = listed < rest ? log1p(-listed / sum) : log(rest / sum);
+        r.d.A = r.d.B = (float)tot;
+        const double p0 = 1.0 - tot;
+        const double lq0 = sum != sum ? sum : rest == 0.0 ? -(double)INFINITY
+                           : listed < rm ? log1p(-listed / sum) : far + log(rest / sum);
+        if (p0 > 0.0 && !(lq0 < -745.0)) {
             r.kl += p0 * (log(p0) - lq0);
-            A = P + p0;
-            B = A - p0 * (sum / rest);
+            r.d.A = (float)(tot + p0);
+            r.d.B = (float)((tot + p0) * (rm / sum) - p0);
+            r.d.mu = mu;
+            r.d.l2u = log2f((float)rest);
         }
     } else {
         const double lt = tot == 0.0 ? 0.0 : log(tot);
         r.shift = (tot == 0.0 ? 0.0 : (double)s) + lt;
         r.kl = tot == 0.0 ? 0.0 : acc / tot - lt + lnS;
-        A = B = tot == 0.0 ? 0.0 : 1.0 + (tot - tot);        // NaN stays NaN
+        r.d.A = r.d.B = (float)(tot == 0.0 ? 0.0 : 1.0 + (tot - tot));        // NaN stays NaN
     }
-    r.d.m = r.none ? 0.f : m;
-    r.d.l2S = r.none ? INFINITY : (float)(lnS * 1.4426950408889634);
-    r.d.A = (float)A;
-    r.d.B = (float)B;
     return r;
+}
+__device__ __forceinline__ float dist_q(const DistRow& d, float c, float x) {
+    return tok_exp2(__builtin_fmaf(x - d.m, c, -d.l2S));
+}
+// an element outside the list, B still to be multiplied
+__device__ __forceinline__ float dist_u(const DistRow& d, float c, float x) {
+    return tok_exp2(__builtin_fmaf(x - d.mu, c, -d.l2u));
+}
+__device__ __forceinline__ void dist_keep(float4* stat, int64_t row, const DistRow& d) {
+    stat[2 * row] = make_float4(d.m, d.l2S, d.A, 0.f);
+    stat[2 * row + 1] = make_float4(d.mu, d.l2u, d.B, 0.f);
+}
+__device__ __forceinline__ DistRow dist_kept(const float4* stat, int64_t row) {
+    const float4 l = stat[2 * row], u = stat[2 * row + 1];
+    return DistRow{l.x, l.y, l.z, u.x, u.y, u.z};
+}
+// a listed element's A q - p; nothing where the student has nothing left
+__device__ __forceinline__ float dist_l(const DistRow& d, float c, float x, float p) {
+    return d.l2S == INFINITY ? 0.f : __builtin_fmaf(d.A, dist_q(d, c, x), -p);
 }
 // an entry's p for the gradient, in fp32
 __device__ __forceinline__ float dist_p(float t, double shift) {
     return tok_exp2((float)(((double)t - shift) * 1.4426950408889634));
 }
 
-// The first wave's work on a row: the loss, and each entry's p.  n, S: the student's sums relative to m over all elements, or
-// in bucket mode over the unlisted ones.  dup: some id may occur twice; the first occurrence carries the sum then.
-__device__ __forceinline__ DistRow dist_epilogue(const DistArgs& a, DistEntries& E, int64_t row, float w, float m, float n,
-                                                 float S, bool dup, int lane) {
+// The first wave's work on a row: the loss, and each entry's p.  n, S: the student's sums relative to mu over all elements, or
+// in bucket mode over the unlisted ones.  dup: some id may occur twice; each occurrence has the whole p then.
+__device__ __forceinline__ DistRow dist_epilogue(const DistArgs& a, DistEntries& E, int64_t row, float w, float m,
+                                                 float mu, float n, float S, bool dup, int lane) {
     const int K = a.K;
     float s = -INFINITY;
     if (!a.bucket) {
@@ -133,40 +164,36 @@ __device__ __forceinline__ DistRow dist_epilogue(const DistArgs& a, DistEntries&
     }
     nl = tok_group<64, TokSum>(nl);
     Sl = tok_group<64, TokSum>(Sl);
-    const DistDone r = dist_finish(a, m, (double)n + (double)S, (double)nl + (double)Sl, te.tot, te.acc, s);
+    const DistDone r = dist_finish(a, m, mu, (double)n + (double)S, (double)nl + (double)Sl, te.tot, te.acc, s);
     for (int j = lane; j < K; j += 64) E.p[j] = dist_p(E.t[j], r.shift);
-    if (dup) {
+    bool twice = false;
+#pragma unroll
+    for (int q = 0; q < DIST_MAX_K / 64; ++q) {
+        const int j = q * 64 + lane;
+        twice |= j < K && E.id[j] >= 0 && !first[q];
+    }
+    if (__ballot(twice)) {
         tok_wave_fence();
         float sum[DIST_MAX_K / 64];
 #pragma unroll
         for (int q = 0; q < DIST_MAX_K / 64; ++q) {
             const int j = q * 64 + lane;
             sum[q] = 0.f;
-            if (first[q])
-                for (int i = j; i < K; ++i) sum[q] += E.id[i] == E.id[j] ? E.p[i] : 0.f;
+            if (j < K)
+                for (int i = 0; i < K; ++i) sum[q] += E.id[i] == E.id[j] ? E.p[i] : 0.f;
         }
         tok_wave_fence();
 #pragma unroll
         for (int q = 0; q < DIST_MAX_K / 64; ++q)
             if (q * 64 + lane < K) E.p[q * 64 + lane] = sum[q];
     }
-#pragma unroll
-    for (int q = 0; q < DIST_MAX_K / 64; ++q) {
-        const int j = q * 64 + lane;
-        if (j < K) {
-            if (!first[q] || r.none) E.p[j] = -1.f;
-            if (a.pk) a.pk[row * K + j] = E.p[j];
-        }
-    }
+    if (a.pk)
+        for (int j = lane; j < K; j += 64) a.pk[row * K + j] = E.p[j];
     if (lane == 0) {
         a.loss[row] = (float)((double)w * (double)a.T * (double)a.T * r.kl);
-        if (a.stat) a.stat[row] = make_float4(r.d.m, r.d.l2S, r.d.A, r.d.B);
+        if (a.stat) dist_keep(a.stat, row, r.d);
     }
     return r.d;
-}
-
-__device__ __forceinline__ float dist_q(const DistRow& d, float c, float x) {
-    return tok_exp2(__builtin_fmaf(x - d.m, c, -d.l2S));
 }
 
 template <typename T> __device__ __forceinline__ void dist_load_entry(const DistArgs& a, DistEntries& E, int64_t row, tok_in<T> x,
@@ -186,6 +213,23 @@ struct DistSums {
         n += is && !skip ? 1.f : 0.f;
     }
 };
+
+// f(element) over a thread's elements of a segment that no bit marks, read again.  Element by element in a loop: unrolled, its masks
+// would take the scalar registers of a wave from the kernel that this is the rare part of (8,192 x 8,000 bf16, K = 64: 69 us, 65).
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void dist_unlisted(tok_in<T> x, int nv, const uint32_t* bits, const F& f) {
+    constexpr int VEC = TokElem<T>::VEC;
+    for (int v = threadIdx.x; v < nv; v += NT) {
+        u32x4_t r = tok_ld16<T>(x + (int64_t)v * VEC);
+        uint32_t listed = bits[(v * VEC) >> 5] >> ((v * VEC) & 31);                  // a vector's bits lie in one word
+#pragma unroll 1
+        for (int e = 0; e < VEC; ++e, listed >>= 1) {
+            if (!(listed & 1)) f(TokElem<T>::get(r, 0));
+            if constexpr (VEC == 4) r = u32x4_t{r[1], r[2], r[3], 0};
+            else r = u32x4_t{r[0] >> 16 | r[1] << 16, r[1] >> 16 | r[2] << 16, r[2] >> 16 | r[3] << 16, r[3] >> 16};
+        }
+    }
+}
 
 template <typename T, int NT, int NV, bool GRAD>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void tok_distill_kernel(DistArgs a) {
@@ -208,10 +252,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void to
     const float w = a.w ? a.w[row] : 1.f;
     tok_out<T> o = (tok_out<T>)a.dx + row * a.r.V;
     if (w == 0.f) {
-        if (a.nseg == 1 && tid == 0) {
-            a.loss[row] = 0.f;
-            if (a.stat) a.stat[row] = make_float4(0.f, INFINITY, 0.f, 0.f);
-        }
+        if (a.nseg == 1 && tid == 0) a.loss[row] = 0.f;
         if constexpr (GRAD) {
             for (int v = tid; v < nvec_row; v += NT) tok_st16<T>(o + (int64_t)v * VEC, u32x4_t{0, 0, 0, 0});
             if (tid < ntail_row) o[nvec_row * VEC + tid] = TokElem<T>::put(0.f);
@@ -291,18 +332,49 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void to
         red[wave][2] = n1;
     }
     __syncthreads();
-    if (wave == 0) {
-        float S = red[0][1], n = red[0][2];
+    float S = red[0][1], n = red[0][2], mu = m;
+#pragma unroll
+    for (int k = 1; k < NW; ++k) {
+        S += red[k][1];
+        n += red[k][2];
+    }
+    S *= tok_exp2(-ref.dmax);
+    if (__builtin_expect(a.bucket && n + S < DIST_FAR, 0)) {                     // the second look at the unlisted elements
+        const bool tail = tid < ntail && !((bits[nv * VEC / 32] >> ((nv * VEC + tid) & 31)) & 1);
+        float um = tail ? s.xt : -INFINITY;
+        dist_unlisted<T, NT>(x + e0, nv, bits, [&](float f) { um = tok_max(um, f); });
+        um = tok_group<64, TokMax>(um);
+        if (lane == 0) red[wave][0] = um;
+        __syncthreads();
+        um = red[0][0];
+#pragma unroll
+        for (int k = 1; k < NW; ++k) um = tok_max(um, red[k][0]);
+        const TokRef ru = tok_ref(um, a.r.c);
+        sum = DistSums{0.f, 0.f};
+        dist_unlisted<T, NT>(x + e0, nv, bits, [&](float f) { sum.add(f, ru, false); });
+        if (tail) sum.add(s.xt, ru, false);
+        S = tok_group<64, TokSum>(sum.S);
+        n = tok_group<64, TokSum>(sum.n);
+        if (lane == 0) {
+            red[wave][1] = S;
+            red[wave][2] = n;
+        }
+        __syncthreads();
+        S = red[0][1];
+        n = red[0][2];
 #pragma unroll
         for (int k = 1; k < NW; ++k) {
             S += red[k][1];
             n += red[k][2];
         }
-        S *= tok_exp2(-ref.dmax);
+        S *= tok_exp2(-ru.dmax);
+        if (um > -INFINITY) mu = um;
+    }
+    if (wave == 0) {
         if (a.nseg > 1) {
-            if (lane == 0) a.part[u] = make_float4(m, n, S, 0.f);
+            if (lane == 0) a.part[u] = make_float4(mu, n, S, m);
         } else {
-            const DistRow d = dist_epilogue(a, E, row, w, m, n, S, dup != 0, lane);
+            const DistRow d = dist_epilogue(a, E, row, w, m, mu, n, S, dup != 0, lane);
             if (lane == 0) rowd = d;
         }
         // fp64 logarithms take as many registers as the row: this wave gives its part up and reads it again (L2)
@@ -318,16 +390,14 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void to
             if (i * NT + tid < nv) {
                 float g[VEC];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) g[e] = fB * dist_q(d, a.r.c, TokElem<T>::get(s.r[i], e));
+                for (int e = 0; e < VEC; ++e) g[e] = fB * dist_u(d, a.r.c, TokElem<T>::get(s.r[i], e));
                 tok_st16<T>(o + (int64_t)(i * NT + tid) * VEC, TokElem<T>::pack(g));
             }
         }
-        if (tid < ntail) o[nv * VEC + tid] = TokElem<T>::put(fB * dist_q(d, a.r.c, s.xt));
+        if (tid < ntail) o[nv * VEC + tid] = TokElem<T>::put(fB * dist_u(d, a.r.c, s.xt));
         __syncthreads();                                 // the listed tokens' stores follow the row's
-        for (int j = tid; j < a.K; j += NT) {
-            const float p = E.p[j];
-            if (E.id[j] >= 0 && p >= 0.f) o[E.id[j]] = TokElem<T>::put(f * (d.A * dist_q(d, a.r.c, E.x[j]) - p));
-        }
+        for (int j = tid; j < a.K; j += NT)
+            if (E.id[j] >= 0) o[E.id[j]] = TokElem<T>::put(f * dist_l(d, a.r.c, E.x[j], E.p[j]));
     }
 }
 
@@ -338,31 +408,33 @@ template <typename T> __global__ __launch_bounds__(64) void tok_distill_join_ker
     const int64_t row = a.r.u0 + blockIdx.x;
     const float w = a.w ? a.w[row] : 1.f;
     if (w == 0.f) {
-        if (lane == 0) {
-            a.loss[row] = 0.f;
-            if (a.stat) a.stat[row] = make_float4(0.f, INFINITY, 0.f, 0.f);
-        }
+        if (lane == 0) a.loss[row] = 0.f;
         return;
     }
     tok_in<T> x = tok_row<T>(a.r, row);
     for (int j = lane; j < a.K; j += 64) dist_load_entry<T>(a, E, row, x, j);
     const float4* part = a.part + row * a.nseg;
-    float m = -INFINITY;
-    for (int s = 0; s < a.nseg; ++s) m = tok_max(m, part[s].x);
+    float m = -INFINITY, mu = -INFINITY;                     // mu: the largest reference of a segment that has anything to sum
+    for (int s = 0; s < a.nseg; ++s) {
+        const float4 p = part[s];
+        m = tok_max(m, p.w);
+        if (p.y + p.z != 0.f) mu = tok_max(mu, p.x);
+    }
     float S = 0.f, n = 0.f;
     for (int s = 0; s < a.nseg; ++s) {
         const float4 p = part[s];
-        if (p.x == m) {
+        if (p.x == mu) {
             n += p.y;
             S += p.z;
-        } else if (p.x > -INFINITY) {
-            S += (p.y + p.z) * tok_exp2((p.x - m) * a.r.c);
+        } else if (p.x > -INFINITY && p.y + p.z != 0.f) {
+            S += (p.y + p.z) * tok_exp2((p.x - mu) * a.r.c);
         } else {
             S += p.z;
         }
     }
+    if (!(mu > -INFINITY)) mu = m;
     __syncthreads();
-    dist_epilogue(a, E, row, w, m, n, S, true, lane);
+    dist_epilogue(a, E, row, w, m, mu, n, S, true, lane);
     __syncthreads();
 }
 
@@ -370,9 +442,30 @@ template <typename T> __global__ __launch_bounds__(64) void tok_distill_join_ker
 // p of the listed tokens goes through LDS (one word an element, NOT_LISTED where none): the lane that owns the element picks
 // it up for the sums and the gradient.
 constexpr uint32_t NOT_LISTED = 0xffffffffu;
+// the gradient of a lane's 8 elements f; words: p of the listed ones
+__device__ __forceinline__ void dist_narrow_dx(const DistRow& d, float c, bool live, float fw, const uint32_t* words, float* f) {
+    if (__builtin_expect(__ballot(live && d.mu != d.m) != 0, 0)) {                     // some row of the wave whose rest has a reference of its own
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t pb = words[e];
+            const float g = pb == NOT_LISTED ? d.B * dist_u(d, c, f[e]) : dist_l(d, c, f[e], __uint_as_float(pb));
+            f[e] = live ? fw * g : 0.f;
+        }
+        return;
+    }
+    const bool none = d.l2S == INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {                            // one exponential for either kind
+        const uint32_t pb = words[e];
+        const bool un = pb == NOT_LISTED;
+        const float q = tok_exp2(__builtin_fmaf(f[e] - d.m, c, -(un ? d.l2u : d.l2S)));
+        const float g = un ? d.B * q : none ? 0.f : __builtin_fmaf(d.A, q, -__uint_as_float(pb));
+        f[e] = live ? fw * g : 0.f;
+    }
+}
 struct DistSum {
     double rest, listed, tot, acc;
-    float m, s, w;
+    float m, mu, s, w;
 };
 
 template <typename T, int G, bool GRAD>
@@ -415,9 +508,26 @@ __global__ __launch_bounds__(256) void tok_distill_narrow_kernel(DistArgs a) {
         un.add(f[e], ref, l);
         li.add(f[e], ref, !l);
     }
-    const float S = tok_group<G, TokSum>(un.S), Sl = tok_group<G, TokSum>(li.S);
-    const float n = tok_group<G, TokSum>(un.n), nl = tok_group<G, TokSum>(li.n);
+    float S = tok_group<G, TokSum>(un.S) * tok_exp2(-ref.dmax), n = tok_group<G, TokSum>(un.n), mu = m;
+    const float Sl = tok_group<G, TokSum>(li.S), nl = tok_group<G, TokSum>(li.n);
     const double sc = (double)tok_exp2(-ref.dmax);
+    const bool far = a.bucket && live && n + S < DIST_FAR;
+    if (__builtin_expect(__ballot(far) != 0, 0)) {                                     // some row of the wave: the second look at the unlisted elements
+        float um = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) um = mine[gl * 8 + e] != NOT_LISTED ? um : tok_max(um, f[e]);
+        um = tok_group<G, TokMax>(um);
+        const TokRef ru = tok_ref(um, a.r.c);
+        DistSums su{0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) su.add(f[e], ru, mine[gl * 8 + e] != NOT_LISTED);
+        const float Su = tok_group<G, TokSum>(su.S) * tok_exp2(-ru.dmax), nu = tok_group<G, TokSum>(su.n);
+        if (far) {
+            S = Su;
+            n = nu;
+            if (um > -INFINITY) mu = um;
+        }
+    }
     s = a.bucket ? 0.f : tok_group<G, TokMax>(s);
     if (!(s > -INFINITY)) s = 0.f;
     const bool dup = __ballot(twice) != 0;                   // any row of this wave
@@ -432,23 +542,24 @@ __global__ __launch_bounds__(256) void tok_distill_narrow_kernel(DistArgs a) {
     // the fp64 logarithms of all rows of the block by one wave, a row a lane (120,000 rows of 200 bf16 logits, K = 8: 70 us, by each
     // wave for its own rows 89)
     if (gl == 0) {
-        sums[gr].rest = (double)n + (double)S * sc;
+        sums[gr].rest = (double)n + (double)S;
         sums[gr].listed = (double)nl + (double)Sl * sc;
         sums[gr].tot = te.tot;
         sums[gr].acc = te.acc;
         sums[gr].m = m;
+        sums[gr].mu = mu;
         sums[gr].s = s;
         sums[gr].w = w;
     }
     __syncthreads();                                         // the marks have been read, too
     if (threadIdx.x < RB) {
         const DistSum q = sums[threadIdx.x];
-        const DistDone d = dist_finish(a, q.m, q.rest, q.listed, q.tot, q.acc, q.s);
+        const DistDone d = dist_finish(a, q.m, q.mu, q.rest, q.listed, q.tot, q.acc, q.s);
         done[threadIdx.x] = d;
         const int64_t rw = (a.r.u0 + blockIdx.x) * RB + threadIdx.x;
         if (rw < a.r.rows) {
             a.loss[rw] = q.w != 0.f ? (float)((double)q.w * (double)a.T * (double)a.T * d.kl) : 0.f;
-            if (a.stat) a.stat[rw] = q.w != 0.f ? make_float4(d.d.m, d.d.l2S, d.d.A, d.d.B) : make_float4(0.f, INFINITY, 0.f, 0.f);
+            if (a.stat && q.w != 0.f) dist_keep(a.stat, rw, d.d);
         }
     }
     __syncthreads();
@@ -458,29 +569,19 @@ __global__ __launch_bounds__(256) void tok_distill_narrow_kernel(DistArgs a) {
             const int64_t id = tok_int(a.ids, a.id64, row * K + j);
             if ((uint64_t)id >= (uint64_t)V) continue;
             float p = dist_p(a.t[row * K + j], r.shift);
-            bool first = true;
-            if (dup) {
+            if (dup) {                                       // each occurrence has the whole p
                 p = 0.f;
                 for (int i = 0; i < K; ++i)
-                    if (tok_int(a.ids, a.id64, row * K + i) == id) {
-                        if (i < j) first = false;
-                        p += dist_p(a.t[row * K + i], r.shift);
-                    }
+                    if (tok_int(a.ids, a.id64, row * K + i) == id) p += dist_p(a.t[row * K + i], r.shift);
             }
-            if (first) mine[id] = __float_as_uint(p);
-            if (a.pk) a.pk[row * K + j] = first && !r.none ? p : -1.f;
+            mine[id] = __float_as_uint(p);
+            if (a.pk) a.pk[row * K + j] = p;
         }
     tok_wave_fence();
     if constexpr (GRAD) {
         if (there && gl * 8 < V) {
             const float fw = w * a.T;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t pb = mine[gl * 8 + e];
-                const float q = dist_q(r.d, a.r.c, f[e]);
-                const float g = pb == NOT_LISTED ? r.d.B * q : r.none ? 0.f : __builtin_fmaf(r.d.A, q, -__uint_as_float(pb));
-                f[e] = live ? fw * g : 0.f;
-            }
+            dist_narrow_dx(r.d, a.r.c, live, fw, mine + gl * 8, f);
             tok_narrow_store<T>((tok_out<T>)a.dx + row * V, V, gl * 8, f);
         }
     }
@@ -544,15 +645,31 @@ template <typename T, bool GRAD> __global__ __launch_bounds__(64) void tok_disti
     else
         l.each(V, [&](int, float f) { un.add(f, ref, false); });
     const double sc = (double)tok_exp2(-ref.dmax);
+    float S = un.S * tok_exp2(-ref.dmax), n = un.n, mu = m;
+    const bool far = a.bucket && live && n + S < DIST_FAR;
+    if (__builtin_expect(__ballot(far) != 0, 0)) {                                     // some row of the wave: the second look at the unlisted elements
+        float um = -INFINITY;
+#pragma unroll 1
+        for (int e = 0; e < V; ++e) um = (in >> e) & 1 ? um : tok_max(um, TokElem<T>::one(x[e]));
+        const TokRef ru = tok_ref(um, a.r.c);
+        DistSums su{0.f, 0.f};
+#pragma unroll 1
+        for (int e = 0; e < V; ++e) su.add(TokElem<T>::one(x[e]), ru, (in >> e) & 1);
+        if (far) {
+            S = su.S * tok_exp2(-ru.dmax);
+            n = su.n;
+            if (um > -INFINITY) mu = um;
+        }
+    }
     DistTeach te{0.0, 0.0};
     for (int j = 0; live && j < K; ++j) {
         const int id = is[lane * K + j];
         if (id >= 0) te.add(ts[lane * K + j], s, TokElem<T>::one(x[id]), m, a.r.dinv_t);
     }
-    const DistDone r = dist_finish(a, m, (double)un.n + (double)un.S * sc, (double)li.n + (double)li.S * sc, te.tot, te.acc, s);
+    const DistDone r = dist_finish(a, m, mu, (double)n + (double)S, (double)li.n + (double)li.S * sc, te.tot, te.acc, s);
     if (there) {
         a.loss[row] = live ? (float)((double)w * (double)a.T * (double)a.T * r.kl) : 0.f;
-        if (a.stat) a.stat[row] = live ? make_float4(r.d.m, r.d.l2S, r.d.A, r.d.B) : make_float4(0.f, INFINITY, 0.f, 0.f);
+        if (a.stat && live) dist_keep(a.stat, row, r.d);
     }
     const float f = w * a.T, fB = f * r.d.B;
     float g[DIST_LANE_K];                                    // the entries' gradients, the student's row still in LDS
@@ -562,22 +679,18 @@ template <typename T, bool GRAD> __global__ __launch_bounds__(64) void tok_disti
         const int id = (GRAD || a.pk) && j < K ? is[lane * K + j] : -1;
         if (id >= 0 && live) {
             float p = 0.f;
-            bool first = true;
             if (!dup) {
                 p = dist_p(ts[lane * K + j], r.shift);
-            } else {
+            } else {                                         // each occurrence has the whole p
                 for (int i = 0; i < K; ++i)
-                    if (is[lane * K + i] == id) {
-                        first &= i >= j;
-                        p += dist_p(ts[lane * K + i], r.shift);
-                    }
+                    if (is[lane * K + i] == id) p += dist_p(ts[lane * K + i], r.shift);
             }
-            if (a.pk) a.pk[row * K + j] = first && !r.none ? p : -1.f;
+            if (a.pk) a.pk[row * K + j] = p;
             if (!r.none) g[j] = f * __builtin_fmaf(r.d.A, dist_q(r.d, a.r.c, TokElem<T>::one(x[id])), -p);
         }
     }
     if constexpr (GRAD) {
-        l.each(V, [&](int, float& v) { v = live ? fB * dist_q(r.d, a.r.c, v) : 0.f; });
+        l.each(V, [&](int, float& v) { v = live ? fB * dist_u(r.d, a.r.c, v) : 0.f; });
         if (there) {
             l.store(x, V);
 #pragma unroll
@@ -612,8 +725,7 @@ template <typename T> __global__ __launch_bounds__(256) void tok_distill_grad_ke
     tok_in<T> x = tok_row<T>(a.r, row);
     const int b0 = ch * 256 * U;
     const bool live = w != 0.f;
-    const float4 st = live ? a.stat[row] : make_float4(0.f, INFINITY, 0.f, 0.f);
-    const DistRow d{st.x, st.y, st.z, st.w};
+    const DistRow d = live ? dist_kept(a.stat, row) : DistRow{0.f, INFINITY, 0.f, 0.f, INFINITY, 0.f};
     const float f = live ? w * a.T * (a.g ? a.g[row] : 1.f) : 0.f, fB = f * d.B;
     u32x4_t r[U];
 #pragma unroll
@@ -628,23 +740,22 @@ template <typename T> __global__ __launch_bounds__(256) void tok_distill_grad_ke
         if (v < nvec) {
             float g[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) g[e] = live ? fB * dist_q(d, a.r.c, TokElem<T>::get(r[i], e)) : 0.f;
+            for (int e = 0; e < VEC; ++e) g[e] = live ? fB * dist_u(d, a.r.c, TokElem<T>::get(r[i], e)) : 0.f;
             tok_st16<T>(o + (int64_t)v * VEC, TokElem<T>::pack(g));
         }
     }
     const bool last = ch == a.chunks - 1;
     if (last && tid < ntail) {
         const int e = nvec * VEC + tid;
-        o[e] = TokElem<T>::put(live ? fB * dist_q(d, a.r.c, TokElem<T>::one(x[e])) : 0.f);
+        o[e] = TokElem<T>::put(live ? fB * dist_u(d, a.r.c, TokElem<T>::one(x[e])) : 0.f);
     }
     __syncthreads();                                     // the listed tokens' stores follow the block's own
     if (live) {
         const int64_t lo = (int64_t)b0 * VEC, hi = last ? a.r.V : lo + 256 * U * VEC;
         for (int j = tid; j < a.K; j += 256) {
             const int64_t id = tok_int(a.ids, a.id64, row * a.K + j);
-            const float p = a.pk[row * a.K + j];
-            if (id >= lo && id < hi && p >= 0.f)
-                o[id] = TokElem<T>::put(f * (d.A * dist_q(d, a.r.c, TokElem<T>::one(x[id])) - p));
+            if (id >= lo && id < hi)
+                o[id] = TokElem<T>::put(f * dist_l(d, a.r.c, TokElem<T>::one(x[id]), a.pk[row * a.K + j]));
         }
     }
 }
@@ -668,21 +779,12 @@ template <typename T, int G> __global__ __launch_bounds__(256) void tok_distill_
     if (live)
         for (int j = gl; j < K; j += G) {
             const int64_t id = tok_int(a.ids, a.id64, row * K + j);
-            const float p = a.pk[row * K + j];
-            if ((uint64_t)id < (uint64_t)V && p >= 0.f) mine[id] = __float_as_uint(p);
+            if ((uint64_t)id < (uint64_t)V) mine[id] = __float_as_uint(a.pk[row * K + j]);
         }
     __syncthreads();
     if (there && gl * 8 < V) {
-        const float4 st = live ? a.stat[row] : make_float4(0.f, INFINITY, 0.f, 0.f);
-        const DistRow d{st.x, st.y, st.z, st.w};
-        const float fw = live ? w * a.T * (a.g ? a.g[row] : 1.f) : 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t pb = mine[gl * 8 + e];
-            const float q = dist_q(d, a.r.c, f[e]);
-            const float g = pb == NOT_LISTED ? d.B * q : __builtin_fmaf(d.A, q, -__uint_as_float(pb));
-            f[e] = live ? fw * g : 0.f;
-        }
+        const DistRow d = live ? dist_kept(a.stat, row) : DistRow{0.f, INFINITY, 0.f, 0.f, INFINITY, 0.f};
+        dist_narrow_dx(d, a.r.c, live, live ? w * a.T * (a.g ? a.g[row] : 1.f) : 0.f, mine + gl * 8, f);
         tok_narrow_store<T>((tok_out<T>)a.dx + row * V, V, gl * 8, f);
     }
 }

@@ -33,6 +33,7 @@ from . import hip_ops as H
 MAX_TOP_K = 128          # csrc/hip/token.h TOK_MAX_K
 MAX_TEACHER_K = 256      # csrc/hip/token_distill.hip DIST_MAX_K
 MAX_VOCAB = 1_000_000    # csrc/hip/token.h TOK_MAX_V
+MIN_LOG_REST = -745.0    # the least logarithm of the student's mass outside the list, csrc/hip/token_distill.hip dist_finish
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TAILS = {"drop": 0, "bucket": 1}
 
@@ -349,7 +350,7 @@ def _distill_hip(logits, ids, logprobs, temperature, bucket, weight, dx, save):
     nseg = _distill_segments(V, code, dx is not None)
     stat = pk = None
     if save or dx is not None and nseg > 0:
-        stat = x.new_empty((rows, 4), dtype=torch.float32)
+        stat = x.new_empty((rows, 8), dtype=torch.float32)
         pk = x.new_empty((rows, K), dtype=torch.float32)
         stp, pkp = stat.data_ptr(), pk.data_ptr()
     if nseg > 1:
@@ -408,11 +409,14 @@ def _distill_torch(logits, ids, logprobs, temperature, tail, weight):
     kl = torch.where(live, p * (torch.where(live, t, 0.0) - torch.where(live, lq, 0.0)), 0.0).sum(-1)
     if tail == "bucket":
         listed = torch.zeros(logits.shape, dtype=torch.float64, device=logits.device).scatter_add_(-1, at, there.double()) > 0
-        q0 = torch.where(listed | none, 0.0, lq_all.exp()).sum(-1)
+        # as logarithms: far below the row's maximum the rest's own sum would lose its digits, then itself
+        rest = lq_all.masked_fill(listed | none, -math.inf)
+        some = ~(rest == -math.inf).all(-1)
+        lq0 = torch.logsumexp(torch.where(some.unsqueeze(-1), rest, 0.0), -1)
         p0 = 1 - p.sum(-1)
-        on = (p0 > 0) & (q0 > 0)
-        p0, q0 = torch.where(on, p0, 1.0), torch.where(on, q0, 1.0)
-        kl = kl + torch.where(on, p0 * (p0.log() - q0.log()), 0.0)
+        on = (p0 > 0) & some & ~(lq0 < MIN_LOG_REST)
+        p0 = torch.where(on, p0, 1.0)
+        kl = kl + torch.where(on, p0 * (p0.log() - lq0), 0.0)
     loss = kl * (temperature * temperature)
     if weight is not None:
         loss = torch.where(weight != 0, loss * weight.double(), 0.0)
@@ -429,8 +433,9 @@ def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     absent entries (shorter lists are padded with -1); entries of the same id add up.  ``tail`` says what becomes of the mass
     outside the list: ``"drop"`` renormalises the teacher over its list (a constant added to a row's values changes nothing,
     so logits divided by the temperature will do), ``"bucket"`` compares the remaining mass of both models as one more
-    outcome (left out where the student gives the rest no mass).  A row without entries has loss 0 under ``"drop"``.  Rows of
-    weight 0 are not read; their loss and gradient are 0.  Only ``logits`` have a gradient."""
+    outcome, however small the student's is; it is left out where the student rules the rest out (``-inf``, or finite mask
+    values that leave it less than ``exp(-745)``, where 64 bits end).  A row without entries has loss 0 under ``"drop"``.
+    Rows of weight 0 are not read; their loss and gradient are 0.  Only ``logits`` have a gradient."""
     temperature = _check_logits(logits, temperature)
     _check_teacher(logits, teacher_ids, teacher_logprobs, tail, weight)
     if not logits.is_cuda:

@@ -330,7 +330,8 @@ def _teacher(x, K, T, g, truncated=False):
     return ids, lp
 
 
-def _check_distill(x, ids, t, T, tail, w, tile=1):
+def _check_distill(x, ids, t, T, tail, w, tile=1, floor=0.0):
+    """``floor``: what a gradient may be off by where exponentials underflow."""
     R, V = x.shape
     loss, dx = O.distill(x, ids, t, T, tail, w)
     lq, none = O.log_q(x, T)
@@ -351,7 +352,7 @@ def _check_distill(x, ids, t, T, tail, w, tile=1):
     # B = A - p0 / q0 carries q0's error: where the rest of the student is small, (p0 / q0) q_v times the bound
     big = (dx.abs() / (wv.abs()[:, None] * T).clamp_min(1e-300)).nan_to_num(0, 0, 0)
     tg = wv.abs()[:, None] * T * ((q * 2 + big) * (2 * e + 8 * O.U) + 6 * O.U * p)
-    tg = tg.nan_to_num() + O.half_ulp(dx.nan_to_num(), x.dtype) * (1 + 1e-6)
+    tg = tg.nan_to_num() + O.half_ulp(dx.nan_to_num(), x.dtype) * (1 + 1e-6) + floor
     xd = x.repeat(tile, 1).cuda().requires_grad_(True)
     i, tt, wd = ids.repeat(tile, 1).cuda(), t.repeat(tile, 1).cuda(), None if w is None else w.repeat(tile).cuda()
     got = TO.topk_distill_loss(xd, i, tt, temperature=T, tail=tail, weight=wd)
@@ -715,3 +716,74 @@ def test_rows_of_large_finite_values(V, tile, dtype, values, T):
     ids[:, 2] = torch.where(ids[:, :2].eq(V // 2).any(-1), -1, ids[:, 2])
     for tail in ("drop", "bucket"):
         _check_distill(x, ids, t, T, tail, None, tile=tile)
+
+
+# ---- a student sure of the listed tokens -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("V,tile", [(4, 1), (40, 1), (40, 6600), (63, 6600), (100, 1), (300, 1), (500, 1), (700, 1), (5000, 1),
+                                    (33000, 1), (70001, 1), (140001, 1)])
+def test_bucket_of_a_student_sure_of_its_list(V, tile, dtype):
+    """The mass outside the list keeps its logarithm however far below the row's maximum it lies (in z = x / T).
+
+    Some elements lie hundreds of octaves below the others outside the list: exponentials below 2^-126 come out as 0, so with
+    w <= 1.5 and A, |B| <= 1 a gradient may be off by 1.5 T 2^-126 (0 for 1e-44 was seen)."""
+    g = torch.Generator().manual_seed(V)
+    K = min(3, V - 1)
+    gaps = torch.tensor([0.0, 30.0, 43.0, 46.0, 80.0, 88.0, 95.0, 104.0, 110.0, 300.0])
+    for T in (1.0, 0.05):
+        x = torch.randn(10, V, generator=g)
+        ids = torch.rand(10, V, generator=g).argsort(-1)[:, :K].contiguous()
+        high = (gaps * T)[:, None] + torch.rand(10, K, generator=g) * T + 5
+        x.scatter_(1, ids, high)
+        x = x.clamp_min(-3)
+        if V > 8:
+            x[8, ids[8, 0]] = -2.0                    # a listed token among the others
+            x[9] = torch.where(torch.zeros(V, dtype=torch.bool).scatter_(0, ids[9], True), x[9],
+                               torch.where(torch.arange(V) < V // 2, -math.inf, x[9]))
+            x[6] = torch.where(torch.zeros(V, dtype=torch.bool).scatter_(0, ids[6], True), x[6], x[6].sub(
+                100 * T * (torch.arange(V) * 8 // V).float()))
+        t = (torch.log_softmax(torch.randn(10, K, generator=g), -1) + math.log(0.9)).contiguous()
+        w = torch.rand(10, generator=g) + 0.5
+        print(V, tile, dtype, T, flush=True)
+        _check_distill(x.to(DTYPES[dtype]), ids, t, T, "bucket", w, tile=tile, floor=1.5 * T * 2.0 ** -126)
+
+
+def test_bucket_gradient_of_a_sure_student_against_differences():
+    """The loss of [200, 0, 0, 0] with the list {0: 0.9} falls when an unlisted logit rises, by p_0 / 3 = 1 / 30 each.  Linear in
+    the logits there but for the softmax of three: third derivative below p_0; rounding 2 tol / 2h with tol 2 ulp of 20."""
+    x, ids, t = torch.tensor([[200.0, 0.0, 0.0, 0.0]]), torch.tensor([[0]]), torch.tensor([[math.log(0.9)]])
+    h = 2.0 ** -3
+    loss, dx = TO.topk_distill_grad(x.cuda(), ids.cuda(), t.cuda(), tail="bucket")
+    assert abs(float(loss) - 19.565) < 1e-2
+    for v in range(4):
+        e = torch.zeros(1, 4)
+        e[0, v] = h
+        up, dn = (TO.topk_distill_loss((x + s * e).cuda(), ids.cuda(), t.cuda(), tail="bucket") for s in (1, -1))
+        assert abs(float((up - dn) / (2 * h) - dx[0, v])) <= h * h / 6 * 0.1 + 2 * 40 * 2.0 ** -23 / (2 * h)
+
+
+@pytest.mark.parametrize("V,tile", [(40, 1), (40, 33000), (300, 1), (700, 1), (70001, 1), (140001, 1)])
+def test_bucket_at_its_end_and_of_rows_that_are_not_numbers(V, tile):
+    """The CPU's rules: less than exp(-745) outside the list is ruled out, NaN anywhere is NaN, no entries compare the whole rows."""
+    x = torch.full((9, V), -3.0)
+    ids = torch.zeros(9, 2, dtype=torch.int64)
+    ids[:, 1] = V - 1
+    x[:, 0] = torch.tensor([700.0, 730.0, 760.0, 5000.0, 1e6, 3e38, 20.0, 20.0, 20.0])
+    x[5, 1:] = torch.finfo(torch.float32).min
+    x[6, V // 2] = math.nan
+    x[7, 0] = math.nan                                  # a listed one
+    x[8, 0] = math.inf
+    t = torch.tensor([[0.6, 0.3]]).log().repeat(9, 1)
+    for i in (ids, torch.full_like(ids, -1)):
+        want, dwant = TO.topk_distill_grad(x, i, t, tail="bucket")
+        xd = x.repeat(tile, 1).cuda().requires_grad_(True)
+        a = i.repeat(tile, 1).cuda(), t.repeat(tile, 1).cuda()
+        loss, dx = TO.topk_distill_grad(xd, *a, tail="bucket")
+        auto = TO.topk_distill_loss(xd, *a, tail="bucket")
+        dauto, = torch.autograd.grad(auto, xd, torch.ones_like(auto))
+        for l, d in ((_first(loss, tile), _first(dx, tile)), (_first(auto.detach(), tile), _first(dauto, tile))):
+            l, d = l.cpu(), d.cpu()
+            assert torch.equal(l.isnan(), want.isnan()) and torch.equal(d.isnan(), dwant.isnan())
+            tol = 2 * O.sum_error(x, 1.0) + 4 * O.U * want.abs()
+            assert ((l - want).abs() <= tol)[~want.isnan()].all()
+            assert ((d - dwant).abs() <= 8 * O.sum_error(x, 1.0))[~dwant.isnan()].all()

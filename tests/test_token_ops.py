@@ -189,3 +189,31 @@ def test_row_layouts():
     assert y.is_contiguous()
     y = TO._rows(torch.zeros(2, 3, 4, 7).permute(2, 0, 1, 3)[:, :, :2])[0]
     assert y.is_contiguous()
+
+
+@pytest.mark.parametrize("T", [1.0, 0.05])
+def test_bucket_of_a_student_sure_of_its_list(T):
+    """The student's mass outside the list counts by its logarithm, down to exp(-745); below that it is ruled out."""
+    p = 0.9
+    for gap in (30.0, 87.0, 110.0, 200.0, 500.0, 740.0):
+        x = torch.tensor([[gap * T, 0.0, 0.0, 0.0]])
+        ids, t = torch.tensor([[0]]), torch.tensor([[math.log(p)]])
+        p64 = math.exp(float(t.double()))
+        gap64 = float(x[0, 0].double()) / T
+        p0, lq0 = 1 - p64, math.log(3) - gap64 - math.log1p(3 * math.exp(-gap64))
+        want = T * T * (p64 * (math.log(p64) + math.log1p(3 * math.exp(-gap64))) + p0 * (math.log(p0) - lq0))
+        loss, dx = TO.topk_distill_grad(x, ids, t, temperature=T, tail="bucket")
+        assert abs(float(loss) - want) <= 4 * O.U * abs(want), gap
+        want_dx = torch.tensor([[p0, -p0 / 3, -p0 / 3, -p0 / 3]]).double() * T
+        assert torch.allclose(dx.double(), want_dx, rtol=4 * O.U + 3 * math.exp(-gap64) * 10, atol=0), gap
+    for rest in (-800 * T, torch.finfo(torch.float32).min, -math.inf):
+        x = torch.tensor([[0.0, rest, rest, rest]])
+        loss, dx = TO.topk_distill_grad(x, ids, t, temperature=T, tail="bucket")
+        assert abs(float(loss) - T * T * p64 * math.log(p64)) <= 4 * O.U * T * T and float(dx.abs().max()) == 0
+
+
+def test_bucket_of_a_row_that_is_not_a_number():
+    """A teacher row without entries compares the whole rows: nothing is lost, unless the student is not a number."""
+    x = torch.tensor([[0.0, 1.0], [math.nan, 1.0]])
+    loss = TO.topk_distill_loss(x, torch.full((2, 1), -1), torch.zeros(2, 1), tail="bucket")
+    assert abs(float(loss[0])) <= 1e-12 and loss[1].isnan()
