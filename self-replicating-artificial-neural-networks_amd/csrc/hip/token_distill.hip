@@ -56,7 +56,8 @@ __device__ __forceinline__ double group_sum64(double v) { return tok_group<64, T
 
 // Sums over a row's entries: with s = the largest t (drop mode) or 0 (bucket), e_k = exp(t_k - s),
 //   tot = sum e_k,   acc = sum e_k ( (t_k - s) - (x_k - m) / T )
-// one fp64 exponential an entry; p_k = e_k / tot (drop) or e_k (bucket).
+// one fp64 exponential an entry; p_k = e_k / tot (drop) or e_k (bucket).  An id that occurs several times is one token: each of its
+// entries then also brings e_k ln( sum of the e_i of that id / e_k ) (dist_parts).
 struct DistTeach {
     double tot, acc;
     __device__ __forceinline__ void add(float t, float s, float x, float m, double inv_t) {
@@ -65,6 +66,18 @@ struct DistTeach {
         if (e != 0.0) acc += e * (l - (x == -INFINITY ? -(double)INFINITY : ((double)x - (double)m) * inv_t));
     }
 };
+// An entry's e ln( sum of its id's e_i / e ).  same(i): entry i has that id; t_at(i): its value.  A term of its own and in fp32: it is
+// rare, and inside the fp64 loop it costs every row registers.  It may be off by some 2^-21 of e, less than ln sum is.
+template <typename S, typename V>
+__device__ __forceinline__ float dist_parts(int K, float t, float s, const S& same, const V& t_at) {
+    float top = t, sum = 0.f;
+    for (int i = 0; i < K; ++i)
+        if (same(i)) top = tok_max(top, t_at(i));
+    for (int i = 0; i < K; ++i)
+        if (same(i)) sum += tok_exp2((t_at(i) - top) * 1.4426950408889634f);
+    const float e = tok_exp2((t - s) * 1.4426950408889634f);
+    return e == 0.f ? 0.f : e * (top - t + __builtin_amdgcn_logf(sum) * 0.6931471805599453f);
+}
 // A row's loss and the gradient's factors.  rest: the student's sum over the elements outside the list relative to mu (mu = m where
 // there is nothing), listed: inside it, relative to m (drop mode: their sum counts, mu = m).  shift: ln p_k = t_k - shift.
 struct DistDone {
@@ -149,7 +162,7 @@ __device__ __forceinline__ DistRow dist_epilogue(const DistArgs& a, DistEntries&
         if (E.id[j] >= 0) te.add(E.t[j], s, E.x[j], m, a.r.dinv_t);
     te.tot = group_sum64(te.tot);
     te.acc = group_sum64(te.acc);
-    bool first[DIST_MAX_K / 64];
+    bool first[DIST_MAX_K / 64], twice = false;
     float nl = 0.f, Sl = 0.f;
 #pragma unroll
     for (int q = 0; q < DIST_MAX_K / 64; ++q) {
@@ -157,6 +170,7 @@ __device__ __forceinline__ DistRow dist_epilogue(const DistArgs& a, DistEntries&
         first[q] = j < K && E.id[j] >= 0;
         if (dup && first[q])
             for (int i = 0; i < j; ++i) first[q] &= E.id[i] != E.id[j];
+        twice |= j < K && E.id[j] >= 0 && !first[q];
         if (a.bucket && first[q]) {
             if (E.x[j] == m) nl += m > -INFINITY ? 1.f : 0.f;
             else if (m > -INFINITY) Sl += tok_exp2((E.x[j] - m) * a.r.c);
@@ -164,15 +178,17 @@ __device__ __forceinline__ DistRow dist_epilogue(const DistArgs& a, DistEntries&
     }
     nl = tok_group<64, TokSum>(nl);
     Sl = tok_group<64, TokSum>(Sl);
+    dup = __ballot(twice) != 0;
+    if (__builtin_expect(dup, 0)) {
+        float more = 0.f;
+        for (int j = lane; j < K; j += 64)
+            if (E.id[j] >= 0)
+                more += dist_parts(K, E.t[j], s, [&](int i) { return E.id[i] == E.id[j]; }, [&](int i) { return E.t[i]; });
+        te.acc += (double)tok_group<64, TokSum>(more);
+    }
     const DistDone r = dist_finish(a, m, mu, (double)n + (double)S, (double)nl + (double)Sl, te.tot, te.acc, s);
     for (int j = lane; j < K; j += 64) E.p[j] = dist_p(E.t[j], r.shift);
-    bool twice = false;
-#pragma unroll
-    for (int q = 0; q < DIST_MAX_K / 64; ++q) {
-        const int j = q * 64 + lane;
-        twice |= j < K && E.id[j] >= 0 && !first[q];
-    }
-    if (__ballot(twice)) {
+    if (__builtin_expect(dup, 0)) {
         tok_wave_fence();
         float sum[DIST_MAX_K / 64];
 #pragma unroll
@@ -537,6 +553,16 @@ __global__ __launch_bounds__(256) void tok_distill_narrow_kernel(DistArgs a) {
             const int64_t id = tok_int(a.ids, a.id64, row * K + j);
             if ((uint64_t)id < (uint64_t)V) te.add(a.t[row * K + j], s, TokElem<T>::one(x[id]), m, a.r.dinv_t);
         }
+    if (__builtin_expect(dup, 0) && live) {
+        float more = 0.f;
+        for (int j = gl; j < K; j += G) {
+            const int64_t id = tok_int(a.ids, a.id64, row * K + j);
+            if ((uint64_t)id < (uint64_t)V)
+                more += dist_parts(K, a.t[row * K + j], s, [&](int i) { return tok_int(a.ids, a.id64, row * K + i) == id; },
+                                   [&](int i) { return a.t[row * K + i]; });
+        }
+        te.acc += (double)more;
+    }
     te.tot = tok_group<G, TokSum>(te.tot);
     te.acc = tok_group<G, TokSum>(te.acc);
     // the fp64 logarithms of all rows of the block by one wave, a row a lane (120,000 rows of 200 bf16 logits, K = 8: 70 us, by each
@@ -665,6 +691,16 @@ template <typename T, bool GRAD> __global__ __launch_bounds__(64) void tok_disti
     for (int j = 0; live && j < K; ++j) {
         const int id = is[lane * K + j];
         if (id >= 0) te.add(ts[lane * K + j], s, TokElem<T>::one(x[id]), m, a.r.dinv_t);
+    }
+    if (__builtin_expect(dup, 0)) {
+        float more = 0.f;
+        for (int j = 0; j < K; ++j) {
+            const int id = is[lane * K + j];
+            if (id >= 0)
+                more += dist_parts(K, ts[lane * K + j], s, [&](int i) { return is[lane * K + i] == id; },
+                                   [&](int i) { return ts[lane * K + i]; });
+        }
+        te.acc += (double)more;
     }
     const DistDone r = dist_finish(a, m, mu, (double)n + (double)S, (double)li.n + (double)li.S * sc, te.tot, te.acc, s);
     if (there) {

@@ -787,3 +787,28 @@ def test_bucket_at_its_end_and_of_rows_that_are_not_numbers(V, tile):
             tol = 2 * O.sum_error(x, 1.0) + 4 * O.U * want.abs()
             assert ((l - want).abs() <= tol)[~want.isnan()].all()
             assert ((d - dwant).abs() <= 8 * O.sum_error(x, 1.0))[~dwant.isnan()].all()
+
+
+# ---- ids that repeat ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("tail", ["drop", "bucket"])
+@pytest.mark.parametrize("V,tile", [(5, 1), (40, 1), (40, 8300), (100, 1), (300, 1), (700, 1), (5000, 1), (70001, 1), (140001, 1)])
+def test_a_token_listed_in_parts_counts_as_one(V, tile, tail):
+    """Entries of one id add up before the logarithm: a list with tokens in two or three parts is the merged list."""
+    g = torch.Generator().manual_seed(V + 1)
+    x = torch.randn(8, V, generator=g) * 2
+    tok = torch.rand(8, V, generator=g).argsort(-1)[:, :3]
+    p = torch.softmax(torch.randn(8, 3, generator=g), -1) * 0.8
+    x[0, tok[0, 0]] += 30                               # sure of the token that is listed in parts
+    whole_ids = torch.cat([tok, torch.full((8, 4), -1)], 1)
+    whole = torch.cat([p, torch.zeros(8, 4)], 1).log()
+    parts_ids = torch.cat([tok, tok[:, :1], tok[:, 1:2], tok[:, :1], torch.full((8, 1), V)], 1)
+    parts = torch.cat([p * torch.tensor([0.5, 0.25, 1.0]), p[:, :1] * 0.25, p[:, 1:2] * 0.75, p[:, :1] * 0.25,
+                       torch.ones(8, 1)], 1).log()
+    _check_distill(x, whole_ids, whole, 1.0, tail, None, tile=tile)
+    _check_distill(x, parts_ids, parts, 1.0, tail, None, tile=tile)
+    want, dwant = O.distill(x, whole_ids, whole, 1.0, tail, None)
+    loss, dx = TO.topk_distill_grad(x.cuda(), parts_ids.cuda(), parts.cuda(), tail=tail)
+    # the parts' logarithms are rounded once each: |ln p| U of their p, in p ln p and in sums of p
+    tol = 2 * O.sum_error(x, 1.0) + 2 * O.U * want.abs() + 12 * O.U * (1 + parts[:, :6].abs().amax(-1).double())
+    _close(loss, want, tol, "loss")
+    assert float((dx.cpu().double() - dwant).abs().max()) <= 4 * O.sum_error(x, 1.0) + 40 * O.U

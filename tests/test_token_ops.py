@@ -217,3 +217,24 @@ def test_bucket_of_a_row_that_is_not_a_number():
     x = torch.tensor([[0.0, 1.0], [math.nan, 1.0]])
     loss = TO.topk_distill_loss(x, torch.full((2, 1), -1), torch.zeros(2, 1), tail="bucket")
     assert abs(float(loss[0])) <= 1e-12 and loss[1].isnan()
+
+
+@pytest.mark.parametrize("tail", ["drop", "bucket"])
+def test_a_token_listed_in_parts_counts_as_one(tail):
+    """Entries of one id add up before the logarithm: two halves on a student's sure token are no divergence."""
+    x = torch.tensor([[30.0, 0.0, 0.0]])
+    loss, dx = TO.topk_distill_grad(x, torch.tensor([[0, 0]]), torch.tensor([[0.5, 0.5]]).log(), tail=tail)
+    whole, dwhole = TO.topk_distill_grad(x, torch.tensor([[0]]), torch.zeros(1, 1), tail=tail)
+    # each half's logarithm is rounded once: 2 |ln 0.5| U of the mass
+    assert abs(float(loss - whole)) <= 2 * O.U and float((dx - dwhole).abs().max()) <= 2 * O.U
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(6, 40, generator=g) * 3
+    tok = torch.rand(6, 40, generator=g).argsort(-1)[:, :3]
+    p = torch.softmax(torch.randn(6, 3, generator=g), -1) * 0.8
+    parts_ids = torch.cat([tok[:, 1:], torch.full((6, 1), 40), tok, tok[:, :1]], 1)
+    parts = torch.cat([p[:, 1:] * 0.25, torch.ones(6, 1), p * torch.tensor([0.5, 0.75, 0.75]), p[:, :1] * 0.5], 1).log()
+    loss, dx = TO.topk_distill_grad(x, parts_ids, parts, tail=tail)
+    want, dwant = TO.topk_distill_grad(x, tok, p.log(), tail=tail)
+    tol = 12 * O.U * (1 + parts.abs().amax(-1))
+    assert ((loss - want).abs() <= tol + 4 * O.U * want.abs()).all()
+    assert ((dx - dwant).abs() <= 12 * O.U).all()

@@ -74,10 +74,12 @@ def distill(x, ids, t, T, tail, w):
             tot = sum(math.exp(v - top) for _, v in entries) if top > -math.inf else 0.0
             entries = [(i, v - top - math.log(tot) if tot > 0 else -math.inf) for i, v in entries]
         for i, v in entries:
-            pi = math.exp(v)
-            p[i] += pi
+            p[i] += math.exp(v)
+        parts = [i for i, _ in entries]
+        for i, v in sorted(dict(reversed(entries)).items(), key=lambda e: parts.index(e[0])):
+            pi = float(p[i])                          # entries of one id are one token
             if pi > 0:
-                kl += pi * (v - float(lq[r, i]))
+                kl += pi * ((v if parts.count(i) == 1 else math.log(pi)) - float(lq[r, i]))
         P = float(p.sum())
         A = B = P
         if tail == "bucket":
