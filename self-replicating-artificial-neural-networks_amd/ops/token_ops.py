@@ -12,9 +12,9 @@ tokens come next -- and train a model from another one's answers:
 
 Logits are ``(..., V)``, float32, bfloat16 or float16, 1 <= V <= 1,000,000.  Leading dimensions may have any strides (a slice
 ``logits[:, :-1]`` is read in place); the last one is copied if it is not contiguous.  Sums are taken in float32 or wider,
-whatever the logits' type; results are float32, gradients have the logits' type.  ``-inf`` logits are tokens ruled out: they
-have probability and gradient 0.  A row of nothing but ``-inf`` has log-probabilities ``-inf``, entropy 0 and no gradient.  A
-row with a NaN or ``+inf`` logit gives NaN.
+whatever the logits' type; results are float32, gradients (in backward mode; tensors with a forward-mode tangent are an error on
+a GPU) have the logits' type.  ``-inf`` logits are tokens ruled out: they have probability and gradient 0.  A row of nothing but
+``-inf`` has log-probabilities ``-inf``, entropy 0 and no gradient.  A row with a NaN or ``+inf`` logit gives NaN.
 
 On a GPU the HIP kernels of ``csrc/hip/token_score.hip`` and ``csrc/hip/token_distill.hip`` run, on the current stream of the
 logits' device; a GPU without the built extension is an error.  On the CPU the same formulas run as torch operations.
@@ -27,6 +27,7 @@ import operator
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import hip_ops as H
 
@@ -171,6 +172,14 @@ def _check_out(out, logits, *inputs):
             a, b = _span(t)
             if a < hi and lo < b:
                 raise ValueError("out must not share memory with the logits or another argument")
+
+
+def _no_tangent(*tensors):
+    """Forward-mode differentiation: the kernels go by a tensor's pointer and would drop its tangent without a word."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("the token operators have no forward-mode derivative on a GPU")
 
 
 # the current stream of a device as the launchers take it; torch.cuda.current_stream() builds a Stream object first (2 of the
@@ -327,6 +336,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
         raise ValueError(f"top_k must be in [0, min({MAX_TOP_K}, V = {logits.shape[-1]})], got {top_k}")
     if not logits.is_cuda:
         return _score_torch(logits, targets, temperature, top_k, ignore_index)
+    _no_tangent(logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         extra = []
         out = _Score.apply(logits, targets, temperature, top_k, ignore_index, extra)
@@ -446,6 +456,7 @@ def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     _check_teacher(logits, teacher_ids, teacher_logprobs, tail, weight)
     if not logits.is_cuda:
         return _distill_torch(logits, teacher_ids, teacher_logprobs, temperature, tail, weight)
+    _no_tangent(logits, teacher_logprobs, weight)
     ids, lp, weight = teacher_ids.contiguous(), _f32(teacher_logprobs), _f32(weight)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _Distill.apply(logits, ids, lp, temperature, _TAILS[tail], weight)

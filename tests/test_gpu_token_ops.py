@@ -812,3 +812,25 @@ def test_a_token_listed_in_parts_counts_as_one(V, tile, tail):
     tol = 2 * O.sum_error(x, 1.0) + 2 * O.U * want.abs() + 12 * O.U * (1 + parts[:, :6].abs().amax(-1).double())
     _close(loss, want, tol, "loss")
     assert float((dx.cpu().double() - dwant).abs().max()) <= 4 * O.sum_error(x, 1.0) + 40 * O.U
+
+
+# ---- calls that are refused on a GPU, and calls in unusual modes --------------------------------------------------------------
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwd
+    x, at, g = _logits(4, 50, "fp32", 30)
+    x, ids, t = x.cuda(), at[:, None].cuda(), torch.zeros(4, 1).cuda()
+    w = torch.ones(4).cuda()
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for f in (lambda: TO.token_logprobs(d, at.cuda()), lambda: TO.topk_distill_loss(d, ids, t),
+                  lambda: TO.topk_distill_loss(x, ids, fwd.make_dual(t, torch.ones_like(t))),
+                  lambda: TO.topk_distill_loss(x, ids, t, weight=fwd.make_dual(w, torch.ones_like(w))),
+                  lambda: TO.token_logprobs(d.clone().requires_grad_(True))):
+            with pytest.raises(RuntimeError):
+                f()
+        a = TO.token_logprobs(x, at.cuda())
+        _, dx = TO.topk_distill_grad(d, ids, t)             # detached: the values alone
+        assert fwd.unpack_dual(dx).tangent is None
+    assert all(torch.equal(p, q) for p, q in zip(a[:2], TO.token_logprobs(x, at.cuda())[:2]))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda z: TO.token_logprobs(z, at.cuda()).logprob, (x,), (torch.ones_like(x),))
