@@ -615,6 +615,8 @@ inline void tok_launch(void (*kernel)(A, X...), int64_t units, int nt, size_t ld
     }
 }
 inline TokRows tok_rows_of(uint64_t x, int64_t rows, int64_t n1, int64_t s0, int64_t s1, int64_t V, double temperature) {
+    // a tensor that only wraps another (functionalisation) has pointer 0: no kernel may read that
+    if (rows && !x) throw std::runtime_error("token operators: the logits have no storage");
     if (rows < 0 || V < 1 || V > TOK_MAX_V) throw std::runtime_error("token operators: vocabulary must be in [1, 10^6]");
     if (n1 < 1 || (rows && rows % n1)) throw std::runtime_error("token operators: rows must be a multiple of n1");
     if (!(temperature > 0)) throw std::runtime_error("token operators: temperature must be positive");

@@ -897,6 +897,7 @@ void launch_tok_distill(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t
     if (rows <= 0) return;
     if (dtype < 0 || dtype > 2) throw std::runtime_error("token operators: unknown logits type");
     if (K < 1 || K > DIST_MAX_K) throw std::runtime_error("tok_distill: 1 to 256 teacher entries a row");
+    if (!ids || !t || !loss) throw std::runtime_error("tok_distill: a tensor has no storage");
     DistArgs a{};
     a.r = tok_rows_of(x, rows, n1, s0, s1, V, temperature);
     a.ids = (int64_t)ids;
@@ -943,6 +944,7 @@ void launch_tok_distill_grad(uint64_t x, int dtype, int64_t rows, int64_t n1, in
     if (rows <= 0) return;
     if (dtype < 0 || dtype > 2) throw std::runtime_error("token operators: unknown logits type");
     if (K < 1 || K > DIST_MAX_K) throw std::runtime_error("tok_distill: 1 to 256 teacher entries a row");
+    if (!ids || !stat || !pk || !dx) throw std::runtime_error("tok_distill: a tensor has no storage");
     DistGradArgs a{};
     a.r = tok_rows_of(x, rows, n1, s0, s1, V, temperature);
     a.ids = (int64_t)ids;

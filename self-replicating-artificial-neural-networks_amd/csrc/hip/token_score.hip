@@ -900,6 +900,7 @@ void launch_tok_score(uint64_t x, int dtype, int64_t rows, int64_t n1, int64_t s
     if (rows <= 0) return;
     if (dtype < 0 || dtype > 2) throw std::runtime_error("token operators: unknown logits type");
     if (k < 0 || k > TOK_MAX_K || k > V) throw std::runtime_error("tok_score: top_k out of range");
+    if (!ent || (lp && !y) || (k && (!ids || !top))) throw std::runtime_error("tok_score: a tensor has no storage");
     ScoreArgs a{};
     a.r = tok_rows_of(x, rows, n1, s0, s1, V, temperature);
     a.y = (int64_t)y;
@@ -949,6 +950,7 @@ void launch_tok_score_grad(uint64_t x, int dtype, int64_t rows, int64_t n1, int6
                            uint64_t gent, uint64_t stat, uint64_t dx, uint64_t stream) {
     if (rows <= 0) return;
     if (dtype < 0 || dtype > 2) throw std::runtime_error("token operators: unknown logits type");
+    if (!stat || !dx) throw std::runtime_error("tok_score: a tensor has no storage");
     ScoreGradArgs a{};
     a.r = tok_rows_of(x, rows, n1, s0, s1, V, temperature);
     a.y = (int64_t)y;

@@ -238,3 +238,21 @@ def test_a_token_listed_in_parts_counts_as_one(tail):
     tol = 12 * O.U * (1 + parts.abs().amax(-1))
     assert ((loss - want).abs() <= tol + 4 * O.U * want.abs()).all()
     assert ((dx - dwant).abs() <= 12 * O.U).all()
+
+
+def test_launchers_refuse_tensors_without_storage():
+    """Pointer 0 (a functionalised tensor's) never reaches a kernel."""
+    from serann.ops import hip_ops as H
+    lib = H.lib(required=False)
+    if lib is None:
+        pytest.skip("extension not built")
+    P = 64                                    # P: never read, every call is refused before its launch
+    score = [P, 0, 1, 1, 0, 9, 9, 1.0, P, 1, 0, 1, -100, 2, P, P, P, P, 0, 0, 0]
+    sgrad = [P, 0, 1, 1, 0, 9, 9, 1.0, P, 1, 0, 1, -100, P, P, P, P, 0]
+    dist = [P, 0, 1, 1, 0, 9, 9, 1.0, P, 1, P, 0, 3, 0, P, 0, P, P, 0, 0]
+    dgrad = [P, 0, 1, 1, 0, 9, 9, 1.0, P, 1, 0, 3, 0, P, P, P, 0]
+    for f, args, needed in ((lib.tok_score, score, (0, 8, 15, 16, 17)), (lib.tok_score_grad, sgrad, (0, 15, 16)),
+                            (lib.tok_distill, dist, (0, 8, 10, 14)), (lib.tok_distill_grad, dgrad, (0, 8, 13, 14, 15))):
+        for i in needed:
+            with pytest.raises(RuntimeError, match="no storage"):
+                f(*(0 if j == i else v for j, v in enumerate(args)))
