@@ -477,9 +477,11 @@ def topk_distill_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
             torch.autograd.graph.increment_version(out)      # autograd notices if it had been saved for a backward pass
     logits = logits.detach()
     if not logits.is_cuda:
-        with torch.enable_grad():
+        with torch.inference_mode(False), torch.enable_grad():      # whatever the caller's mode, autograd works here
             x = logits.clone().requires_grad_(True)
-            loss = _distill_torch(x, teacher_ids, teacher_logprobs, temperature, tail, weight)
+            ids, lp, weight = (t.clone() if t is not None and t.is_inference() else t
+                               for t in (teacher_ids, teacher_logprobs, weight))
+            loss = _distill_torch(x, ids, lp, temperature, tail, weight)
             dx, = torch.autograd.grad(loss.sum(), x)
         return loss.detach(), dx.contiguous() if out is None else out.copy_(dx)
     ids, lp, weight = teacher_ids.contiguous(), _f32(teacher_logprobs), _f32(weight)

@@ -834,3 +834,14 @@ def test_forward_mode_derivatives_are_refused():
     assert all(torch.equal(p, q) for p, q in zip(a[:2], TO.token_logprobs(x, at.cuda())[:2]))
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda z: TO.token_logprobs(z, at.cuda()).logprob, (x,), (torch.ones_like(x),))
+
+
+def test_inference_mode():
+    x, at, g = _logits(6, 90, "fp32", 31)
+    ids, t = _teacher(x, 5, 1.0, g)
+    want = tuple(TO.token_logprobs(x.cuda(), at.cuda(), top_k=3)) + TO.topk_distill_grad(x.cuda(), ids.cuda(), t.cuda())
+    with torch.inference_mode():
+        xd = x.cuda()
+        got = tuple(TO.token_logprobs(xd, at.cuda(), top_k=3)) + TO.topk_distill_grad(xd, ids.cuda(), t.cuda(),
+                                                                                     out=torch.empty_like(xd))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

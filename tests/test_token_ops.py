@@ -256,3 +256,21 @@ def test_launchers_refuse_tensors_without_storage():
         for i in needed:
             with pytest.raises(RuntimeError, match="no storage"):
                 f(*(0 if j == i else v for j, v in enumerate(args)))
+
+
+@pytest.mark.parametrize("tail", ["drop", "bucket"])
+def test_inference_mode(tail):
+    """The gradient in one call needs no autograd of the caller's: inference mode and its tensors do, inside and outside."""
+    x, _, g = _rows(5, 12, 2)
+    ids, t, w = torch.randint(0, 12, (5, 3), generator=g), torch.full((5, 3), -1.5), torch.rand(5, generator=g)
+    want = TO.topk_distill_grad(x, ids, t, weight=w, tail=tail)
+    with torch.inference_mode():
+        a = [v.clone() for v in (x, ids, t, w)]
+        assert a[0].is_inference()
+        got = TO.topk_distill_grad(*a[:3], weight=a[3], tail=tail, out=torch.empty_like(a[0]))
+        mixed = TO.topk_distill_grad(x, ids, t, weight=w, tail=tail)
+        score = TO.token_logprobs(a[0], a[1][:, 0], top_k=2)
+    later = TO.topk_distill_grad(*a[:3], weight=a[3], tail=tail)
+    for r in (got, mixed, later):
+        assert torch.equal(r[0], want[0]) and torch.equal(r[1], want[1])
+    assert all(torch.equal(p, q) for p, q in zip(score, TO.token_logprobs(x, ids[:, 0], top_k=2)))
