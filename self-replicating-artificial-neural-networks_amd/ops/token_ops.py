@@ -290,7 +290,7 @@ def _log_softmax(logits, temperature):
 
 
 def _score_torch(logits, targets, temperature, top_k, ignore_index):
-    skip = (targets == ignore_index) if targets is not None else None
+    skip = (targets.long() == ignore_index) if targets is not None else None      # an int32 comparison would wrap the index
     if skip is not None:
         logits = torch.where(skip.unsqueeze(-1), 0.0, logits)           # not read
     lq, none = _log_softmax(logits, temperature)

@@ -845,3 +845,10 @@ def test_inference_mode():
         got = tuple(TO.token_logprobs(xd, at.cuda(), top_k=3)) + TO.topk_distill_grad(xd, ids.cuda(), t.cuda(),
                                                                                      out=torch.empty_like(xd))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_ignore_index_beyond_the_targets_type():
+    x, _, _ = _logits(4, 30, "fp32", 32)
+    y = torch.tensor([0, 1, 2, 3], dtype=torch.int32).cuda()
+    a, b = TO.token_logprobs(x.cuda(), y, ignore_index=1 << 40), TO.token_logprobs(x.cuda(), y.long())
+    assert torch.equal(a.logprob, b.logprob) and torch.equal(a.entropy, b.entropy)

@@ -274,3 +274,12 @@ def test_inference_mode(tail):
     for r in (got, mixed, later):
         assert torch.equal(r[0], want[0]) and torch.equal(r[1], want[1])
     assert all(torch.equal(p, q) for p, q in zip(score, TO.token_logprobs(x, ids[:, 0], top_k=2)))
+
+
+def test_ignore_index_beyond_the_targets_type():
+    """int32 targets and an index of 64 bits: none of them is ignored."""
+    x, _, _ = _rows(4, 10, 5)
+    y = torch.arange(4, dtype=torch.int32)
+    a = TO.token_logprobs(x, y, ignore_index=1 << 40)
+    b = TO.token_logprobs(x, y.long())
+    assert torch.equal(a.logprob, b.logprob) and torch.equal(a.entropy, b.entropy)
