@@ -852,3 +852,35 @@ def test_ignore_index_beyond_the_targets_type():
     y = torch.tensor([0, 1, 2, 3], dtype=torch.int32).cuda()
     a, b = TO.token_logprobs(x.cuda(), y, ignore_index=1 << 40), TO.token_logprobs(x.cuda(), y.long())
     assert torch.equal(a.logprob, b.logprob) and torch.equal(a.entropy, b.entropy)
+
+
+# ---- many short rows that do not lie one behind the other ---------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("V", [1, 13, 40, 64])
+@pytest.mark.parametrize("view", ["shifted", "columns", "transposed", "expanded"])
+def test_many_short_strided_rows(view, V, dtype):
+    """From 65,536 rows on, a view of short rows: the same bits as its contiguous copy (which is tested against the definition)."""
+    g = torch.Generator().manual_seed(V)
+    n = 66000
+    if view == "shifted":
+        base, x = (b := torch.randn(120, 551, V, generator=g).to(DTYPES[dtype]).cuda()), b[:, :-1]
+    elif view == "columns":
+        base, x = (b := torch.randn(n, V + 3, generator=g).to(DTYPES[dtype]).cuda()), b[:, 1:V + 1]
+    elif view == "transposed":
+        base, x = (b := torch.randn(550, 120, V, generator=g).to(DTYPES[dtype]).cuda()), b.transpose(0, 1)
+    else:
+        base, x = (b := torch.randn(1, 550, V, generator=g).to(DTYPES[dtype]).cuda()), b.expand(120, 550, V)
+    lead = x.shape[:-1]
+    y = torch.randint(0, V, lead, generator=g).cuda()
+    y.view(-1)[::7] = IGN
+    k = min(V, 5)
+    a, b = TO.token_logprobs(x, y, top_k=k), TO.token_logprobs(x.contiguous(), y, top_k=k)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    ids, t = a.top_ids, a.top_logprobs
+    w = torch.rand(lead, generator=g).cuda()
+    for tail in ("drop", "bucket"):
+        a, b = (TO.topk_distill_grad(v, ids, t, tail=tail, weight=w) for v in (x, x.contiguous()))
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+        xa = x.detach().requires_grad_(True)
+        loss = TO.topk_distill_loss(xa, ids, t, tail=tail, weight=w)
+        assert torch.equal(loss.detach(), b[0])
