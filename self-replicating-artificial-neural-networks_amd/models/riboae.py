@@ -160,15 +160,21 @@ class GeneticAutoencoder(nn.Module):
     def encode(self, x):
         return self.inference_net(x).argmax(-1)
 
+    def _hip(self, cls, name, device):
+        """The HIP decoder or encoder of the current weights, made anew when they or the device have changed."""
+        op = getattr(self, name)
+        if op is None or op.stale(self, device):
+            op = cls(self, device)
+            setattr(self, name, op)
+        return op
+
     # -- positions one by one: log-probabilities, entropies, next-best tokens ----------------------------
     def _eval_logits(self, bits):
         """(n, G) genotype bits -> (n, L, V) logits in eval mode, on the HIP kernels on a GPU (like ``decode_tokens``)."""
         if bits.is_cuda:
             from ..ops.riboae_ops import HipRiboDecoder, available
             if available():
-                if self._hip_decoder is None or self._hip_decoder.stale(self):
-                    self._hip_decoder = HipRiboDecoder(self, bits.device)
-                return self._hip_decoder.logits(bits)
+                return self._hip(HipRiboDecoder, "_hip_decoder", bits.device).logits(bits)
         return self.generative_net.logits(F.one_hot(bits.long(), self.alphabet).float())
 
     @torch.no_grad()
@@ -204,9 +210,9 @@ class GeneticAutoencoder(nn.Module):
         self.eval()
         if x.is_cuda:
             from ..ops.riboae_ops import HipRiboEncoder, available
-            if available() and (self._hip_encoder is None or self._hip_encoder.stale(self)):
-                self._hip_encoder = HipRiboEncoder(self, x.device)
-        bits = self._hip_encoder(x) if x.is_cuda and self._hip_encoder is not None else self.encode(x)
+            bits = self._hip(HipRiboEncoder, "_hip_encoder", x.device)(x) if available() else self.encode(x)
+        else:
+            bits = self.encode(x)
         r = token_logprobs(self._eval_logits(bits), temperature=temperature, top_k=top_k)
         return r.top_ids, r.top_logprobs, float(temperature)
 
@@ -218,9 +224,7 @@ class GeneticAutoencoder(nn.Module):
         if str(device).startswith("cuda"):
             from ..ops.riboae_ops import HipRiboEncoder, available
             if available():
-                if self._hip_encoder is None or self._hip_encoder.stale(self):
-                    self._hip_encoder = HipRiboEncoder(self, device)
-                return self._hip_encoder(t).cpu().numpy()
+                return self._hip(HipRiboEncoder, "_hip_encoder", device)(t).cpu().numpy()
         return self.encode(t).cpu().numpy()
 
     @torch.no_grad()
@@ -230,9 +234,7 @@ class GeneticAutoencoder(nn.Module):
         if str(device).startswith("cuda"):
             from ..ops.riboae_ops import HipRiboDecoder, available
             if available():
-                if self._hip_decoder is None or self._hip_decoder.stale(self):
-                    self._hip_decoder = HipRiboDecoder(self, device)
-                return self._hip_decoder(g).cpu().numpy()
+                return self._hip(HipRiboDecoder, "_hip_decoder", device)(g).cpu().numpy()
         return self.decode(g).cpu().numpy()
 
 

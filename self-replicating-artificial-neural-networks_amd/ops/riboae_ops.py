@@ -30,12 +30,37 @@ def available() -> bool:
     return H.available()
 
 
-class HipRiboDecoder:
-    def __init__(self, model, device):
-        self.device = torch.device(device)
+def _indexed(device) -> torch.device:
+    d = torch.device(device)
+    return torch.device(d.type, torch.cuda.current_device()) if d.type == "cuda" and d.index is None else d
+
+
+class _FoldedWeights:
+    """Copies of a model's weights in the kernels' layouts, and what they were made from: every parameter and statistic by its
+    storage and version (in-place writes raise it; the storage is held, so its address stays its own), the device, and
+    ``model._param_version``, which kernels that write parameters past autograd raise (``riboae.hip_trainer``)."""
+
+    def _made_from(self, model, net, device):
+        self.device = _indexed(device)
         self.version = getattr(model, "_param_version", 0)
         self.model_id = id(model)
+        self.sources = [(t.detach(), self._at(t)) for t in (*net.parameters(), *net.buffers())]
+
+    @staticmethod
+    def _at(t):
+        return t.data_ptr(), None if t.is_inference() else t._version
+
+    def _stale(self, model, net, device) -> bool:
+        now = [self._at(t) for t in (*net.parameters(), *net.buffers())]
+        return (id(model) != self.model_id or getattr(model, "_param_version", 0) != self.version
+                or (device is not None and _indexed(device) != self.device)
+                or now != [at for _, at in self.sources] or any(v is None for _, v in now))
+
+
+class HipRiboDecoder(_FoldedWeights):
+    def __init__(self, model, device):
         gn = model.generative_net
+        self._made_from(model, gn, device)
         G, A, V, L = model.genotype_length, model.alphabet, model.vocab, model.max_len
         self.G, self.A, self.V, self.L = G, A, V, L
         with torch.no_grad():
@@ -64,8 +89,8 @@ class HipRiboDecoder:
         self.C1 = w.shape[0]
         self._plans = {}
 
-    def stale(self, model) -> bool:
-        return id(model) != self.model_id or getattr(model, "_param_version", 0) != self.version
+    def stale(self, model, device=None) -> bool:
+        return self._stale(model, model.generative_net, device)
 
     def _plan(self, B: int):
         """Buffers and gemm3 launches for a batch of B genotypes (cached per B)."""
@@ -163,17 +188,15 @@ def _fold_bn(bn):
     return s_, bn.bias - bn.running_mean * s_
 
 
-class HipRiboEncoder:
+class HipRiboEncoder(_FoldedWeights):
     """Eval-mode ``inference_net`` + argmax on the HIP kernels (see the module docstring)."""
 
     SPLIT_KSTEPS = 48           # 32-wide k steps per split-K block of the flatten Dense
 
     def __init__(self, model, device, chunk: int = 128):
-        self.device = torch.device(device)
-        self.version = getattr(model, "_param_version", 0)
-        self.model_id = id(model)
-        self.chunk = int(chunk)
         net = model.inference_net
+        self._made_from(model, net, device)
+        self.chunk = int(chunk)
         self.L, self.E = net.max_len, net.emb_dim
         self.G, self.A = net.genotype_length, net.alphabet
         with torch.no_grad():
@@ -192,8 +215,8 @@ class HipRiboEncoder:
             self.bd = H.padded(net.dense.bias.to(self.device, torch.float32).contiguous())
         self._plans = {}
 
-    def stale(self, model) -> bool:
-        return id(model) != self.model_id or getattr(model, "_param_version", 0) != self.version
+    def stale(self, model, device=None) -> bool:
+        return self._stale(model, model.inference_net, device)
 
     def _plan(self, B: int):
         """Buffers, descriptors and tile tables for a chunk of B sequences (cached per B)."""

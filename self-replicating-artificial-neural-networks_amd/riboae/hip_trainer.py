@@ -521,7 +521,12 @@ class HipRiboTrainer:
             lib.adam(self.p.data_ptr(), self.g.data_ptr(), self.m.data_ptr(), self.v.data_ptr(), self.pbf.data_ptr(),
                      self.step_i.data_ptr(), self.lr_t.data_ptr(), self.pa.size, float(lr), self.b1, self.b2,
                      self.eps, s)
+        self._written()
         return {"loss": nelbo, "nll": -logpx.mean(), "kld": kl.mean()}
+
+    def _written(self):
+        """The kernels have written parameters or moving statistics: copies of them elsewhere are out of date."""
+        self.model._param_version = getattr(self.model, "_param_version", 0) + 1
 
     # checkpoint interface of the trainer's optimizer (riboae/trainer.py saves ``opt.state_dict()``)
     def _moment_views(self, arena: torch.Tensor) -> List[torch.Tensor]:
@@ -580,6 +585,7 @@ class HipRiboTrainer:
         self.g.zero_()
         with torch.no_grad():
             self.stats.copy_(st0)
+        self._written()
         out = {}
         for name, mod, attr, klayout, perm in self.specs:
             off, cnt = self.pa.items[name]

@@ -213,3 +213,81 @@ def test_gpu_trainer_learns_from_a_teacher(tmp_path, engine):
     hist = T.train("kd", _model(2), data, None, str(tmp_path), batch_size=32, max_steps=6, device="cuda", log=lambda *a: None,
                    demo_every=0, engine=engine, teacher=_model(1), teacher_top_k=4)
     assert len(hist) == 6 and np.isfinite(hist).all()
+
+
+def _changes(m):
+    """What changes a model's weights or statistics, one after the other."""
+    other = _model(5).to(next(m.parameters()).device)
+    yield "load_state_dict", lambda: m.load_state_dict(other.state_dict())
+    x = torch.randint(0, 12, (16, 32), generator=torch.Generator().manual_seed(2)).to(next(m.parameters()).device)
+
+    def optimizer_step():
+        m.train()
+        opt = torch.optim.Adam(m.parameters(), lr=0.05)
+        m.compute_loss(x, 0.3, 0.05)["loss"].backward()
+        opt.step()
+
+    def statistics_alone():
+        m.train()
+        with torch.no_grad():
+            m.compute_loss(x, 0.3, 0.05)
+
+    def reassigned():
+        with torch.no_grad():
+            for _ in range(3):                        # a freed weight's address may come back
+                m.generative_net.dense.weight = torch.nn.Parameter(torch.randn_like(m.generative_net.dense.weight) * 0.2)
+                m.inference_net.dense.weight.data = torch.randn_like(m.inference_net.dense.weight) * 0.2
+
+    yield "optimizer step", optimizer_step
+    yield "moving statistics", statistics_alone
+    yield "reassigned", reassigned
+
+
+def test_folded_weights_know_what_they_were_made_from():
+    """Copies of weights in the kernels' layouts are stale after any change of what they were made from."""
+    from serann.ops.riboae_ops import HipRiboDecoder, HipRiboEncoder
+    m = _model(1)
+    for name, change in _changes(m):
+        dec, enc = HipRiboDecoder(m, "cpu"), HipRiboEncoder(m, "cpu")
+        m.eval()
+        m.encode_tokens(np.zeros((2, 32), np.int64))
+        assert not dec.stale(m) and not enc.stale(m) and not dec.stale(m, "cpu") and dec.stale(m, "meta")
+        change()
+        assert dec.stale(m) and enc.stale(m), name
+    dec = HipRiboDecoder(m, "cpu")
+    assert dec.stale(copy.deepcopy(m))
+    m._param_version = 7
+    assert dec.stale(m)
+
+
+@pytest.mark.gpu
+def test_gpu_scores_and_targets_follow_the_weights():
+    """Scores, teacher targets and codes are those of a model made anew from the current weights, whatever changed them."""
+    from serann.riboae.hip_trainer import HipRiboTrainer
+    m = _model(1).cuda()
+    bits, x = _bits(9), torch.randint(0, 12, (9, 32), generator=torch.Generator().manual_seed(8)).cuda()
+
+    def look(model):
+        s = model.score_tokens(bits, device="cuda", top_k=3)
+        ids, lp, _ = model.distill_targets(x, 4)
+        return [s[k] for k in sorted(s)] + [ids.cpu().numpy(), lp.cpu().numpy(), model.encode_tokens(x.cpu().numpy(), "cuda"),
+                                            model.decode_tokens(bits, "cuda")]
+
+    def agree(name):
+        fresh = _model(3).cuda()
+        fresh.load_state_dict(m.state_dict())
+        for a, b in zip(look(m), look(fresh)):
+            np.testing.assert_array_equal(a, b, err_msg=name)
+
+    before = look(m)
+    for name, change in _changes(m):
+        change()
+        agree(name)
+        after = look(m)
+        assert any((a != b).any() for a, b in zip(before, after)), name
+        before = after
+    tr = HipRiboTrainer(m.train(), device="cuda")
+    tr.step(x, 0.3, 0.05, 0.05)
+    agree("trainer step")
+    tr.step(x, 0.3, 0.05, 0.05, update=False)
+    agree("step without update")
