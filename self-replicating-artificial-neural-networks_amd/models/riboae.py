@@ -162,11 +162,13 @@ class GeneticAutoencoder(nn.Module):
 
     def _hip(self, cls, name, device):
         """The HIP decoder or encoder of the current weights, made anew when they or the device have changed."""
-        op = getattr(self, name)
-        if op is None or op.stale(self, device):
-            op = cls(self, device)
-            setattr(self, name, op)
-        return op
+        from ..ops.riboae_ops import LOCK
+        with LOCK:
+            op = getattr(self, name)
+            if op is None or op.stale(self, device):
+                op = cls(self, device)
+                setattr(self, name, op)
+            return op
 
     # -- positions one by one: log-probabilities, entropies, next-best tokens ----------------------------
     def _eval_logits(self, bits):
@@ -183,6 +185,7 @@ class GeneticAutoencoder(nn.Module):
         """How this decoder rates every position of the phenotypes of ``genotypes`` (n, G): ``tokens`` (the given ones, by
         default the decoded sequence), their ``logprob``, the position's ``entropy`` and, with ``top_k``, its best tokens
         ``top_ids`` and their ``top_logprobs`` (``ops.token_ops.token_logprobs``)."""
+        from ..ops.riboae_ops import LOCK
         from ..ops.token_ops import token_logprobs
         if len(genotypes) == 0:
             shape = (0, self.max_len)
@@ -196,7 +199,8 @@ class GeneticAutoencoder(nn.Module):
         self.eval()
         g = torch.as_tensor((np.asarray(genotypes) > 0.5).astype(np.int64), device=device)
         t = torch.as_tensor(np.asarray(tokens), device=device).long()
-        r = token_logprobs(self._eval_logits(g), t, temperature=temperature, top_k=top_k)
+        with LOCK:
+            r = token_logprobs(self._eval_logits(g), t, temperature=temperature, top_k=top_k)
         out = {"tokens": t, "logprob": r.logprob, "entropy": r.entropy}
         if top_k:
             out.update(top_ids=r.top_ids, top_logprobs=r.top_logprobs)
@@ -206,6 +210,7 @@ class GeneticAutoencoder(nn.Module):
     def distill_targets(self, x, top_k: int, temperature: float = 1.0):
         """What this autoencoder teaches about the token batch ``x`` (B, L): (ids, log-probabilities, temperature) of its
         ``top_k`` best tokens at each position of its own reconstruction, in eval mode, for ``compute_loss(teacher=...)``."""
+        from ..ops.riboae_ops import LOCK
         from ..ops.token_ops import token_logprobs
         self.eval()
         if x.is_cuda:
@@ -213,7 +218,8 @@ class GeneticAutoencoder(nn.Module):
             bits = self._hip(HipRiboEncoder, "_hip_encoder", x.device)(x) if available() else self.encode(x)
         else:
             bits = self.encode(x)
-        r = token_logprobs(self._eval_logits(bits), temperature=temperature, top_k=top_k)
+        with LOCK:
+            r = token_logprobs(self._eval_logits(bits), temperature=temperature, top_k=top_k)
         return r.top_ids, r.top_logprobs, float(temperature)
 
     # -- numpy inference API used by the codec ----------------------------------------------------

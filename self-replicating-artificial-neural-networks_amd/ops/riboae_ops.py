@@ -20,6 +20,9 @@ evolutionary_experiment/logic/ribosomal_autoencoder.py:116-124).
 """
 from __future__ import annotations
 
+import contextlib
+import threading
+
 import numpy as np
 import torch
 
@@ -28,6 +31,18 @@ from . import hip_ops as H
 
 def available() -> bool:
     return H.available()
+
+
+# held while a decoder or encoder enqueues its launches, and until what reads its buffers is enqueued (``logits``)
+LOCK = threading.RLock()
+
+
+def _tensors(v):
+    if isinstance(v, torch.Tensor):
+        yield v
+    elif isinstance(v, (dict, list, tuple)):
+        for x in v.values() if isinstance(v, dict) else v:
+            yield from _tensors(x)
 
 
 def _indexed(device) -> torch.device:
@@ -45,6 +60,24 @@ class _FoldedWeights:
         self.version = getattr(model, "_param_version", 0)
         self.model_id = id(model)
         self.sources = [(t.detach(), self._at(t)) for t in (*net.parameters(), *net.buffers())]
+        self.stream = torch.cuda.current_stream(self.device) if self.device.type == "cuda" else None
+
+    def __reduce__(self):
+        return type(None), ()                         # a copied or pickled model makes its own
+
+    @contextlib.contextmanager
+    def _enqueueing(self):
+        """One caller at a time, on the operator's own device; the copies and buffers are everyone's, so a stream that was not
+        the last to use them waits for that one (everything that was enqueued there, readers of a returned view too)."""
+        with LOCK, torch.cuda.device(self.device):
+            cur = torch.cuda.current_stream(self.device)
+            if cur != self.stream and not torch.cuda.is_current_stream_capturing():
+                cur.wait_stream(self.stream)
+                self.stream = cur
+                for t in _tensors({k: v for k, v in self.__dict__.items() if k != "sources"}):
+                    if t.is_cuda:
+                        t.record_stream(cur)
+            yield
 
     @staticmethod
     def _at(t):
@@ -132,18 +165,21 @@ class HipRiboDecoder(_FoldedWeights):
     @torch.no_grad()
     def logits(self, bits: torch.Tensor) -> torch.Tensor:
         """(n, G) genotype bits -> (n, L, V) fp32 logits of the MFMA decode, a view of the plan's buffer (valid until the
-        next call with n genotypes): what ``token_ops.token_logprobs`` scores positions from."""
-        return self._forward(bits)["logits"].view(bits.shape[0], self.L, self.V)
+        next call with n genotypes; ``LOCK`` held until its reader is enqueued keeps other threads' calls off it): what
+        ``token_ops.token_logprobs`` scores positions from."""
+        with self._enqueueing():
+            return self._forward(bits)["logits"].view(bits.shape[0], self.L, self.V)
 
     @torch.no_grad()
     def __call__(self, bits: torch.Tensor) -> torch.Tensor:
         B = bits.shape[0]
-        pl = self._forward(bits)
-        lib, s = H.lib(), H.stream_handle()
-        lib.group_argmax(pl["logits"].data_ptr(), pl["out"].data_ptr(), B * self.L, self.V, s)
-        out = pl["out"].long().clone()
-        self._rescore(bits, pl, out)
-        return out
+        with self._enqueueing():
+            pl = self._forward(bits)
+            lib, s = H.lib(), H.stream_handle()
+            lib.group_argmax(pl["logits"].data_ptr(), pl["out"].data_ptr(), B * self.L, self.V, s)
+            out = pl["out"].long().clone()
+            self._rescore(bits, pl, out)
+            return out
 
     # bf16 operands round each product h_k * w_k by a relative ~2^-9 (input and weight); over the K = 3072
     # products of a logit that is a random walk of std ~ 2^-9 * sqrt(2/3) * ||h|| ||w|| / sqrt(K).  A position
@@ -276,11 +312,13 @@ class HipRiboEncoder(_FoldedWeights):
     @torch.no_grad()
     def logits(self, tokens: torch.Tensor) -> torch.Tensor:
         """(n, L) token ids -> (n, G, A) fp32 logits of the eval-mode inference net."""
-        return self._run(tokens, want_logits=True)
+        with self._enqueueing():
+            return self._run(tokens, want_logits=True)
 
     @torch.no_grad()
     def __call__(self, tokens: torch.Tensor) -> torch.Tensor:
-        return self._run(tokens, want_logits=False)
+        with self._enqueueing():
+            return self._run(tokens, want_logits=False)
 
     def _run(self, tokens: torch.Tensor, want_logits: bool):
         tok = tokens.to(self.device).to(torch.int32)

@@ -291,3 +291,55 @@ def test_gpu_scores_and_targets_follow_the_weights():
     agree("trainer step")
     tr.step(x, 0.3, 0.05, 0.05, update=False)
     agree("step without update")
+
+
+def test_folded_weights_stay_with_their_model():
+    import pickle
+    from serann.ops.riboae_ops import HipRiboDecoder
+    m = _model(1)
+    m._hip_decoder = HipRiboDecoder(m, "cpu")
+    assert copy.deepcopy(m)._hip_decoder is None and pickle.loads(pickle.dumps(m))._hip_decoder is None
+    assert m._hip_decoder is not None
+
+
+@pytest.mark.gpu
+def test_gpu_targets_and_scores_from_two_streams_and_two_threads():
+    """Batches of one size share a model's buffers: calls from other streams and threads come out as one after the other."""
+    import threading
+    m = _model(1).cuda()
+    g = torch.Generator().manual_seed(4)
+    xs = [torch.randint(0, 12, (24, 32), generator=g).cuda() for _ in range(6)]
+    bits = [_bits(24, seed=s) for s in range(6)]
+    want = [m.distill_targets(x, 4)[:2] for x in xs]
+    scored = [m.score_tokens(b, device="cuda", top_k=2) for b in bits]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(4):                                # one thread, no waits between the streams
+        got = []
+        for i, x in enumerate(xs):
+            with torch.cuda.stream(streams[i % 3]):
+                got.append(m.distill_targets(x, 4)[:2])
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    out, errors = {}, []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(streams[k]):
+                for i in range(6):
+                    out[k, i] = m.distill_targets(xs[i], 4)[:2] + (m.score_tokens(bits[i], device="cuda", top_k=2),)
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:                    # a failed thread is a failed test
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(3)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors, errors
+    for (_, i), (ids, lp, s) in out.items():
+        assert torch.equal(ids, want[i][0]) and torch.equal(lp, want[i][1])
+        for k in s:
+            np.testing.assert_array_equal(s[k], scored[i][k])
