@@ -439,6 +439,13 @@ def _distill_torch(logits, ids, logprobs, temperature, tail, weight):
     return loss.float()
 
 
+def check_distill(logits, teacher_ids, teacher_logprobs, *, temperature=1.0, tail="drop", weight=None) -> float:
+    """The checks of :func:`topk_distill_loss` alone: raises as it would, returns the temperature as a float."""
+    temperature = _check_logits(logits, temperature)
+    _check_teacher(logits, teacher_ids, teacher_logprobs, tail, weight)
+    return temperature
+
+
 def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, *,
                       temperature: float = 1.0, tail: str = "drop", weight: Optional[torch.Tensor] = None) -> torch.Tensor:
     """KL divergence from a teacher's top tokens to ``softmax(logits / temperature)``, times ``temperature ** 2`` and the row's
@@ -452,8 +459,7 @@ def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     outcome, however small the student's is; it is left out where the student rules the rest out (``-inf``, or finite mask
     values that leave it less than ``exp(-745)``, where 64 bits end).  A row without entries has loss 0 under ``"drop"``.
     Rows of weight 0 are not read; their loss and gradient are 0.  Only ``logits`` have a gradient."""
-    temperature = _check_logits(logits, temperature)
-    _check_teacher(logits, teacher_ids, teacher_logprobs, tail, weight)
+    temperature = check_distill(logits, teacher_ids, teacher_logprobs, temperature=temperature, tail=tail, weight=weight)
     if not logits.is_cuda:
         return _distill_torch(logits, teacher_ids, teacher_logprobs, temperature, tail, weight)
     _no_tangent(logits, teacher_logprobs, weight)
@@ -469,8 +475,7 @@ def topk_distill_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     """The losses of :func:`topk_distill_loss` and the gradient of their sum with respect to ``logits``, in one pass over the
     logits where a row fits a block's registers.  The gradient has the logits' shape and type, is contiguous, and goes to
     ``out`` when given (which must not share memory with any argument).  Nothing is recorded for autograd."""
-    temperature = _check_logits(logits, temperature)
-    _check_teacher(logits, teacher_ids, teacher_logprobs, tail, weight)
+    temperature = check_distill(logits, teacher_ids, teacher_logprobs, temperature=temperature, tail=tail, weight=weight)
     if out is not None:
         _check_out(out, logits, teacher_ids, teacher_logprobs, weight)
         if not out.is_inference():

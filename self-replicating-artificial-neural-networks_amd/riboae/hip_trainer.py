@@ -31,7 +31,7 @@ import numpy as np
 import torch
 
 from ..ops import hip_ops as H
-from ..ops.token_ops import topk_distill_grad
+from ..ops.token_ops import check_distill, topk_distill_grad
 
 SLACK = 64
 
@@ -470,6 +470,9 @@ class HipRiboTrainer:
         if tuple(tokens.shape) != (B, L):
             raise ValueError(f"expected a (B, {L}) token batch, got {tuple(tokens.shape)}")
         pl = self._plan(B, fused=update)
+        if teacher is not None:                           # refused before the step counter or a moving statistic has changed
+            ids, logp, distill_t = teacher
+            check_distill(pl.buf["yh2"][:B * L * V].view(B, L, V), ids, logp, temperature=distill_t)
         tp = float(prior_temperature if prior_temperature is not None else self.model.prior_temperature)
         lib, s = self.lib, H.stream_handle()
         if update and pl.skip is not None:
@@ -503,7 +506,6 @@ class HipRiboTrainer:
             lib.cat_loglik_bwd(buf["yh2"].data_ptr(), buf["tok"].data_ptr(), buf["gout"].data_ptr(),
                                buf["dh2"].data_ptr(), B, L, V, s, 1)
         else:
-            ids, logp, distill_t = teacher
             weight = torch.full((B, L), 1.0 / B, device=self.dev)
             out = buf["dh2"][:B * L * V].view(B, L, V)
             div, _ = topk_distill_grad(buf["yh2"][:B * L * V].view(B, L, V), ids, logp, temperature=distill_t,

@@ -343,3 +343,22 @@ def test_gpu_targets_and_scores_from_two_streams_and_two_threads():
         assert torch.equal(ids, want[i][0]) and torch.equal(lp, want[i][1])
         for k in s:
             np.testing.assert_array_equal(s[k], scored[i][k])
+
+
+@pytest.mark.gpu
+def test_a_refused_teacher_leaves_the_hip_trainer_as_it_was():
+    from serann.riboae.hip_trainer import HipRiboTrainer
+    m = _model(2).cuda().train()
+    tr = HipRiboTrainer(m, device="cuda")
+    x = torch.randint(0, 12, (16, 32), generator=torch.Generator().manual_seed(1)).cuda()
+    ids, lp, t = _model(1).cuda().distill_targets(x, 4)
+    tr.step(x, 0.3, 0.05, 1e-3, teacher=(ids, lp, t))
+    torch.cuda.synchronize()
+    was = [v.clone() for v in (tr.p, tr.stats, tr.m, tr.v, tr.step_i)]
+    for bad in ((ids.cpu(), lp, t), (ids[:8], lp[:8], t), (ids.float(), lp, t), (ids, lp, 0.0), (ids, lp), (ids, lp[..., :2], t)):
+        with pytest.raises((TypeError, ValueError)):
+            tr.step(x, 0.3, 0.05, 1e-3, teacher=bad)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(was, (tr.p, tr.stats, tr.m, tr.v, tr.step_i)))
+    tr.step(x, 0.3, 0.05, 1e-3, teacher=(ids, lp, t))
+    assert int(tr.step_i) == int(was[4]) + 1
