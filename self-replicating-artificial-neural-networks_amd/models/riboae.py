@@ -19,6 +19,7 @@ does the encode path (embedding gather, LDS-halo convolutions, split-K Dense, gr
 """
 from __future__ import annotations
 
+import contextlib
 import math
 import os
 from typing import Dict, Optional
@@ -171,6 +172,17 @@ class GeneticAutoencoder(nn.Module):
             return op
 
     # -- positions one by one: log-probabilities, entropies, next-best tokens ----------------------------
+    @contextlib.contextmanager
+    def _in_eval_mode(self):
+        """Eval mode inside, every module's own mode again afterwards: a model may be asked in the middle of its training."""
+        was = [(m, m.training) for m in self.modules()]
+        self.eval()
+        try:
+            yield
+        finally:
+            for m, training in was:
+                m.training = training
+
     def _eval_logits(self, bits):
         """(n, G) genotype bits -> (n, L, V) logits in eval mode, on the HIP kernels on a GPU (like ``decode_tokens``)."""
         if bits.is_cuda:
@@ -194,17 +206,17 @@ class GeneticAutoencoder(nn.Module):
             if top_k:
                 out.update(top_ids=np.zeros(shape + (top_k,), np.int64), top_logprobs=np.zeros(shape + (top_k,), np.float32))
             return out
-        if tokens is None:
-            tokens = self.decode_tokens(genotypes, device=device)
-        self.eval()
-        g = torch.as_tensor((np.asarray(genotypes) > 0.5).astype(np.int64), device=device)
-        t = torch.as_tensor(np.asarray(tokens), device=device).long()
-        with LOCK:
-            r = token_logprobs(self._eval_logits(g), t, temperature=temperature, top_k=top_k)
-        out = {"tokens": t, "logprob": r.logprob, "entropy": r.entropy}
-        if top_k:
-            out.update(top_ids=r.top_ids, top_logprobs=r.top_logprobs)
-        return {k: v.cpu().numpy() for k, v in out.items()}
+        with self._in_eval_mode():
+            if tokens is None:
+                tokens = self.decode_tokens(genotypes, device=device)
+            g = torch.as_tensor((np.asarray(genotypes) > 0.5).astype(np.int64), device=device)
+            t = torch.as_tensor(np.asarray(tokens), device=device).long()
+            with LOCK:
+                r = token_logprobs(self._eval_logits(g), t, temperature=temperature, top_k=top_k)
+            out = {"tokens": t, "logprob": r.logprob, "entropy": r.entropy}
+            if top_k:
+                out.update(top_ids=r.top_ids, top_logprobs=r.top_logprobs)
+            return {k: v.cpu().numpy() for k, v in out.items()}
 
     @torch.no_grad()
     def distill_targets(self, x, top_k: int, temperature: float = 1.0):
@@ -212,15 +224,15 @@ class GeneticAutoencoder(nn.Module):
         ``top_k`` best tokens at each position of its own reconstruction, in eval mode, for ``compute_loss(teacher=...)``."""
         from ..ops.riboae_ops import LOCK
         from ..ops.token_ops import token_logprobs
-        self.eval()
-        if x.is_cuda:
-            from ..ops.riboae_ops import HipRiboEncoder, available
-            bits = self._hip(HipRiboEncoder, "_hip_encoder", x.device)(x) if available() else self.encode(x)
-        else:
-            bits = self.encode(x)
-        with LOCK:
-            r = token_logprobs(self._eval_logits(bits), temperature=temperature, top_k=top_k)
-        return r.top_ids, r.top_logprobs, float(temperature)
+        with self._in_eval_mode():
+            if x.is_cuda:
+                from ..ops.riboae_ops import HipRiboEncoder, available
+                bits = self._hip(HipRiboEncoder, "_hip_encoder", x.device)(x) if available() else self.encode(x)
+            else:
+                bits = self.encode(x)
+            with LOCK:
+                r = token_logprobs(self._eval_logits(bits), temperature=temperature, top_k=top_k)
+            return r.top_ids, r.top_logprobs, float(temperature)
 
     # -- numpy inference API used by the codec ----------------------------------------------------
     @torch.no_grad()

@@ -102,6 +102,23 @@ def test_a_teacher_leaves_the_moving_statistics_of_a_step(kind):
         assert torch.equal(a, b), name
 
 
+def test_scores_and_targets_leave_a_model_in_its_mode():
+    """Asked in the middle of training, a model goes on with batch statistics; its answers are those of eval mode."""
+    m = _model(1)
+    x, bits = torch.randint(0, 12, (6, 32), generator=torch.Generator().manual_seed(5)), _bits(4)
+    want, scored = m.distill_targets(x, 3), m.score_tokens(bits, top_k=2)
+    m.train()
+    m.generative_net.bn1.eval()
+    got, again = m.distill_targets(x, 3), m.score_tokens(bits, top_k=2)
+    assert m.training and m.generative_net.bn2.training and not m.generative_net.bn1.training
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for k in scored:
+        np.testing.assert_array_equal(again[k], scored[k])
+    with pytest.raises(ValueError):
+        m.score_tokens(bits, top_k=13)
+    assert m.training
+
+
 def test_trainer_learns_from_a_teacher(tmp_path):
     teacher, m = _model(1), _model(2)
     before = copy.deepcopy(teacher.state_dict())
