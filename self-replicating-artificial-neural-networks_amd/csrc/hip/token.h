@@ -19,7 +19,7 @@
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16_t;
 
-constexpr int TOK_MAX_K = 128;        // top alternatives / teacher entries a row
+constexpr int TOK_MAX_K = 128;        // top alternatives a row
 constexpr int64_t TOK_MAX_V = 1000000;
 constexpr int TOK_MAX_SEG = 62;       // segments a row is cut into at most: 10^6 fp32 logits in 64 KB pieces; a lane each to join
 constexpr int TOK_NARROW_V = 512;     // rows of up to 64 x 8 elements: a group of 8-64 lanes a row, no LDS reduction
@@ -583,6 +583,8 @@ template <typename T> struct TokLane {
 // 13.7); longer ones are cut into pieces of up to 4096 vectors (64 KB: four blocks a CU, so that one loads while another
 // counts; pieces of 8192 make 1,000 rows of 128,001 bf16 logits 57 us instead of 50) and joined by a second launch.
 constexpr int TOK_PIECE_VEC = 4096;
+static_assert((TOK_MAX_V / 4 + TOK_PIECE_VEC - 1) / TOK_PIECE_VEC <= TOK_MAX_SEG && TOK_MAX_SEG <= 64,
+              "the join of the scores gives each segment of a row a lane");
 struct TokPlan {
     int nt, nv, nseg, segvec;
 };

@@ -13,8 +13,9 @@ tokens come next -- and train a model from another one's answers:
 Logits are ``(..., V)``, float32, bfloat16 or float16, 1 <= V <= 1,000,000.  Leading dimensions may have any strides (a slice
 ``logits[:, :-1]`` is read in place); the last one is copied if it is not contiguous.  Sums are taken in float32 or wider,
 whatever the logits' type; results are float32, gradients (in backward mode; tensors with a forward-mode tangent are an error on
-a GPU) have the logits' type.  ``-inf`` logits are tokens ruled out: they have probability and gradient 0.  A row of nothing but
-``-inf`` has log-probabilities ``-inf``, entropy 0 and no gradient.  A row with a NaN or ``+inf`` logit gives NaN.
+a GPU) have the logits' type.  ``-inf`` logits are tokens ruled out: they have probability 0, and gradient 0 unless they are the
+target or in the teacher's list (the formula's then, next to an infinite loss).  A row of nothing but ``-inf`` has
+log-probabilities ``-inf``, entropy 0 and no gradient.  A row with a NaN or ``+inf`` logit gives NaN.
 
 On a GPU the HIP kernels of ``csrc/hip/token_score.hip`` and ``csrc/hip/token_distill.hip`` run, on the current stream of the
 logits' device; a GPU without the built extension is an error.  On the CPU the same formulas run as torch operations.
