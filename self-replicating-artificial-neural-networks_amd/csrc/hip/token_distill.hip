@@ -66,8 +66,8 @@ struct DistTeach {
         if (e != 0.0) acc += e * (l - (x == -INFINITY ? -(double)INFINITY : ((double)x - (double)m) * inv_t));
     }
 };
-// An entry's e ln( sum of its id's e_i / e ).  same(i): entry i has that id; t_at(i): its value.  A term of its own and in fp32: it is
-// rare, and inside the fp64 loop it costs every row registers.  It may be off by some 2^-21 of e, less than ln sum is.
+// An entry's e ln( sum of its id's e_i / e ).  same(i): entry i has that id; t_at(i): its value.  A term of its own and in fp32: it
+// is rare, and inside the fp64 loop it costs every row registers.  It may be off by some 2^-21 of e, less than ln sum is.
 template <typename S, typename V>
 __device__ __forceinline__ float dist_parts(int K, float t, float s, const S& same, const V& t_at) {
     float top = t, sum = 0.f;
@@ -230,8 +230,9 @@ struct DistSums {
     }
 };
 
-// f(element) over a thread's elements of a segment that no bit marks, read again.  Element by element in a loop: unrolled, its masks
-// would take the scalar registers of a wave from the kernel that this is the rare part of (8,192 x 8,000 bf16, K = 64: 69 us, 65).
+// f(element) over a thread's elements of a segment that no bit marks, read again.  Element by element in a loop: unrolled, its
+// masks would take the scalar registers of a wave from the kernel that this is the rare part of (8,192 x 8,000 bf16, K = 64, tail
+// bucket: 69 us, 65).  It is worth a second read: 8,192 x 32,000 bf16 with every row sure of its list 433 us, 224 else.
 template <typename T, int NT, typename F>
 __device__ __forceinline__ void dist_unlisted(tok_in<T> x, int nv, const uint32_t* bits, const F& f) {
     constexpr int VEC = TokElem<T>::VEC;
@@ -355,7 +356,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void to
         n += red[k][2];
     }
     S *= tok_exp2(-ref.dmax);
-    if (__builtin_expect(a.bucket && n + S < DIST_FAR, 0)) {                     // the second look at the unlisted elements
+    if (__builtin_expect(a.bucket && n + S < DIST_FAR, 0)) {    // the second look at the unlisted elements
         const bool tail = tid < ntail && !((bits[nv * VEC / 32] >> ((nv * VEC + tid) & 31)) & 1);
         float um = tail ? s.xt : -INFINITY;
         dist_unlisted<T, NT>(x + e0, nv, bits, [&](float f) { um = tok_max(um, f); });
@@ -460,7 +461,7 @@ template <typename T> __global__ __launch_bounds__(64) void tok_distill_join_ker
 constexpr uint32_t NOT_LISTED = 0xffffffffu;
 // the gradient of a lane's 8 elements f; words: p of the listed ones
 __device__ __forceinline__ void dist_narrow_dx(const DistRow& d, float c, bool live, float fw, const uint32_t* words, float* f) {
-    if (__builtin_expect(__ballot(live && d.mu != d.m) != 0, 0)) {                     // some row of the wave whose rest has a reference of its own
+    if (__builtin_expect(__ballot(live && d.mu != d.m) != 0, 0)) {    // some row of the wave whose rest has a reference of its own
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const uint32_t pb = words[e];
@@ -528,7 +529,7 @@ __global__ __launch_bounds__(256) void tok_distill_narrow_kernel(DistArgs a) {
     const float Sl = tok_group<G, TokSum>(li.S), nl = tok_group<G, TokSum>(li.n);
     const double sc = (double)tok_exp2(-ref.dmax);
     const bool far = a.bucket && live && n + S < DIST_FAR;
-    if (__builtin_expect(__ballot(far) != 0, 0)) {                                     // some row of the wave: the second look at the unlisted elements
+    if (__builtin_expect(__ballot(far) != 0, 0)) {    // some row of the wave: the second look at the unlisted elements
         float um = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 8; ++e) um = mine[gl * 8 + e] != NOT_LISTED ? um : tok_max(um, f[e]);
@@ -565,8 +566,8 @@ __global__ __launch_bounds__(256) void tok_distill_narrow_kernel(DistArgs a) {
     }
     te.tot = tok_group<G, TokSum>(te.tot);
     te.acc = tok_group<G, TokSum>(te.acc);
-    // the fp64 logarithms of all rows of the block by one wave, a row a lane (120,000 rows of 200 bf16 logits, K = 8: 70 us, by each
-    // wave for its own rows 89)
+    // the fp64 logarithms of all rows of the block by one wave, a row a lane (120,000 rows of 200 bf16 logits, K = 8, tail bucket:
+    // 70 us, by each wave for its own rows 89, when both were tried; 73 now, with the rest's own reference)
     if (gl == 0) {
         sums[gr].rest = (double)n + (double)S;
         sums[gr].listed = (double)nl + (double)Sl * sc;
@@ -673,7 +674,7 @@ template <typename T, bool GRAD> __global__ __launch_bounds__(64) void tok_disti
     const double sc = (double)tok_exp2(-ref.dmax);
     float S = un.S * tok_exp2(-ref.dmax), n = un.n, mu = m;
     const bool far = a.bucket && live && n + S < DIST_FAR;
-    if (__builtin_expect(__ballot(far) != 0, 0)) {                                     // some row of the wave: the second look at the unlisted elements
+    if (__builtin_expect(__ballot(far) != 0, 0)) {    // some row of the wave: the second look at the unlisted elements
         float um = -INFINITY;
 #pragma unroll 1
         for (int e = 0; e < V; ++e) um = (in >> e) & 1 ? um : tok_max(um, TokElem<T>::one(x[e]));

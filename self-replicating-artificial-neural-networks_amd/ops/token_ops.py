@@ -418,16 +418,13 @@ def _distill_torch(logits, ids, logprobs, temperature, tail, weight):
     p = t.exp()
     live = p != 0
     # an id that occurs several times is one token: each of its entries takes the logarithm of their sum
-    near = torch.sort(torch.where(there, ids.long(), -1 - torch.arange(ids.shape[-1], device=ids.device)), -1).values
-    if (near[..., 1:] == near[..., :-1]).any():
-        whole = torch.zeros(logits.shape, dtype=torch.float64, device=logits.device).scatter_add_(-1, at, p).gather(-1, at)
-        count = torch.zeros(logits.shape, dtype=torch.int32, device=logits.device).scatter_add_(-1, at, there.int())
-        t = torch.where(there & (count.gather(-1, at) > 1), whole.log(), t)
+    count = torch.zeros_like(lq_all).scatter_add(-1, at, there.double())
+    whole = torch.zeros_like(lq_all).scatter_add(-1, at, p).gather(-1, at)
+    t = torch.where(there & (count.gather(-1, at) > 1), whole.log(), t)
     kl = torch.where(live, p * (torch.where(live, t, 0.0) - torch.where(live, lq, 0.0)), 0.0).sum(-1)
     if tail == "bucket":
-        listed = torch.zeros(logits.shape, dtype=torch.float64, device=logits.device).scatter_add_(-1, at, there.double()) > 0
         # as logarithms: far below the row's maximum the rest's own sum would lose its digits, then itself
-        rest = lq_all.masked_fill(listed | none, -math.inf)
+        rest = lq_all.masked_fill((count > 0) | none, -math.inf)
         some = ~(rest == -math.inf).all(-1)
         lq0 = torch.logsumexp(torch.where(some.unsqueeze(-1), rest, 0.0), -1)
         p0 = 1 - p.sum(-1)

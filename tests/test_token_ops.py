@@ -283,3 +283,14 @@ def test_ignore_index_beyond_the_targets_type():
     a = TO.token_logprobs(x, y, ignore_index=1 << 40)
     b = TO.token_logprobs(x, y.long())
     assert torch.equal(a.logprob, b.logprob) and torch.equal(a.entropy, b.entropy)
+
+
+@pytest.mark.parametrize("tail", ["drop", "bucket"])
+def test_per_row_transforms(tail):
+    """On the CPU a row at a time under vmap, and its gradient, are the batch's."""
+    x, _, g = _rows(5, 12, 4)
+    ids, t = torch.randint(0, 12, (5, 3), generator=g), torch.full((5, 3), -1.5)
+    loss, dx = TO.topk_distill_grad(x, ids, t, tail=tail)
+    f = lambda a, b, c: TO.topk_distill_loss(a, b, c, tail=tail)
+    assert torch.allclose(torch.func.vmap(f)(x, ids, t), loss, rtol=2 * O.U, atol=1e-9)
+    assert torch.allclose(torch.func.vmap(torch.func.grad(f))(x, ids, t), dx, rtol=4 * O.U, atol=4 * O.U)
