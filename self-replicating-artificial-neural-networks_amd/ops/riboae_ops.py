@@ -69,7 +69,8 @@ class _FoldedWeights:
     def _enqueueing(self):
         """One caller at a time, on the operator's own device; the copies and buffers are everyone's, so a stream that was not
         the last to use them waits for that one (everything that was enqueued there, readers of a returned view too)."""
-        with LOCK, torch.cuda.device(self.device):
+        # (buffers made in a caller's inference mode could not be written outside it)
+        with LOCK, torch.cuda.device(self.device), torch.inference_mode(False), torch.no_grad():
             cur = torch.cuda.current_stream(self.device)
             if cur != self.stream and not torch.cuda.is_current_stream_capturing():
                 cur.wait_stream(self.stream)

@@ -379,3 +379,26 @@ def test_a_refused_teacher_leaves_the_hip_trainer_as_it_was():
     assert all(torch.equal(a, b) for a, b in zip(was, (tr.p, tr.stats, tr.m, tr.v, tr.step_i)))
     tr.step(x, 0.3, 0.05, 1e-3, teacher=(ids, lp, t))
     assert int(tr.step_i) == int(was[4]) + 1
+
+
+@pytest.mark.gpu
+def test_gpu_scores_and_targets_in_and_after_inference_mode():
+    """What a model keeps for the kernels is of use in inference mode and outside, whichever asked first."""
+    bits, x = _bits(7), torch.randint(0, 12, (7, 32), generator=torch.Generator().manual_seed(3)).cuda()
+
+    def look(m):
+        s = m.score_tokens(bits, device="cuda", top_k=3)
+        ids, lp, _ = m.distill_targets(x, 4)
+        return [s[k] for k in sorted(s)] + [ids.cpu().numpy(), lp.cpu().numpy(), m.encode_tokens(x.cpu().numpy(), "cuda")]
+
+    want = look(_model(1).cuda())
+    m = _model(1).cuda()
+    with torch.inference_mode():
+        inside = look(m)
+    after = look(m)
+    with torch.inference_mode():
+        again = look(m)
+        made_inside = look(_model(1).cuda())
+    for got in (inside, after, again, made_inside):
+        for a, b in zip(got, want):
+            np.testing.assert_array_equal(a, b)
