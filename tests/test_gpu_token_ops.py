@@ -884,3 +884,43 @@ def test_many_short_strided_rows(view, V, dtype):
         xa = x.detach().requires_grad_(True)
         loss = TO.topk_distill_loss(xa, ids, t, tail=tail, weight=w)
         assert torch.equal(loss.detach(), b[0])
+
+
+@pytest.mark.parametrize("V", [40, 300, 9000, 70001, 140001])
+def test_rare_rows_captured_and_replayed(V):
+    """What only some rows take -- a rest with its own reference, ids that repeat, large values -- is decided anew on every
+    replay, forward and backward."""
+    g = torch.Generator().manual_seed(V)
+    plain = torch.randn(12, V, generator=g)
+    ids = torch.rand(12, V, generator=g).argsort(-1)[:, :6].contiguous()
+    t = (torch.log_softmax(torch.randn(12, 6, generator=g), -1) + math.log(0.9)).contiguous()
+    sure = plain.scatter(1, ids, torch.tensor([0.0, 50.0, 120.0] * 4)[:, None] + torch.rand(12, 6, generator=g))
+    large = plain.clone()
+    large[::3] = 1e10
+    twice = ids.clone()
+    twice[::2, 4] = ids[::2, 1]
+    z, i, tt = plain.cuda(), ids.cuda(), t.cuda()
+
+    def call(z, i):
+        x = z.detach().requires_grad_(True)
+        loss = TO.topk_distill_loss(x, i, tt, tail="bucket")
+        dx, = torch.autograd.grad(loss, x, torch.ones_like(loss))
+        s = TO.token_logprobs(z, i[:, 0], top_k=3)
+        return (loss.detach(), dx) + TO.topk_distill_grad(z, i, tt, tail="bucket") + tuple(s)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(z, i)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = call(z, i)
+    for src, si in ((plain, ids), (sure, ids), (large, twice), (sure, twice), (plain, ids)):
+        z.copy_(src)
+        i.copy_(si)
+        want = [v.clone() for v in call(src.cuda(), si.cuda())]
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(_same(a, b) for a, b in zip(out, want))
